@@ -293,6 +293,40 @@ int ltq_viterbi_tb_noalloc(const float* x, const float* w, int w_stride, const f
                            int K, int m, const int* m_extra, int n_extra, int Gfull, int n_cand, int sub, int U_hi,
                            int mix, int pp, int tb_passes, int tb_cand1, int tb_window, void* stream);
 
+/*
+ * The operators at the vocabulary's ends: a teacher's top logits, the token table, the block-scaled 8-bit product.  `dtype`
+ * codes: 0 fp32, 1 bf16, 2 fp16.  Row strides (ld*) in elements; rows may start at any multiple of the element size.
+ *
+ * ltq_distill_topk: divergence of T rows of student logits [T, V] from a teacher's K top logits.  idx [T, K] (int64 when
+ *   idx64, else int32; a slot whose id is outside [0, V) is empty), teacher [T, K] their logits.  q = softmax(z /
+ *   temperature).  Without teacher_lse, p is the softmax of the live slots' logits / temperature; with it ([T], the
+ *   log-sum-exp of all the teacher's logits / temperature) p_k = exp(u_k / temperature - lse) and the remaining mass
+ *   p_r = max(0, 1 - sum p) is one outcome, against the student's mass q_r outside the slots.  weight [T] (or NULL: 1):
+ *       loss = weight (sum p (log p - log q) + p_r (log p_r - log q_r))
+ *   mode 0: loss [T], and stats [T, 2] = (log-sum-exp of z / temperature, log q_r) when not NULL; mode 1: the same and
+ *   dlogits = d loss / d logits (dtype, row stride ld_d; may be `logits` itself with ld_d = ld); mode 2: dlogits alone, from
+ *   stats, times grad[t * grad_stride] (or NULL: 1).  Terms with p = 0 are 0; a row without a live slot has loss and gradient
+ *   0, as has a row of weight 0, whose logits are not read; slots that name one token add up.  V <= 2^20, K <= 1024.
+ */
+int ltq_distill_topk(const void* logits, int dtype, long long ld, const void* idx, int idx64, long long ld_idx,
+                     const void* teacher, int teacher_dtype, long long ld_t, const float* teacher_lse,
+                     const float* weight, const float* grad, long long grad_stride, int T, int V, int K,
+                     float temperature, int mode, float* loss, float* stats, void* dlogits, long long ld_d, void* stream);
+/*
+ * ltq_embed_lookup: out [n, D] = scale * table[tokens] (table [V, D], out of its dtype; tokens int64 when tok64, else
+ *   int32; a token outside [0, V) reads as zeros).
+ * ltq_embed_grad: out [V, D] (out_dtype) = scale * sum of the rows of dout [n, D] (dtype) whose token is the row, summed in
+ *   fp32 in the order of the positions; accumulate = 1 adds to out instead (rows that no token names are not touched).
+ *   Tokens outside [0, V) and `padding` (-1: none) take no gradient.  workspace: 256-byte aligned, at least
+ *   ltq_embed_grad_workspace_bytes(n, D).  n <= 2^30, D <= 2^20.  Bit-identical from call to call.
+ */
+int ltq_embed_lookup(const void* table, int dtype, long long ld, const void* tokens, int tok64, long long n, int V,
+                     int D, float scale, void* out, long long ld_out, void* stream);
+size_t ltq_embed_grad_workspace_bytes(long long n, int D);
+int ltq_embed_grad(const void* tokens, int tok64, long long n, int V, long long padding, const void* dout, int dtype,
+                   long long ld_d, int D, float scale, void* out, int out_dtype, long long ld_out, int accumulate,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

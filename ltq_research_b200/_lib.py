@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
+from contextlib import nullcontext
 from pathlib import Path
 
 import torch
@@ -59,7 +60,15 @@ SIGNATURES = {
     # allocation-free variant (scratch inside the library): same arguments without the workspace
     "ltq_viterbi_tb_noalloc_capacity": (SZ, []),
     "ltq_viterbi_tb_noalloc": (I, [P, P, I, P, P, P, P, P, P] + [I] * 5 + [P] + [I] * 10 + [P]),
+    # operators at the vocabulary's ends
+    "ltq_distill_topk": (I, [P, I, LL, P, I, LL, P, I, LL, P, P, P, LL, I, I, I, ctypes.c_float, I, P, P, P, LL, P]),
+    "ltq_embed_lookup": (I, [P, I, LL, P, I, LL, I, I, ctypes.c_float, P, LL, P]),
+    "ltq_embed_grad_workspace_bytes": (SZ, [LL, I]),
+    "ltq_embed_grad": (I, [P, I, LL, I, LL, P, I, LL, I, ctypes.c_float, P, I, LL, I, P, SZ, P]),
 }
+
+# element type codes of the C ABI
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 class LtqLibraryError(RuntimeError):
@@ -76,6 +85,8 @@ KERNELS_PER_CALL = {
     "ltq_ldlq_inter": 1, "ltq_ldlq_inter3": 1, "ltq_bf16x6_split": 1, "ltq_bf16x6_split_batched": 1,
     "ltq_trtri256_lower": 1, "ltq_chol256_diag": 1, "lut_subs_quant": 1, "ltq_int8_rings": 1, "ltq_matvec_slice": 1,
     "ltq_pack_slice": 1, "ltq_decode_slice": 1,
+    "ltq_distill_topk": lambda a: int(a[13] > 0), "ltq_embed_lookup": lambda a: int(a[5] > 0),
+    "ltq_embed_grad": lambda a: 3 if a[2] > 8 else (2 if a[2] > 0 else int(not a[13])),
 }
 
 
@@ -151,6 +162,11 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
     if dev is None:
         raise RuntimeError("ltq_research_b200: no CUDA tensor given")
     return dev
+
+
+def on_device(device: torch.device):
+    """Context with `device` current, as a launch on its streams needs."""
+    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def ptr(t) -> int | None:

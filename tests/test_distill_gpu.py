@@ -1,0 +1,301 @@
+"""The divergence from a teacher's top logits and its gradient against their formulas in 64 bits.
+
+Tolerances.  z / tau in units of log2 is at most 64 here, so one fp32 rounding of it is 64 * 2^-24 = 4e-6, which is the
+relative error of an exponential; a sum of V / 512 positive terms adds less.  A logarithm of a probability is then good to
+1e-5, the teacher's p to 1e-5 of itself, and a loss (probabilities that sum to 1 times logarithms of at most 30) to 4e-4 at
+worst where every p errs the same way; they are normalised by the same sum, so 1e-4 stands.  The gradient is w / tau
+(q P - p): 4e-5 w / tau, and half a unit of the logits' type."""
+import math
+
+import pytest
+import torch
+
+from ltq_research_b200 import distill
+
+pytestmark = pytest.mark.gpu
+HALF_ULP = {t: torch.finfo(t).eps / 2 for t in (torch.float32, torch.bfloat16, torch.float16)}
+
+
+def plain(logits, idx, teacher, lse=None, weight=None, tau=1.0):
+    """Loss and gradient, 64 bits, row by row from the definition."""
+    T, V = logits.shape
+    z = logits.double().cpu() / tau
+    loss, grad = torch.zeros(T, dtype=torch.float64), torch.zeros(T, V, dtype=torch.float64)
+    for t in range(T):
+        w = 1.0 if weight is None else float(weight[t])
+        if w == 0.0:
+            continue
+        slots = [(int(i), float(u) / tau) for i, u in zip(idx[t].cpu(), teacher[t].double().cpu()) if 0 <= int(i) < V]
+        m = float(z[t].max())
+        e = torch.exp(z[t] - m) if m > -math.inf else torch.zeros(V, dtype=torch.float64)
+        S = float(e.sum())
+        q = e / S if S > 0 else e
+        if lse is not None:
+            p = [math.exp(u - float(lse[t])) for _, u in slots]
+        else:
+            um = max([u for _, u in slots], default=0.0)
+            p = [math.exp(u - um) if u > -math.inf else 0.0 for _, u in slots]
+            n = sum(p)
+            p = [x / n for x in p] if n > 0 else p
+        top = torch.zeros(V, dtype=torch.bool)
+        target = torch.zeros(V, dtype=torch.float64)
+        for (i, _), pk in zip(slots, p):
+            top[i] = True
+            target[i] += pk
+            if pk > 0:
+                loss[t] += w * pk * (math.log(pk) - (math.log(float(q[i])) if q[i] > 0 else -math.inf))
+        rest = max(0.0, 1.0 - sum(p)) if lse is not None and not bool(top.all()) else 0.0
+        qr = float(q[~top].sum())
+        if rest > 0:
+            loss[t] += w * rest * (math.log(rest) - (math.log(qr) if qr > 0 else -math.inf))
+        P = sum(p) + rest
+        g = q * P - target
+        if rest > 0 and qr > 0:
+            g = g - torch.where(top, torch.zeros_like(q), q * (rest / qr))
+        grad[t] = w / tau * g
+    return loss, grad
+
+
+def make(T, V, K, dtype, seed=0, rest=True, pad=0, tau=1.0):
+    g = torch.Generator().manual_seed(seed)
+    z = torch.randn(T, V, generator=g) * 2
+    z.scatter_add_(1, torch.randint(0, V, (T, 4), generator=g), 4 + 4 * torch.rand(T, 4, generator=g))
+    u_all = z + 0.5 * torch.randn(T, V, generator=g)
+    u, idx = torch.topk(u_all, K, dim=1)
+    lse = torch.logsumexp(u_all / tau, 1) if rest else None
+    buf = torch.zeros(T, V + pad, dtype=dtype, device="cuda")
+    logits = buf[:, :V]
+    logits.copy_(z)
+    return logits, idx.cuda(), u.cuda(), None if lse is None else lse.cuda()
+
+
+def check(logits, idx, teacher, lse=None, weight=None, tau=1.0, got=None):
+    want_l, want_d = plain(logits, idx, teacher, lse, weight, tau)
+    kw = dict(teacher_lse=lse, weight=weight, temperature=tau)
+    loss, d = got if got is not None else distill.topk_loss_grad(logits, idx, teacher, **kw)
+    w = (torch.ones(logits.shape[0]) if weight is None else weight.cpu()).double().abs()
+    fin = torch.isfinite(want_l)
+    assert torch.equal(torch.isfinite(loss.cpu()), fin)
+    assert torch.equal(loss.cpu()[~fin].double(), want_l[~fin])
+    assert bool(((loss.cpu().double() - want_l).abs()[fin] <= 1e-4 * w[fin]).all())
+    err = (d.double().cpu() - want_d).abs()
+    tol = 4e-5 * (w / tau)[:, None] + HALF_ULP[logits.dtype] * 1.01 * want_d.abs() + (2.0 ** -25 if logits.dtype == torch.float16 else 0)
+    assert bool((err <= tol).all()), float((err - tol).max())
+    return loss, d
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("T,V,K,pad", [(1, 1, 1, 0), (3, 5, 2, 0), (2, 31, 31, 1), (5, 1000, 17, 0), (3, 1003, 64, 0),
+                                       (4, 4099, 128, 5), (2, 20000, 300, 8), (1, 3000, 1024, 0)])
+def test_loss_and_gradient(T, V, K, pad, rest, dtype):
+    logits, idx, u, lse = make(T, V, K, dtype, seed=V + K, rest=rest, pad=pad)
+    loss, d = check(logits, idx, u, lse)
+    loss0, stats = distill.topk_loss(logits, idx, u, teacher_lse=lse)
+    assert torch.equal(loss, loss0)  # one code path
+    g = torch.linspace(-1.0, 2.0, T, device="cuda")
+    d2 = distill.topk_grad(logits, idx, u, stats, grad=g, teacher_lse=lse)
+    check(logits, idx, u, lse, weight=g, got=(loss * g, d2))
+
+
+@pytest.mark.parametrize("V", [128256, 262144])
+def test_long_rows(V):
+    logits, idx, u, lse = make(2, V, 64, torch.bfloat16, seed=V)
+    check(logits, idx, u, lse)
+    logits, idx, u, lse = make(2, V, 20, torch.float32, seed=V + 1, rest=False)
+    check(logits, idx, u, lse)
+
+
+@pytest.mark.parametrize("T", [40, 200, 700, 2500])
+def test_row_counts(T):
+    """Row counts on both sides of every choice of CTAs per row."""
+    logits, idx, u, lse = make(T, 2048 + 13, 9, torch.bfloat16, seed=T)
+    check(logits, idx, u, lse)
+
+
+@pytest.mark.parametrize("tau", [0.5, 2.0])
+def test_temperature_and_teacher_types(tau):
+    logits, idx, u, lse = make(6, 777, 12, torch.bfloat16, seed=5, tau=tau)
+    check(logits, idx, u, lse, tau=tau)
+    for dt in (torch.bfloat16, torch.float16):
+        ub = u.to(dt)
+        check(logits, idx.int(), ub, None, tau=tau)
+
+
+def test_empty_slots_and_rows():
+    logits, idx, u, lse = make(6, 500, 8, torch.float32, seed=7)
+    idx[0, 3:] = -1
+    idx[1] = -5                        # no live slot
+    idx[2, 0] = 500                    # beyond the vocabulary: empty
+    idx[3, 2] = 2 ** 40
+    u[4, 1] = -math.inf                # a slot of probability 0
+    u[5] = -math.inf
+    loss, d = check(logits, idx, u, None)
+    assert loss[1] == 0 and not d[1].any() and loss[5] == 0 and not d[5].any()
+    loss, d = check(logits[:5], idx[:5], u[:5], lse[:5])
+    assert loss[1].abs() < 1e-6
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_weights_and_masked_rows(dtype):
+    logits, idx, u, lse = make(5, 1003, 6, dtype, seed=8)
+    w = torch.tensor([0.0, 1.0, 0.25, 0.0, 3.0], device="cuda")
+    logits[0] = float("nan")
+    logits[3] = -math.inf
+    clean = logits.clone()
+    clean[0] = 0
+    want = plain(clean, idx, u, lse, w)
+    loss, d = distill.topk_loss_grad(logits, idx, u, teacher_lse=lse, weight=w)
+    assert loss[0] == 0 and loss[3] == 0 and not d[0].any() and not d[3].any()
+    assert bool(((loss.cpu().double() - want[0]).abs() <= 3e-4).all())
+    assert torch.isfinite(d).all()
+
+
+@pytest.mark.parametrize("rest", [False, True])
+def test_masked_vocabulary(rest):
+    """Tokens the student excludes: no share of the gradient; a kept one among them makes the loss infinite."""
+    logits, idx, u, lse = make(4, 900, 5, torch.float32, seed=9, rest=rest)
+    keep = torch.zeros(4, 900, dtype=torch.bool, device="cuda").scatter_(1, idx, True)
+    keep[:, ::3] = True
+    logits[~keep] = -math.inf
+    logits[1, idx[1, 0]] = -math.inf
+    logits[2] = -math.inf               # nothing left
+    logits[3] = torch.where(keep[3], logits[3], torch.finfo(torch.float32).min)
+    loss, d = check(logits, idx, u, lse)
+    assert loss[1] == math.inf and loss[2] == math.inf and torch.isfinite(d).all()
+    assert not d[0][~keep[0]].any()
+
+
+def test_student_gives_the_rest_nothing():
+    logits, idx, u, lse = make(1, 300, 4, torch.float32, seed=10)
+    rest = torch.ones(300, dtype=torch.bool, device="cuda")
+    rest[idx[0]] = False
+    logits[0, rest] = -math.inf
+    loss, d = distill.topk_loss_grad(logits, idx, u, teacher_lse=lse)
+    assert loss[0] == math.inf and torch.isfinite(d).all() and not d[0, rest].any()
+
+
+def test_nan_reaches_its_row_only():
+    logits, idx, u, lse = make(3, 700, 4, torch.bfloat16, seed=11)
+    logits[1, 690] = float("nan")
+    loss, d = distill.topk_loss_grad(logits, idx, u, teacher_lse=lse)
+    assert torch.isnan(loss[1]) and torch.isnan(d[1]).all()
+    assert torch.isfinite(loss[[0, 2]]).all() and torch.isfinite(d[[0, 2]]).all()
+
+
+@pytest.mark.parametrize("rest", [False, True])
+def test_slots_that_name_one_token(rest):
+    logits, idx, u, lse = make(3, 640, 12, torch.float32, seed=12, rest=rest)
+    idx[0, 5] = idx[0, 1]
+    idx[0, 9] = idx[0, 1]
+    idx[1, :] = 17
+    if rest:
+        lse += 1.5
+    loss, d = check(logits, idx, u, lse)
+    again = distill.topk_loss_grad(logits, idx, u, teacher_lse=lse)
+    assert torch.equal(loss, again[0]) and torch.equal(d, again[1])
+
+
+@pytest.mark.parametrize("V", [1, 7, 40])
+def test_slots_hold_every_token(V):
+    logits, idx, u, lse = make(3, V, V, torch.float32, seed=13)
+    check(logits, idx, u, lse)
+    idx2 = torch.cat([idx, idx[:, :1]], 1)
+    idx2[:, -1] = -1
+    check(logits, idx2, torch.cat([u, u[:, :1]], 1), lse)
+
+
+@pytest.mark.parametrize("off_in,off_out", [(0, 0), (1, 1), (3, 3), (1, 0), (0, 5)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_alignments(dtype, off_in, off_out):
+    T, V, K = 3, 1537, 7
+    logits, idx, u, lse = make(T, V, K, dtype, seed=14)
+    buf = torch.zeros(T * (V + 3) + 16, dtype=dtype, device="cuda")
+    view = buf[off_in:off_in + T * (V + 3)].view(T, V + 3)[:, :V]
+    view.copy_(logits)
+    obuf = torch.full((T * (V + 3) + 16,), 7.0, dtype=dtype, device="cuda")
+    out = obuf[off_out:off_out + T * (V + 3)].view(T, V + 3)[:, :V]
+    loss, d = distill.topk_loss_grad(view, idx, u, teacher_lse=lse, out=out)
+    assert d is out
+    check(logits, idx, u, lse, got=(loss, out))
+    rest = obuf.clone()
+    rest[off_out:off_out + T * (V + 3)].view(T, V + 3)[:, :V] = 7.0
+    assert (rest == 7.0).all()  # nothing is written beside the rows
+    own = distill.topk_loss_grad(view, idx, u, teacher_lse=lse)[1]
+    assert torch.equal(own, out)
+
+
+@pytest.mark.parametrize("V", [1000, 128256])
+def test_in_place(V):
+    logits, idx, u, lse = make(9, V, 8, torch.bfloat16, seed=15)
+    want = distill.topk_loss_grad(logits, idx, u, teacher_lse=lse)
+    got = distill.topk_loss_grad(logits, idx, u, teacher_lse=lse, out=logits)
+    assert got[1] is logits and torch.equal(got[0], want[0]) and torch.equal(logits, want[1])
+
+
+def test_other_stream():
+    logits, idx, u, lse = make(64, 5000, 8, torch.bfloat16, seed=16)
+    want = distill.topk_loss_grad(logits, idx, u, teacher_lse=lse)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = distill.topk_loss_grad(logits, idx, u, teacher_lse=lse)
+    s.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("rest", [False, True])
+def test_gradient_against_differences(rest):
+    """Central differences of the kernel's own loss: h = 0.05 along a random direction; the third derivative along a unit
+    direction is below 1, so h^2 / 6 = 4e-4, and 1e-5 / h = 2e-4 from the losses' rounding."""
+    logits, idx, u, lse = make(8, 400, 6, torch.float32, seed=17, rest=rest)
+    v = torch.randn(8, 400, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    v[torch.arange(8), idx[:, 0]] += 5.0
+    v = v / v.norm(dim=1, keepdim=True)
+    d = distill.topk_loss_grad(logits, idx, u, teacher_lse=lse)[1]
+    h = 0.05
+    up = distill.topk_loss(logits + h * v, idx, u, teacher_lse=lse)[0]
+    dn = distill.topk_loss(logits - h * v, idx, u, teacher_lse=lse)[0]
+    assert ((up - dn) / (2 * h) - (d * v).sum(1)).abs().max() < 1e-3
+
+
+def test_autograd():
+    logits, idx, u, lse = make(7, 600, 5, torch.float32, seed=18)
+    z = logits.clone().requires_grad_()
+    w = torch.linspace(0, 2, 7, device="cuda")
+    loss = distill.distill_loss(z, idx, u, teacher_lse=lse, weight=w)
+    loss.mean().backward()
+    want = distill.topk_loss_grad(logits, idx, u, teacher_lse=lse, weight=w / 7)[1]
+    assert (z.grad - want).abs().max() < 1e-6
+
+
+def test_no_rows():
+    loss, d = distill.topk_loss_grad(torch.empty(0, 9, device="cuda"), torch.empty(0, 2, dtype=torch.int64, device="cuda"),
+                                     torch.empty(0, 2, device="cuda"))
+    assert loss.shape == (0,) and d.shape == (0, 9)
+
+
+def test_refusals():
+    logits, idx, u, lse = make(4, 100, 5, torch.float32, seed=19)
+    f = distill.topk_loss_grad
+    for bad in [dict(logits=logits.double()), dict(idx=idx.float()), dict(u=u.double())]:
+        a = dict(logits=logits, idx=idx, u=u) | bad
+        with pytest.raises(TypeError):
+            f(a["logits"], a["idx"], a["u"])
+    for bad in [dict(logits=logits[:3]), dict(idx=idx[:, :4]), dict(logits=logits.t()), dict(logits=logits[:1].expand(4, 100)),
+                dict(logits=logits[0]), dict(idx=idx[:, :0], u=u[:, :0])]:
+        a = dict(logits=logits, idx=idx, u=u) | bad
+        with pytest.raises(ValueError):
+            f(a["logits"], a["idx"], a["u"])
+    for kw in [dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=float("nan")), dict(weight=lse[:2]),
+               dict(weight=lse.double()), dict(teacher_lse=lse[:, None]), dict(out=logits.half()), dict(out=logits[:, 1:])]:
+        with pytest.raises(ValueError):
+            f(logits, idx, u, **kw)
+    wide = torch.zeros(5, 100, device="cuda")
+    with pytest.raises(ValueError):  # overlaps the logits without being them
+        f(wide[:4], idx, u, out=wide[1:])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        f(logits.cpu(), idx, u)
+    with pytest.raises(ValueError):
+        f(torch.zeros(1, 1100, device="cuda"), torch.zeros(1, 1025, dtype=torch.int64, device="cuda"),
+          torch.zeros(1, 1025, device="cuda"))
