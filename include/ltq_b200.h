@@ -326,6 +326,23 @@ size_t ltq_embed_grad_workspace_bytes(long long n, int D);
 int ltq_embed_grad(const void* tokens, int tok64, long long n, int V, long long padding, const void* dout, int dtype,
                    long long ld_d, int D, float scale, void* out, int out_dtype, long long ld_out, int accumulate,
                    void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * Products in 8-bit floating point (e4m3) with a scale per block of 128.  scale = max |block| / 448, at least 2^-126; a block
+ * with a NaN or an infinity becomes NaN.  Rows of 8-bit operands: 16-byte aligned, strides multiples of 16.
+ * ltq_fp8_quant_rows: x [M, K] -> q [M, K] and one scale per row and 128 columns, s[b * ld_s + m].
+ * ltq_fp8_quant_blocks: w [N, K] -> q [N, K] and one scale per 128 x 128 block, s[nb * ld_s + b].
+ * ltq_fp8_gemm: C[m, n] = sum_b sa[b * ld_sa + m] sb[(n / 128) * ld_sb + b] sum_{k in block b} A[m, k] B[n, k], C of `dtype`
+ *   with row stride ldc.  sa 16-byte aligned, ld_sa a multiple of 4 and at least M.  workspace: 256-byte aligned, at least
+ *   ltq_fp8_gemm_workspace_bytes(M, N, K).  err as for ltq_gemm_bf16_tn.  Bit-identical from call to call.
+ */
+int ltq_fp8_quant_rows(const void* x, int dtype, long long ld, int M, int K, uint8_t* q, long long ld_q, float* s,
+                       long long ld_s, void* stream);
+int ltq_fp8_quant_blocks(const void* w, int dtype, long long ld, int N, int K, uint8_t* q, long long ld_q, float* s,
+                         long long ld_s, void* stream);
+size_t ltq_fp8_gemm_workspace_bytes(int M, int N, int K);
+int ltq_fp8_gemm(const uint8_t* A, long long lda, const float* sa, long long ld_sa, const uint8_t* B, long long ldb,
+                 const float* sb, long long ld_sb, void* C, int dtype, long long ldc, int M, int N, int K,
+                 void* workspace, size_t workspace_bytes, int* err, void* stream);
 
 #ifdef __cplusplus
 }

@@ -65,6 +65,10 @@ SIGNATURES = {
     "ltq_embed_lookup": (I, [P, I, LL, P, I, LL, I, I, ctypes.c_float, P, LL, P]),
     "ltq_embed_grad_workspace_bytes": (SZ, [LL, I]),
     "ltq_embed_grad": (I, [P, I, LL, I, LL, P, I, LL, I, ctypes.c_float, P, I, LL, I, P, SZ, P]),
+    "ltq_fp8_quant_rows": (I, [P, I, LL, I, I, P, LL, P, LL, P]),
+    "ltq_fp8_quant_blocks": (I, [P, I, LL, I, I, P, LL, P, LL, P]),
+    "ltq_fp8_gemm_workspace_bytes": (SZ, [I, I, I]),
+    "ltq_fp8_gemm": (I, [P, LL, P, LL, P, LL, P, LL, P, I, LL, I, I, I, P, SZ, P, P]),
 }
 
 # element type codes of the C ABI
@@ -87,6 +91,8 @@ KERNELS_PER_CALL = {
     "ltq_pack_slice": 1, "ltq_decode_slice": 1,
     "ltq_distill_topk": lambda a: int(a[13] > 0), "ltq_embed_lookup": lambda a: int(a[5] > 0),
     "ltq_embed_grad": lambda a: 3 if a[2] > 8 else (2 if a[2] > 0 else int(not a[13])),
+    "ltq_fp8_quant_rows": lambda a: int(a[3] > 0), "ltq_fp8_quant_blocks": lambda a: int(a[3] > 0),
+    "ltq_fp8_gemm": lambda a: int(a[11] > 0 and a[12] > 0),
 }
 
 
