@@ -1,9 +1,8 @@
-// Products in 8-bit floating point (e4m3) with a scale for each block of 128 (B200, sm_100a).
+// Quantization to 8-bit floating point (e4m3) with a scale for each block of 128 (B200, sm_100a); the products are in
+// ltq_fp8_gemm.cu.
 //
-// Quantization of 128 values: s = max |x| / 448 (at least 2^-126), q = e4m3(x / s), round to nearest even; a block with a
+// 128 values: s = max |x| / 448 (at least 2^-126), q = e4m3(x / s), an fp32 quotient rounded to nearest even; a block with a
 // NaN or an infinity becomes NaN.  Activations: one scale per row and 128 columns; weights: one per 128 x 128 block.
-//     y[m, n] = sum_b sa[m, b] sw[n / 128, b] (sum over block b of qa[m, k] qw[n, k])
-// Each block's sum is taken in fp32 and joined with its scales in fp32.
 #include <cuda_fp8.h>
 #include "ltq_b200.h"
 #include "vec_types.cuh"
@@ -90,61 +89,6 @@ __global__ void __launch_bounds__(256) quant_blocks_kernel(const T* __restrict__
     if (threadIdx.x == 0) s[blockIdx.y * ld_s + blockIdx.x] = sc;
 }
 
-struct GemmArgs {
-    const uint8_t* A;
-    long long lda;
-    const float* sa;  // [block][M], block stride ld_sa
-    long long ld_sa;
-    const uint8_t* B;
-    long long ldb;
-    const float* sb;  // [N / 128][block], row stride ld_sb
-    long long ld_sb;
-    void* C;
-    long long ldc;
-    int M, N, K;
-};
-
-__device__ __forceinline__ float e4m3(uint8_t v)
-{
-    const __half_raw h = __nv_cvt_fp8_to_halfraw(v, __NV_E4M3);
-    return __half2float(*reinterpret_cast<const __half*>(&h));
-}
-
-// 64 x 64 tiles, 16 columns of K at a time through shared memory
-template <typename T>
-__global__ void __launch_bounds__(256) gemm_simple_kernel(const GemmArgs g)
-{
-    __shared__ float a[16][65], b[16][65];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < g.K; k0 += QB) {
-        float part[4][4] = {};
-        const int ke = min(g.K, k0 + QB);
-        for (int k = k0; k < ke; k += 16) {
-            for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-                const int r = i >> 4, c = i & 15;
-                a[c][r] = m0 + r < g.M && k + c < ke ? e4m3(g.A[(long long)(m0 + r) * g.lda + k + c]) : 0.f;
-                b[c][r] = n0 + r < g.N && k + c < ke ? e4m3(g.B[(long long)(n0 + r) * g.ldb + k + c]) : 0.f;
-            }
-            __syncthreads();
-            for (int c = 0; c < 16; c++)
-                for (int i = 0; i < 4; i++)
-                    for (int j = 0; j < 4; j++) part[i][j] = fmaf(a[c][ty * 4 + i], b[c][tx * 4 + j], part[i][j]);
-            __syncthreads();
-        }
-        const float sb = g.sb[(n0 / QB) * g.ld_sb + k0 / QB];
-        for (int i = 0; i < 4; i++) {
-            const float s = m0 + ty * 4 + i < g.M ? g.sa[k0 / QB * g.ld_sa + m0 + ty * 4 + i] * sb : 0.f;
-            for (int j = 0; j < 4; j++) acc[i][j] = fmaf(s, part[i][j], acc[i][j]);
-        }
-    }
-    for (int i = 0; i < 4; i++)
-        for (int j = 0; j < 4; j++) {
-            const int m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (m < g.M && n < g.N) ((T*)g.C)[(long long)m * g.ldc + n] = from_f<T>(acc[i][j]);
-        }
-}
-
 template <typename T>
 int quant_rows(const void* x, long long ld, int M, int K, uint8_t* q, long long ld_q, float* s, long long ld_s, cudaStream_t st)
 {
@@ -161,8 +105,6 @@ int quant_blocks(const void* w, long long ld, int N, int K, uint8_t* q, long lon
     quant_blocks_kernel<T><<<grid, 256, 0, st>>>((const T*)w, ld, N, K, q, ld_q, s, ld_s, aligned);
     return (int)cudaGetLastError();
 }
-
-bool bad_operand(const void* q, long long ld, int K) { return !q || (uintptr_t)q % 16 || ld % 16 || ld < K; }
 
 }  // namespace
 
@@ -191,25 +133,4 @@ extern "C" int ltq_fp8_quant_blocks(const void* w, int dtype, long long ld, int 
     if (dtype == DT_F32) return quant_blocks<float>(w, ld, N, K, q, ld_q, s, ld_s, st);
     if (dtype == DT_BF16) return quant_blocks<__nv_bfloat16>(w, ld, N, K, q, ld_q, s, ld_s, st);
     return quant_blocks<__half>(w, ld, N, K, q, ld_q, s, ld_s, st);
-}
-
-extern "C" size_t ltq_fp8_gemm_workspace_bytes(int M, int N, int K) { return 0; }
-
-extern "C" int ltq_fp8_gemm(const uint8_t* A, long long lda, const float* sa, long long ld_sa, const uint8_t* B, long long ldb,
-                            const float* sb, long long ld_sb, void* C, int dtype, long long ldc, int M, int N, int K,
-                            void* workspace, size_t workspace_bytes, int* err, void* stream)
-{
-    const int es = dt_bytes(dtype);
-    if (!es || M < 0 || N < 0 || K < 1 || ldc < N || ld_sa < M || ld_sa % 4 || ld_sb < (K + QB - 1) / QB) return -1;
-    if (M == 0 || N == 0) return 0;
-    if (bad_operand(A, lda, K) || bad_operand(B, ldb, K) || !sa || (uintptr_t)sa % 16 || !sb || (uintptr_t)sb % 4 || !C ||
-        (uintptr_t)C % es || M > 65535 * 64)
-        return -1;
-    const GemmArgs g{A, lda, sa, ld_sa, B, ldb, sb, ld_sb, C, ldc, M, N, K};
-    const dim3 grid((N + 63) / 64, (M + 63) / 64);
-    const cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == DT_F32) gemm_simple_kernel<float><<<grid, 256, 0, st>>>(g);
-    else if (dtype == DT_BF16) gemm_simple_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(g);
-    else gemm_simple_kernel<__half><<<grid, 256, 0, st>>>(g);
-    return (int)cudaGetLastError();
 }

@@ -1,0 +1,495 @@
+// Block-scaled products of e4m3 operands on the tensor cores (B200, sm_100a): tcgen05.mma kind::f8f6f4, TMA operand loads,
+// the partial sums of each block of 128 joined under their scales in registers.
+//
+//     C[m, n] = sum_b sa[m, b] sb[n / 128, b] P_b[m, n],   P_b = sum over block b of A[m, k] B[n, k]
+//
+// The scales change from block to block of K, so tensor memory holds only the sum P_b of one block and the epilogue warps
+// read it back, multiply and add it to fp32 registers while the next block's product runs into the other half of tensor
+// memory.  A pair of CTAs works on a 256 x 256 tile (cta_group::2: each loads 128 rows of A and 128 of B and holds 128 rows
+// of the sums): per block 32 KB of operands a CTA for 2 * 128^2 * 256 operations, 64 bytes a clock of L2 reads an SM at full rate,
+// where one CTA with a 128 x 256 tile would need 96.
+//
+//   warp 8        lane 0: TMA producer, A and B blocks into a ring of W_STAGES buffers (128-byte swizzle) on both CTAs; the
+//                 bytes of both are counted on the first CTA's "full" mbarrier
+//   warp 9        lane 0 of the first CTA: four tcgen05.mma (K 32 each) a block; tcgen05.commit frees the buffers of both CTAs
+//                 and hands the sum to both CTAs' epilogue warps
+//   warps 0 .. 7  epilogue: lanes' quarter w % 4 of the rows, half w / 4 of the columns, 128 sums a thread
+//
+// Pairs walk the tiles (rows first, so that neighbours share B in L2).  What is left after the last full round of tiles is cut
+// along K into equal shares (a share may end inside a tile); the parts go to a workspace and join_parts_kernel adds them in the
+// order of K.  Every wait is bounded: when one runs out *err is set, the role stops and the CTAs still meet at their last barrier.
+#include "ltq_b200.h"
+#include "tc_pipe.cuh"
+#include "vec_types.cuh"
+
+namespace {
+
+constexpr int QB = 128;  // K block: the width of a scale
+constexpr uint32_t WAIT_LIMIT = 1u << 24;
+
+// ------------------------------------------------------------------------------------------------ cta_group::2 pieces
+
+__device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank)
+{
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t addr)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(addr) : "memory");
+}
+__device__ __forceinline__ bool wait_cluster(uint64_t* b, uint32_t parity, int* err)
+{
+    for (uint32_t i = 0; i < WAIT_LIMIT; i++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(ok)
+            : "r"(smem_u32(b)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+    }
+    if (err) atomicExch(err, 1);
+    return false;
+}
+// the copy lands in this CTA's shared memory, its bytes are counted on the mbarrier at `bar` (of either CTA of the pair)
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint64_t* bar)  // arrives on both CTAs' mbarriers at this address
+{
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+// instruction descriptor, kind::f8f6f4: D fp32 (bits 4-5 = 1), A and B e4m3 (bits 7-9, 10-12 = 0), both K-major
+__host__ __device__ constexpr uint32_t idesc_f8(int m, int n)
+{
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void mma_f8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld16_issue(uint32_t taddr, uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+// waits for the reads issued so far; the registers pass through, so that no use of them moves above the wait
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y)
+{
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(map), "r"(smem_u32(src)),
+                 "r"(x), "r"(y)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+}
+
+// --------------------------------------------------------------------------------------------------- the wide kernel
+
+constexpr int WT = 256;                                  // tile of a pair, both ways
+constexpr int W_STAGES = 6;
+constexpr int W_OP = 128 * QB, W_STAGE = 2 * W_OP;       // one operand's block of a CTA: 16 KB
+constexpr int W_THREADS = 384;
+// registers a thread: 168 at launch (384 x 168 = 64512 of the SM's 65536); the epilogue's eight warps take 232, the others keep 40
+constexpr int W_REGS_EPILOGUE = 232, W_REGS_ROLES = 40;
+static_assert(256 * W_REGS_EPILOGUE + 128 * W_REGS_ROLES <= W_THREADS * 168, "the shares fit the launch's registers");
+constexpr int W_STORE = 4096;                            // staging of an epilogue warp: a 32-row box of 128 bytes
+constexpr int W_SMEM = W_STAGES * W_STAGE + 8 * W_STORE + 256 + 1024;
+static_assert(W_SMEM <= 232448, "shared memory of one CTA");
+constexpr int PART_FLOATS = 128 * WT;                    // a CTA's rows of a partial tile
+
+struct WideArgs {
+    const float* sa;
+    long long ld_sa;
+    const float* sb;
+    long long ld_sb;
+    void* C;
+    long long ldc;
+    float* parts;  // [pair][2][CTA][column / 4][row][4]
+    int* err;
+    int M, N, nkb, mt, whole, tma_c;  // whole: tiles done in one piece
+    long long shared_units;           // blocks of K of the tiles after them,
+    int sharers;                      // shared equally by the first `sharers` pairs (at least one block each)
+};
+
+struct Segment {
+    int tile, k0, k1;
+};
+// the pieces of work of pair c of G, in order
+struct Walk {
+    int c, G, nkb, whole, t;
+    long long u, u1;
+    __device__ Walk(const WideArgs& g, int c_, int G_)
+        : c(c_), G(G_), nkb(g.nkb), whole(g.whole), t(c_), u(0), u1(0)
+    {
+        if (c < g.sharers) u = g.shared_units * c / g.sharers, u1 = g.shared_units * (c + 1) / g.sharers;
+    }
+    __device__ bool next(Segment& s)
+    {
+        if (t < whole) {
+            s = {t, 0, nkb};
+            t += G;
+            return true;
+        }
+        if (u >= u1) return false;
+        const int k0 = (int)(u % nkb);
+        const long long left = u1 - u;
+        s = {whole + (int)(u / nkb), k0, left < nkb - k0 ? k0 + (int)left : nkb};
+        u += s.k1 - s.k0;
+        return true;
+    }
+};
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
+    gemm_wide_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                     const __grid_constant__ CUtensorMap tmC, const WideArgs g)
+{
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* store = smem + W_STAGES * W_STAGE;
+    uint64_t* full = reinterpret_cast<uint64_t*>(store + 8 * W_STORE);
+    uint64_t* empty = full + W_STAGES;
+    uint64_t* accfull = empty + W_STAGES;
+    uint64_t* accempty = accfull + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accempty + 2);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < W_STAGES; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&accfull[i], 1);
+            mbar_init(&accempty[i], 16);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 8) {
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];\n" ::"l"(&tmA) : "memory");
+            asm volatile("prefetch.tensormap [%0];\n" ::"l"(&tmB) : "memory");
+        }
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_slot)), "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(W_REGS_ROLES));
+        if (warp == 8 && lane == 0) {
+            Walk walk(g, pair, npairs);
+            Segment s;
+            int i = 0;
+            bool ok = true;
+            while (ok && walk.next(s)) {
+                const int m0 = (s.tile % g.mt) * WT + rank * 128, n0 = (s.tile / g.mt) * WT + rank * 128;
+                for (int k = s.k0; k < s.k1; k++, i++) {
+                    const int st = i % W_STAGES;
+                    if (i >= W_STAGES && !wait_cluster(&empty[st], (i / W_STAGES - 1) & 1, g.err)) {
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0) mbar_expect_tx(&full[st], 2 * W_STAGE);  // both CTAs' bytes
+                    const uint32_t bar = map_rank(&full[st], 0);
+                    tma_load_2d_pair(smem + st * W_STAGE, &tmA, k * QB, m0, bar);
+                    tma_load_2d_pair(smem + st * W_STAGE + W_OP, &tmB, k * QB, n0, bar);
+                }
+            }
+            // a buffer is free again once its copies have landed and been read: none is in flight when the CTA leaves
+            for (int j = i > W_STAGES ? i - W_STAGES : 0; j < i; j++) wait_cluster(&empty[j % W_STAGES], (j / W_STAGES) & 1, g.err);
+        }
+        if (warp == 9 && rank == 0 && lane == 0) {
+            Walk walk(g, pair, npairs);
+            Segment s;
+            constexpr uint32_t ID = idesc_f8(256, WT);
+            int i = 0;
+            bool ok = true;
+            while (ok && walk.next(s))
+                for (int k = s.k0; k < s.k1; k++, i++) {
+                    const int st = i % W_STAGES, buf = i & 1;
+                    if ((i >= 2 && !wait_cluster(&accempty[buf], (i / 2 - 1) & 1, g.err)) ||
+                        !wait_cluster(&full[st], (i / W_STAGES) & 1, g.err)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a = smem_u32(smem + st * W_STAGE), b = a + W_OP, d = tmem + buf * WT;
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++)
+                        mma_f8_pair(d, sw128_kmajor_desc(a + 32 * kk), sw128_kmajor_desc(b + 32 * kk), ID, kk != 0);
+                    commit_pair(&empty[st]);
+                    commit_pair(&accfull[buf]);
+                }
+        }
+        __syncwarp();
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(W_REGS_EPILOGUE));
+        Walk walk(g, pair, npairs);
+        Segment s;
+        constexpr int BOX = 128 / sizeof(T);  // columns of a store box
+        const int quarter = warp & 3, half = warp >> 2;
+        uint8_t* box = store + warp * W_STORE;
+        const uint32_t lane_base = tmem + ((uint32_t)(32 * quarter) << 16) + half * 128;
+        const uint32_t free_bar[2] = {map_rank(&accempty[0], 0), map_rank(&accempty[1], 0)};
+        int i = 0;
+        bool ok = true;
+        while (ok && walk.next(s)) {
+            const int m0 = (s.tile % g.mt) * WT + rank * 128 + 32 * quarter, m = m0 + lane;
+            const int n0 = (s.tile / g.mt) * WT + half * 128;
+            const bool live = m < g.M && n0 < g.N;
+            const float* pa = g.sa + m;
+            const float* pb = g.sb + (long long)(n0 / QB) * g.ld_sb;
+            float acc[128];
+#pragma unroll
+            for (int j = 0; j < 128; j++) acc[j] = 0.f;
+            float sc = live ? pa[s.k0 * g.ld_sa] * pb[s.k0] : 0.f;
+            for (int k = s.k0; k < s.k1; k++, i++) {
+                const int buf = i & 1;
+                const float next = live && k + 1 < s.k1 ? pa[(k + 1) * g.ld_sa] * pb[k + 1] : 0.f;
+                ok = wait_cluster(&accfull[buf], (i / 2) & 1, g.err);
+                __syncwarp();
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t t = lane_base + buf * WT;
+                uint32_t r[2][16];
+                tmem_ld16_issue(t, r[0]);
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    tmem_ld_wait(r[c & 1]);
+                    if (c < 7) tmem_ld16_issue(t + 16 * (c + 1), r[(c + 1) & 1]);
+                    else {  // the sums are in registers: the buffer goes back to the MMAs
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) arrive_cluster(free_bar[buf]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; j++) acc[16 * c + j] = fmaf(__uint_as_float(r[c & 1][j]), sc, acc[16 * c + j]);
+                }
+                sc = next;
+            }
+            if (!ok) break;
+            if (s.k0 != 0 || s.k1 != g.nkb) {  // a part of the tile's sum
+                float* part = g.parts + (((long long)pair * 2 + (s.k0 ? 0 : 1)) * 2 + rank) * PART_FLOATS;
+#pragma unroll
+                for (int c = 0; c < 32; c++)
+                    *reinterpret_cast<float4*>(part + ((half * 32 + c) * 128 + 32 * quarter + lane) * 4) =
+                        make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
+                continue;
+            }
+#pragma unroll
+            for (int c = 0; c < 128; c += BOX) {
+                if (n0 + c >= g.N || m0 >= g.M) break;  // warp-uniform
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
+                __syncwarp();
+#pragma unroll
+                for (int q = 0; q < 8; q++) {
+                    float v[16 / sizeof(T)];
+#pragma unroll
+                    for (int e = 0; e < 16 / (int)sizeof(T); e++) v[e] = acc[c + q * (16 / sizeof(T)) + e];
+                    *reinterpret_cast<uint4*>(box + lane * 128 + ((q ^ (lane & 7)) << 4)) = pack16(v, T());
+                }
+                if (g.tma_c) {
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) tma_store_2d(&tmC, box, n0 + c, m0);
+                } else {  // rows that TMA cannot address: element by element, a row at a time
+                    __syncwarp();
+                    for (int r = 0; r < 32 && m0 + r < g.M; r++)
+                        for (int e = lane; e < BOX && n0 + c + e < g.N; e += 32)
+                            ((T*)g.C)[(long long)(m0 + r) * g.ldc + n0 + c + e] = *reinterpret_cast<const T*>(
+                                box + r * 128 + (((e * (int)sizeof(T) / 16) ^ (r & 7)) << 4) + e * sizeof(T) % 16);
+                    __syncwarp();
+                }
+            }
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+    if (warp == 8) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// tiles whose K was cut: the parts of 32 rows of a CTA's half, summed in the order of K
+template <typename T>
+__global__ void __launch_bounds__(256) join_parts_kernel(const WideArgs g)
+{
+    __shared__ float rows[32][WT + 1];
+    const int tile = g.whole + blockIdx.x, rank = blockIdx.y >> 2, r0 = (blockIdx.y & 3) * 32;
+    const int m0 = (tile % g.mt) * WT + rank * 128 + r0, n0 = (tile / g.mt) * WT;
+    if (m0 >= g.M) return;
+    const long long a = (long long)blockIdx.x * g.nkb, b = a + g.nkb, U = g.shared_units;
+    const int npairs = g.sharers;
+    int c0 = (int)(a * npairs / U);  // the pair whose share holds block a, or the one before it
+    while (U * (c0 + 1) / npairs <= a) c0++;
+    if (U * c0 / npairs <= a && U * (c0 + 1) / npairs >= b) return;  // one pair did all of the tile
+    const int r = threadIdx.x & 31;
+    for (int c4 = threadIdx.x >> 5; c4 < WT / 4; c4 += 8) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = c0; c < npairs && U * c / npairs < b; c++) {
+            // a share that begins inside the tile left part 0, one that begins at its first block or before it part 1
+            const long long u0 = U * c / npairs;
+            const int slot = u0 > a ? 0 : 1;
+            const float4 x = *reinterpret_cast<const float4*>(
+                g.parts + (((long long)c * 2 + slot) * 2 + rank) * PART_FLOATS + ((long long)c4 * 128 + r0 + r) * 4);
+            v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+        }
+        rows[r][4 * c4] = v.x, rows[r][4 * c4 + 1] = v.y, rows[r][4 * c4 + 2] = v.z, rows[r][4 * c4 + 3] = v.w;
+    }
+    __syncthreads();
+    for (int q = threadIdx.x >> 5; q < 32 && m0 + q < g.M; q += 8)
+        for (int e = threadIdx.x & 31; e < WT && n0 + e < g.N; e += 32)
+            ((T*)g.C)[(long long)(m0 + q) * g.ldc + n0 + e] = from_f<T>(rows[q][e]);
+}
+
+// ---------------------------------------------------------------------------------------------------------- host side
+
+bool make_map_8(CUtensorMap* m, const void* base, long long rows, long long cols, long long ld, int box_rows)
+{
+    auto f = encode_fn();
+    if (!f) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld};
+    cuuint32_t box[2] = {QB, (cuuint32_t)box_rows}, one[2] = {1, 1};
+    return f(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool make_map_out(CUtensorMap* m, void* base, int es, long long rows, long long cols, long long ld)
+{
+    auto f = encode_fn();
+    if (!f) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)(ld * es)};
+    cuuint32_t box[2] = {(cuuint32_t)(128 / es), 32}, one[2] = {1, 1};
+    return f(m, es == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, dims, strides, box, one,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int sm_count()
+{
+    static std::atomic<int> n[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    int v = n[dev].load(std::memory_order_relaxed);
+    if (!v) {
+        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+        n[dev].store(v, std::memory_order_relaxed);
+    }
+    return v;
+}
+
+struct WidePlan {
+    int mt, tiles, nkb, pairs, whole, sharers;
+    long long shared_units;
+    size_t workspace;
+};
+// Whole tiles in rounds of one per pair; the tiles of a last round that would leave pairs idle are shared along K when that
+// saves more than the parts cost (their traffic and a launch, about 10 us; a block of K takes 0.27 us).
+WidePlan plan_wide(int M, int N, int K, int sms)
+{
+    WidePlan p{};
+    p.mt = (M + WT - 1) / WT;
+    p.tiles = p.mt * ((N + WT - 1) / WT);
+    p.nkb = (K + QB - 1) / QB;
+    p.pairs = sms / 2 > 0 ? sms / 2 : 1;
+    const int rest = p.tiles % p.pairs;
+    const bool share = rest && (double)(p.pairs - rest) / p.pairs * p.nkb * 0.27 > 10.0;
+    p.whole = share ? p.tiles - rest : p.tiles;
+    p.shared_units = (long long)(p.tiles - p.whole) * p.nkb;
+    p.sharers = (int)(p.shared_units / 4 < p.pairs ? (p.shared_units + 3) / 4 : p.pairs);  // at least about four blocks each
+    const int busy = p.whole < p.sharers ? p.sharers : p.whole;
+    if (busy < p.pairs) p.pairs = busy;
+    p.workspace = (size_t)p.sharers * 4 * PART_FLOATS * 4;
+    return p;
+}
+
+template <typename T>
+int run_wide(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const WideArgs& g, const WidePlan& p, cudaStream_t st)
+{
+    static std::atomic<int> ready[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+    if (!ready[dev].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(gemm_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, W_SMEM);
+        if (e != cudaSuccess) return (int)e;
+        ready[dev].store(1, std::memory_order_release);
+    }
+    gemm_wide_kernel<T><<<2 * p.pairs, W_THREADS, W_SMEM, st>>>(ta, tb, tc, g);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || p.whole == p.tiles) return (int)e;
+    join_parts_kernel<T><<<dim3(p.tiles - p.whole, 8), 256, 0, st>>>(g);
+    return (int)cudaGetLastError();
+}
+
+bool bad_operand(const void* q, long long ld, int K) { return !q || (uintptr_t)q % 16 || ld % 16 || ld < K; }
+
+}  // namespace
+
+extern "C" size_t ltq_fp8_gemm_workspace_bytes(int M, int N, int K)
+{
+    if (M < 1 || N < 1 || K < 1) return 0;
+    return plan_wide(M, N, K, sm_count()).workspace;
+}
+
+extern "C" int ltq_fp8_gemm(const uint8_t* A, long long lda, const float* sa, long long ld_sa, const uint8_t* B, long long ldb,
+                            const float* sb, long long ld_sb, void* C, int dtype, long long ldc, int M, int N, int K,
+                            void* workspace, size_t workspace_bytes, int* err, void* stream)
+{
+    const int es = dt_bytes(dtype);
+    if (!es || M < 0 || N < 0 || K < 1 || ldc < N || ld_sa < M || ld_sa % 4 || ld_sb < (K + QB - 1) / QB) return -1;
+    if (M == 0 || N == 0) return 0;
+    if (bad_operand(A, lda, K) || bad_operand(B, ldb, K) || !sa || (uintptr_t)sa % 16 || !sb || (uintptr_t)sb % 4 || !C ||
+        (uintptr_t)C % es || K > 0x7fffffff - QB || (long long)((M + WT - 1LL) / WT) * ((N + WT - 1LL) / WT) > 0x3fffffff)
+        return -1;
+    const WidePlan p = plan_wide(M, N, K, sm_count());
+    if (p.workspace && (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < p.workspace)) return -1;
+    CUtensorMap ta, tb, tc{};
+    if (!make_map_8(&ta, A, M, K, lda, 128) || !make_map_8(&tb, B, N, K, ldb, 128)) return -1;
+    const int tma_c = (uintptr_t)C % 16 == 0 && ldc * es % 16 == 0;
+    if (tma_c && !make_map_out(&tc, C, es, M, N, ldc)) return -1;
+    const WideArgs g{sa, ld_sa, sb, ld_sb, C, ldc, (float*)workspace, err, M, N, p.nkb, p.mt, p.whole, tma_c, p.shared_units, p.sharers};
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == DT_F32) return run_wide<float>(ta, tb, tc, g, p, st);
+    if (dtype == DT_BF16) return run_wide<__nv_bfloat16>(ta, tb, tc, g, p, st);
+    return run_wide<__half>(ta, tb, tc, g, p, st);
+}

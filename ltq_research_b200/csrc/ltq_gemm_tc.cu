@@ -23,12 +23,11 @@
 // Every wait on an mbarrier is bounded: after GEMM_WAIT_LIMIT polls the thread records a timeout in *err (when given)
 // and leaves its loop; the CTA still meets at its final barrier and frees its tensor memory.  No cluster, no multicast:
 // every TMA load reads this GPU's own memory.
-#include <cuda.h>
-#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <atomic>
 #include "ltq_b200.h"
+#include "tc_pipe.cuh"
 
 namespace {
 
@@ -47,7 +46,6 @@ constexpr int B_BYTES = BN * BK * 2;            // 32 KB
 constexpr int STAGE_BYTES = A_BYTES + B_BYTES;  // 48 KB, a multiple of the 1024-byte swizzle atom
 // two stages (97 KB of shared memory) let two CTAs share an SM, which measured faster than three stages at one CTA
 constexpr int TMEM_COLS = BN;  // a power of two >= 32
-constexpr uint32_t GEMM_WAIT_LIMIT = 1u << 26;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /* alignment */ + 256 /* barriers */;
 static_assert(4 * 32 * ((BN < 128 ? BN : 128) + 4) * 4 <= STAGES * STAGE_BYTES, "epilogue staging exceeds the buffers");
 
@@ -58,35 +56,6 @@ struct GemmParams {
     float alpha, beta;
     int* err;
 };
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(uint64_t* b, uint32_t count)
-{
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(smem_u32(b)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* b, uint32_t bytes)
-{
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint64_t* b, uint32_t parity)
-{
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(b)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// bounded wait for the phase with parity `parity`; false after `limit` polls (the timeout is recorded in *err)
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, int* err, uint32_t limit = GEMM_WAIT_LIMIT)
-{
-    for (uint32_t i = 0; i < limit; i++)
-        if (mbar_try_wait(b, parity)) return true;
-    if (err) atomicExch(err, 1);
-    return false;
-}
 
 // Self-test of the bounded wait: one thread waits on a fresh mbarrier that expects one arrival; with arrive = 1 the
 // arrival is made first and the wait completes (*done = 1), with arrive = 0 nothing arrives and the wait gives up after
@@ -102,34 +71,6 @@ __global__ void gemm_wait_selftest_kernel(int arrive, uint32_t limit, int* err, 
     }
 }
 
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar)
-{
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
-            smem_u32(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-        : "memory");
-}
-
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar)
-{
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(
-            smem_u32(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
-        : "memory");
-}
-
-// shared-memory matrix descriptor (tcgen05): K-major tile of rows x 64 bf16 with the 128-byte swizzle, as TMA writes it:
-// 8-row atoms of 1024 bytes one after the other (stride byte offset 1024), the second 16-byte column chunk adjacent
-// (leading byte offset 16), descriptor version 1, layout 2 (128-byte swizzle).  `addr` may step through the atom's
-// row in 32-byte units (one K = 16 slice of bf16), the hardware applying the swizzle to the computed address.
-__device__ __forceinline__ uint64_t sw128_kmajor_desc(uint32_t addr)
-{
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-
 // instruction descriptor, kind::f16: D fp32 (bits 4-5 = 1), A and B bf16 (bits 7-9, 10-12 = 1), both K-major
 // (bits 15, 16 = 0), N >> 3 at bits 17-22, M >> 4 at bits 24-28
 constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
@@ -142,28 +83,6 @@ __device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t a_desc, uint
         "l"(a_desc), "l"(b_desc), "r"(IDESC), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void umma_commit(uint64_t* bar)
-{
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
-
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16])
-{
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15}, [%16];\n"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
-}
-
 // Epilogue for beta = 0 or 1 without reading C: per warp, 32 rows x 32 columns at a time go from tensor memory (thread
 // = row) to a 4 KB shared buffer in the 128-byte-swizzled layout of a {32 x 32} fp32 box (row r's 16-byte chunk k at
 // chunk k ^ (r & 7): conflict-free 16-byte stores), then one lane has TMA store the box into C (beta 0) or add it to C
@@ -478,22 +397,6 @@ __global__ void __launch_bounds__(128, 1) gemm_bf16x3p_tn_kernel(const __grid_co
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
     }
-}
-
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn()
-{
-    static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> fn{nullptr};
-    PFN_cuTensorMapEncodeTiled_v12000 f = fn.load(std::memory_order_acquire);
-    if (!f) {
-        void* ptr = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            return nullptr;
-        f = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-        fn.store(f, std::memory_order_release);
-    }
-    return f;
 }
 
 // Persistent form of gemm_bf16x3p_tn_kernel for beta 0 / 1 (TMA store / reduce-add epilogue): one CTA per SM walks
