@@ -35,23 +35,11 @@ __device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
     return a;
 }
+// Arrival on an mbarrier of either CTA.  What it guards is tensor memory, ordered by the tcgen05 fences, so it carries no
+// cluster-wide release: that waits for the warp's outstanding loads and cost 2000 cycles a block of K.
 __device__ __forceinline__ void arrive_cluster(uint32_t addr)
 {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(addr) : "memory");
-}
-__device__ __forceinline__ bool wait_cluster(uint64_t* b, uint32_t parity, int* err)
-{
-    for (uint32_t i = 0; i < WAIT_LIMIT; i++) {
-        uint32_t ok;
-        asm volatile(
-            "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-            : "=r"(ok)
-            : "r"(smem_u32(b)), "r"(parity)
-            : "memory");
-        if (ok) return true;
-    }
-    if (err) atomicExch(err, 1);
-    return false;
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(addr) : "memory");
 }
 // the copy lands in this CTA's shared memory, its bytes are counted on the mbarrier at `bar` (of either CTA of the pair)
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar)
@@ -82,21 +70,18 @@ __device__ __forceinline__ void mma_f8_pair(uint32_t d, uint64_t a, uint64_t b, 
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld16_issue(uint32_t taddr, uint32_t (&r)[16])
+__device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, uint32_t (&r)[32])
 {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15}, [%16];\n"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
 }
 // waits for the reads issued so far; the registers pass through, so that no use of them moves above the wait
-__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16])
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32])
 {
     asm volatile("tcgen05.wait::ld.sync.aligned;\n"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
                  :
                  : "memory");
 }
@@ -219,7 +204,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
                 const int m0 = (s.tile % g.mt) * WT + rank * 128, n0 = (s.tile / g.mt) * WT + rank * 128;
                 for (int k = s.k0; k < s.k1; k++, i++) {
                     const int st = i % W_STAGES;
-                    if (i >= W_STAGES && !wait_cluster(&empty[st], (i / W_STAGES - 1) & 1, g.err)) {
+                    if (i >= W_STAGES && !mbar_wait(&empty[st], (i / W_STAGES - 1) & 1, g.err, WAIT_LIMIT)) {
                         ok = false;
                         break;
                     }
@@ -230,7 +215,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
                 }
             }
             // a buffer is free again once its copies have landed and been read: none is in flight when the CTA leaves
-            for (int j = i > W_STAGES ? i - W_STAGES : 0; j < i; j++) wait_cluster(&empty[j % W_STAGES], (j / W_STAGES) & 1, g.err);
+            for (int j = i > W_STAGES ? i - W_STAGES : 0; j < i; j++) mbar_wait(&empty[j % W_STAGES], (j / W_STAGES) & 1, g.err, WAIT_LIMIT);
         }
         if (warp == 9 && rank == 0 && lane == 0) {
             Walk walk(g, pair, npairs);
@@ -241,8 +226,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
             while (ok && walk.next(s))
                 for (int k = s.k0; k < s.k1; k++, i++) {
                     const int st = i % W_STAGES, buf = i & 1;
-                    if ((i >= 2 && !wait_cluster(&accempty[buf], (i / 2 - 1) & 1, g.err)) ||
-                        !wait_cluster(&full[st], (i / W_STAGES) & 1, g.err)) {
+                    if ((i >= 2 && !mbar_wait(&accempty[buf], (i / 2 - 1) & 1, g.err, WAIT_LIMIT)) ||
+                        !mbar_wait(&full[st], (i / W_STAGES) & 1, g.err, WAIT_LIMIT)) {
                         ok = false;
                         break;
                     }
@@ -276,30 +261,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
             float acc[128];
 #pragma unroll
             for (int j = 0; j < 128; j++) acc[j] = 0.f;
-            float sc = live ? pa[s.k0 * g.ld_sa] * pb[s.k0] : 0.f;
-            for (int k = s.k0; k < s.k1; k++, i++) {
-                const int buf = i & 1;
-                const float next = live && k + 1 < s.k1 ? pa[(k + 1) * g.ld_sa] * pb[k + 1] : 0.f;
-                ok = wait_cluster(&accfull[buf], (i / 2) & 1, g.err);
-                __syncwarp();
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t t = lane_base + buf * WT;
-                uint32_t r[2][16];
-                tmem_ld16_issue(t, r[0]);
+            float sc[4], na[4], nb[4];  // scales of four blocks, and of the next four on their way: L2 answers later than a block
+            auto fetch = [&](int k) {
 #pragma unroll
-                for (int c = 0; c < 8; c++) {
-                    tmem_ld_wait(r[c & 1]);
-                    if (c < 7) tmem_ld16_issue(t + 16 * (c + 1), r[(c + 1) & 1]);
-                    else {  // the sums are in registers: the buffer goes back to the MMAs
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) arrive_cluster(free_bar[buf]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 16; j++) acc[16 * c + j] = fmaf(__uint_as_float(r[c & 1][j]), sc, acc[16 * c + j]);
+                for (int j = 0; j < 4; j++) {
+                    const bool in = live && k + j < s.k1;
+                    na[j] = in ? pa[(k + j) * g.ld_sa] : 0.f;
+                    nb[j] = in ? pb[k + j] : 0.f;
                 }
-                sc = next;
+            };
+            fetch(s.k0);
+            for (int kq = s.k0; kq < s.k1 && ok; kq += 4) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) sc[j] = na[j] * nb[j];
+                fetch(kq + 4);
+#pragma unroll
+                for (int kj = 0; kj < 4; kj++) {
+                    if (kq + kj >= s.k1) break;
+                    const int buf = i & 1;
+                    ok = mbar_wait(&accfull[buf], (i / 2) & 1, g.err, WAIT_LIMIT);
+                    i++;
+                    __syncwarp();
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t t = lane_base + buf * WT;
+                    uint32_t r[2][32];
+                    tmem_ld32_issue(t, r[0]);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        tmem_ld_wait(r[c & 1]);
+                        if (c < 3) tmem_ld32_issue(t + 32 * (c + 1), r[(c + 1) & 1]);
+                        else {  // the sums are in registers: the buffer goes back to the MMAs
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) arrive_cluster(free_bar[buf]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; j++)
+                            acc[32 * c + j] = fmaf(__uint_as_float(r[c & 1][j]), sc[kj], acc[32 * c + j]);
+                    }
+                }
             }
             if (!ok) break;
             if (s.k0 != 0 || s.k1 != g.nkb) {  // a part of the tile's sum
