@@ -85,6 +85,10 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32])
                  :
                  : "memory");
 }
+__device__ __forceinline__ void tmem_ld_pin(uint32_t (&r)[32])
+{
+    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y)
 {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(map), "r"(smem_u32(src)),
@@ -149,6 +153,13 @@ struct Walk {
     }
 };
 
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
+}
+
 template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
     gemm_wide_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -195,7 +206,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(W_REGS_ROLES));
-        if (warp == 8 && lane == 0) {
+        if (warp == 8) {
             Walk walk(g, pair, npairs);
             Segment s;
             int i = 0;
@@ -208,36 +219,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
                         ok = false;
                         break;
                     }
-                    if (rank == 0) mbar_expect_tx(&full[st], 2 * W_STAGE);  // both CTAs' bytes
                     const uint32_t bar = map_rank(&full[st], 0);
+                    if (elect_one()) {
+                    if (rank == 0) mbar_expect_tx(&full[st], 2 * W_STAGE);  // both CTAs' bytes
                     tma_load_2d_pair(smem + st * W_STAGE, &tmA, k * QB, m0, bar);
                     tma_load_2d_pair(smem + st * W_STAGE + W_OP, &tmB, k * QB, n0, bar);
+                    }
+                    __syncwarp();
                 }
             }
             // a buffer is free again once its copies have landed and been read: none is in flight when the CTA leaves
             for (int j = i > W_STAGES ? i - W_STAGES : 0; j < i; j++) mbar_wait(&empty[j % W_STAGES], (j / W_STAGES) & 1, g.err, WAIT_LIMIT);
         }
-        if (warp == 9 && rank == 0 && lane == 0) {
+        if (warp == 9 && rank == 0) {
+            // the whole warp runs the loop and one elected lane issues: the operands then stay in uniform registers
             Walk walk(g, pair, npairs);
             Segment s;
             constexpr uint32_t ID = idesc_f8(256, WT);
-            int i = 0;
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint64_t base = sw128_kmajor_desc(smem_u32(smem));
+            int st = 0, buf = 0;
+            uint32_t full_parity = 0, free_parity = 1;  // the first wait for either buffer passes at once
             bool ok = true;
             while (ok && walk.next(s))
-                for (int k = s.k0; k < s.k1; k++, i++) {
-                    const int st = i % W_STAGES, buf = i & 1;
-                    if ((i >= 2 && !mbar_wait(&accempty[buf], (i / 2 - 1) & 1, g.err, WAIT_LIMIT)) ||
-                        !mbar_wait(&full[st], (i / W_STAGES) & 1, g.err, WAIT_LIMIT)) {
-                        ok = false;
-                        break;
-                    }
+                for (int k = s.k0; k < s.k1; k++) {
+                    ok = mbar_wait(&full[st], full_parity, g.err, WAIT_LIMIT) &&
+                         mbar_wait(&accempty[buf], free_parity, g.err, WAIT_LIMIT);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
                     tc_fence_after();
-                    const uint32_t a = smem_u32(smem + st * W_STAGE), b = a + W_OP, d = tmem + buf * WT;
+                    const uint64_t a = base + (uint32_t)(st * (W_STAGE >> 4)), b = a + (W_OP >> 4);
+                    const uint32_t d = tm + buf * WT;
+                    if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < 4; kk++)
-                        mma_f8_pair(d, sw128_kmajor_desc(a + 32 * kk), sw128_kmajor_desc(b + 32 * kk), ID, kk != 0);
-                    commit_pair(&empty[st]);
-                    commit_pair(&accfull[buf]);
+                        for (int kk = 0; kk < 4; kk++) mma_f8_pair(d, a + 2 * kk, b + 2 * kk, ID, kk != 0);
+                        commit_pair(&accfull[buf]);
+                        commit_pair(&empty[st]);
+                    }
+                    __syncwarp();
+                    if (++st == W_STAGES) st = 0, full_parity ^= 1;
+                    if ((buf ^= 1) == 0) free_parity ^= 1;
                 }
         }
         __syncwarp();
@@ -287,19 +308,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
                     const uint32_t t = lane_base + buf * WT;
                     uint32_t r[2][32];
                     tmem_ld32_issue(t, r[0]);
+                    tmem_ld32_issue(t + 32, r[1]);
+                    tmem_ld_wait(r[0]);
+                    tmem_ld_pin(r[1]);
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        tmem_ld_wait(r[c & 1]);
-                        if (c < 3) tmem_ld32_issue(t + 32 * (c + 1), r[(c + 1) & 1]);
-                        else {  // the sums are in registers: the buffer goes back to the MMAs
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) arrive_cluster(free_bar[buf]);
-                        }
+                    for (int j = 0; j < 32; j++) acc[j] = fmaf(__uint_as_float(r[0][j]), sc[kj], acc[j]);
+                    tmem_ld32_issue(t + 64, r[0]);
 #pragma unroll
-                        for (int j = 0; j < 32; j++)
-                            acc[32 * c + j] = fmaf(__uint_as_float(r[c & 1][j]), sc[kj], acc[32 * c + j]);
-                    }
+                    for (int j = 0; j < 32; j++) acc[32 + j] = fmaf(__uint_as_float(r[1][j]), sc[kj], acc[32 + j]);
+                    tmem_ld32_issue(t + 96, r[1]);
+                    tmem_ld_wait(r[0]);
+                    tmem_ld_pin(r[1]);
+                    tc_fence_before();  // the sums are in registers: the buffer goes back to the MMAs
+                    __syncwarp();
+                    if (lane == 0) arrive_cluster(free_bar[buf]);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) acc[64 + j] = fmaf(__uint_as_float(r[0][j]), sc[kj], acc[64 + j]);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) acc[96 + j] = fmaf(__uint_as_float(r[1][j]), sc[kj], acc[96 + j]);
                 }
             }
             if (!ok) break;
