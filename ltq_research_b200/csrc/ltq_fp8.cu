@@ -44,23 +44,98 @@ __device__ __forceinline__ void store4(uint8_t* row, int c, int K, uint32_t q)
         for (int i = 0; c + i < K; i++) row[c + i] = (uint8_t)(q >> (8 * i));
 }
 
-// a warp per row and 128 columns
+// Activations.  A warp takes 1024 columns of ROWS rows, eight columns a lane and load (16 bytes of a 16-bit type), so a block
+// of 128 is half a warp's load and the maximum four exchanges; a row's loads are in flight while the row before it is worked on.  The scales of a
+// CTA's rows are gathered in shared memory and leave as one run of rows per block, the layout the products read.
+// The quotient x / s is rounded correctly without a division each: with r = 1 / s correctly rounded, q = x r and then
+// q + (x - q s) r is the correctly rounded quotient (Markstein's correction, IBM J. Res. Dev. 34, 1990) while the remainder
+// stays above the smallest normal number, which 2^-80 <= s guarantees for every quotient that e4m3 does not round to 0;
+// smaller scales take the division.  128 MB of bf16 in, 64 MB out: see the measured rate at the launch.
+__device__ __forceinline__ float quotient(float x, float s, float r)
+{
+    const float q = __fmul_rn(x, r);
+    return __fmaf_rn(__fmaf_rn(-q, s, x), r, q);
+}
+// eight elements of a row from column c on (zeros beyond K), as they are
 template <typename T>
-__global__ void __launch_bounds__(256) quant_rows_kernel(const T* __restrict__ x, long long ld, int M, int K,
+struct Raw8 {
+    uint4 u[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int c, int K, bool aligned, Raw8<T>& x)
+{
+    if (aligned && c + 8 <= K) {
+#pragma unroll
+        for (int h = 0; h < (int)sizeof(T) / 2; h++) x.u[h] = __ldg(reinterpret_cast<const uint4*>(row + c) + h);
+    } else {
+        T t[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) t[i] = c + i < K ? row[c + i] : from_f<T>(0.f);
+        memcpy(&x, t, sizeof(x));
+    }
+}
+__device__ __forceinline__ void unpack8(const Raw8<float>& x, float (&f)[8])
+{
+    f[0] = __uint_as_float(x.u[0].x), f[1] = __uint_as_float(x.u[0].y), f[2] = __uint_as_float(x.u[0].z), f[3] = __uint_as_float(x.u[0].w);
+    f[4] = __uint_as_float(x.u[1].x), f[5] = __uint_as_float(x.u[1].y), f[6] = __uint_as_float(x.u[1].z), f[7] = __uint_as_float(x.u[1].w);
+}
+__device__ __forceinline__ void unpack8(const Raw8<__nv_bfloat16>& x, float (&f)[8]) { unpack16(x.u[0], f, __nv_bfloat16()); }
+__device__ __forceinline__ void unpack8(const Raw8<__half>& x, float (&f)[8]) { unpack16(x.u[0], f, __half()); }
+
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) quant_rows_kernel(const T* __restrict__ x, long long ld, int M, int K,
                                                          uint8_t* __restrict__ q, long long ld_q, float* __restrict__ s,
                                                          long long ld_s, int aligned)
 {
-    const int kb = (K + QB - 1) / QB, lane = threadIdx.x & 31;
-    const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (unit >= (long long)M * kb) return;
-    const int m = (int)(unit / kb), b = (int)(unit - (long long)m * kb), c = b * QB + 4 * lane;
-    float v[4];
-    load4(x + m * ld, c, K, aligned, v);
-    uint32_t a = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
-    a = __reduce_max_sync(0xffffffffu, a);
-    const float sc = block_scale(a);
-    store4(q + m * ld_q, c, K, quant4(v, sc));
-    if (lane == 0) s[b * ld_s + m] = sc;
+    __shared__ float sc[8][8 * ROWS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c0 = blockIdx.x * 1024;
+    const int mb = blockIdx.y * (8 * ROWS);
+    const int m0 = mb + warp * ROWS, m1 = min(M, m0 + ROWS);
+    Raw8<T> next[4];
+    if (m0 < m1)
+#pragma unroll
+        for (int j = 0; j < 4; j++) load8(x + (long long)m0 * ld, c0 + 256 * j + 8 * lane, K, aligned, next[j]);
+    for (int m = m0; m < m1; m++) {
+        Raw8<T> cur[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) cur[j] = next[j];
+        if (m + 1 < m1)  // the next row's loads are on their way while this one is worked on
+#pragma unroll
+            for (int j = 0; j < 4; j++) load8(x + (m + 1) * ld, c0 + 256 * j + 8 * lane, K, aligned, next[j]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float v[8];
+            unpack8(cur[j], v);
+            uint32_t a = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) a = max(a, abs_bits(v[i]));
+#pragma unroll
+            for (int o = 8; o; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+            const float scale = block_scale(a), r = __frcp_rn(scale);
+            if (!(scale >= 0x1p-80f)) {  // a tiny scale, or NaN
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = __fdiv_rn(v[i], scale);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = quotient(v[i], scale, r);
+            }
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                w[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+            const int c = c0 + 256 * j + 8 * lane;
+            uint8_t* o = q + m * ld_q + c;
+            if (c + 8 <= K) *reinterpret_cast<uint2*>(o) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+            else
+                for (int i = 0; c + i < K; i++) o[i] = (uint8_t)(w[i >> 1] >> (8 * (i & 1)));
+            if ((lane & 15) == 0) sc[2 * j + (lane >> 4)][m - mb] = scale;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 8 * 8 * ROWS; i += 256) {
+        const int b = blockIdx.x * 8 + i / (8 * ROWS), m = mb + i % (8 * ROWS);
+        if (b * QB < K && m < M) s[b * ld_s + m] = sc[i / (8 * ROWS)][i % (8 * ROWS)];
+    }
 }
 
 // a CTA per 128 x 128 block
@@ -89,12 +164,12 @@ __global__ void __launch_bounds__(256) quant_blocks_kernel(const T* __restrict__
     if (threadIdx.x == 0) s[blockIdx.y * ld_s + blockIdx.x] = sc;
 }
 
-template <typename T>
+template <typename T, int ROWS>
 int quant_rows(const void* x, long long ld, int M, int K, uint8_t* q, long long ld_q, float* s, long long ld_s, cudaStream_t st)
 {
-    const long long units = (long long)M * ((K + QB - 1) / QB);
-    const int aligned = (uintptr_t)x % (4 * sizeof(T)) == 0 && ld % 4 == 0;
-    quant_rows_kernel<T><<<(unsigned)((units + 7) / 8), 256, 0, st>>>((const T*)x, ld, M, K, q, ld_q, s, ld_s, aligned);
+    const int aligned = (uintptr_t)x % 16 == 0 && ld * sizeof(T) % 16 == 0;
+    const dim3 grid((K + 1023) / 1024, (M + 8 * ROWS - 1) / (8 * ROWS));
+    quant_rows_kernel<T, ROWS><<<grid, 256, 0, st>>>((const T*)x, ld, M, K, q, ld_q, s, ld_s, aligned);
     return (int)cudaGetLastError();
 }
 template <typename T>
@@ -115,11 +190,15 @@ extern "C" int ltq_fp8_quant_rows(const void* x, int dtype, long long ld, int M,
     if (!es || M < 0 || K < 1 || ld < K || ld_s < M || ld_q % 16 || ld_q < K) return -1;
     if (M == 0) return 0;
     if (!x || (uintptr_t)x % es || !q || (uintptr_t)q % 16 || !s || (uintptr_t)s % 4) return -1;
-    if ((long long)M * ((K + QB - 1) / QB) > (1LL << 33)) return -1;
+    if (M > 65535 * 8) return -1;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == DT_F32) return quant_rows<float>(x, ld, M, K, q, ld_q, s, ld_s, st);
-    if (dtype == DT_BF16) return quant_rows<__nv_bfloat16>(x, ld, M, K, q, ld_q, s, ld_s, st);
-    return quant_rows<__half>(x, ld, M, K, q, ld_q, s, ld_s, st);
+    // one row a warp while that fills the GPU no more than a few times over, else four
+    const bool few = (long long)M * ((K + 1023) / 1024) < 8192;
+#define QUANT(T) return few ? quant_rows<T, 1>(x, ld, M, K, q, ld_q, s, ld_s, st) : quant_rows<T, 4>(x, ld, M, K, q, ld_q, s, ld_s, st)
+    if (dtype == DT_F32) QUANT(float);
+    if (dtype == DT_BF16) QUANT(__nv_bfloat16);
+    QUANT(__half);
+#undef QUANT
 }
 
 extern "C" int ltq_fp8_quant_blocks(const void* w, int dtype, long long ld, int N, int K, uint8_t* q, long long ld_q, float* s,
