@@ -13,6 +13,7 @@
 // A term with p_k = 0 is 0.  A row of weight 0, or without a live slot, has loss 0 and gradient 0 (weight 0: its logits
 // are not read).  Where q_{id_k} = 0 < p_k the loss is +inf and the gradient finite (q_j = 0).  NaN logits give NaN.
 #include <float.h>
+#include <atomic>
 #include "ltq_b200.h"
 #include "vec_types.cuh"
 
@@ -21,6 +22,7 @@ namespace {
 constexpr int DK_MAX = 1024;          // slots of a row
 constexpr int D_THREADS = 512;
 constexpr int D_MAXCL = 8;
+constexpr int D_SMEM = 200 * 1024;   // dynamic shared memory of a CTA at most
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 enum { M_LOSS = 0, M_BOTH = 1, M_GRAD = 2 };
 
@@ -42,11 +44,27 @@ struct DistillParams {
     int T, V, K, idx64, u_dt;
     float inv_tau;
     int cl;        // CTAs of a row (cluster size)
+    int hold;      // M_BOTH: vectors of a CTA's slice that stay in shared memory between the passes
+    int bit_words; // words of the bitmap, before the held vectors in shared memory
     int vec_out;   // dz rows have the alignment of z rows
 };
 
 // products and sums are written out (no contraction left to the compiler), so that every mode gives the same bits
-__device__ __forceinline__ float ex2(float x) { return exp2f(x); }
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;  // ex2.approx: relative error 2^-22, results below 2^-126 are 0
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_wait()
+{
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
 
 // (m, s) <- s 2^m-scaled sums joined: the pair (m, s) stands for s * 2^m
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2)
@@ -57,18 +75,9 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2)
     m = M;
 }
 
-template <int OP>  // 0 max, 1 sum; every thread gets the result; red: 32 floats of shared memory
-__device__ __forceinline__ float block_reduce(float v, float* red)
+template <int OP>  // 0 max, 1 sum, over the lanes of a warp; every lane gets the result
+__device__ __forceinline__ float warp_reduce(float v)
 {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const float w = __shfl_xor_sync(0xffffffffu, v, o);
-        v = OP ? v + w : fmaxf(v, w);
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = (threadIdx.x & 31) < D_THREADS / 32 ? red[threadIdx.x & 31] : (OP ? 0.f : -INFINITY);
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         const float w = __shfl_xor_sync(0xffffffffu, v, o);
@@ -76,21 +85,8 @@ __device__ __forceinline__ float block_reduce(float v, float* red)
     }
     return v;
 }
-
-// joins the (m, s) pairs of all threads in a fixed order; every thread gets the result
-__device__ __forceinline__ void block_join(float& m, float& s, float* red)
+__device__ __forceinline__ void warp_join(float& m, float& s)
 {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-        join(m, s, m2, s2);
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m, red[32 + (threadIdx.x >> 5)] = s;
-    __syncthreads();
-    const int l = threadIdx.x & 31;
-    m = l < D_THREADS / 32 ? red[l] : -INFINITY;
-    s = l < D_THREADS / 32 ? red[32 + l] : 0.f;
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
@@ -106,25 +102,25 @@ __device__ __forceinline__ float load_u(const void* u, int dt, long long i)
 }
 
 template <typename T, int MODE, bool REST>
-__global__ void __launch_bounds__(D_THREADS) distill_kernel(const DistillParams p)
+__global__ void __launch_bounds__(D_THREADS, 3) distill_kernel(const DistillParams p)
 {
-    constexpr int VEC = 16 / sizeof(T);
-    extern __shared__ uint32_t dsm[];
-    __shared__ float red[64];
-    __shared__ float pr[DK_MAX];   // p_k
-    __shared__ float zk[DK_MAX];   // z of the slot's token, in units of log2 (slots of this CTA; all slots on CTA 0)
-    __shared__ int id[DK_MAX];     // token or -1
+    constexpr int VEC = 16 / sizeof(T), WARPS = D_THREADS / 32;
+    extern __shared__ __align__(16) uint32_t dsm[];  // bitmap, held vectors, slots
+    __shared__ float red[2][WARPS];
+    __shared__ float slot_sums[6];  // sum p, p_r, sum p log p, and the pair of the slots' tokens in this CTA's slice
     __shared__ float xch[4][D_MAXCL];
     __shared__ int dup;
     uint32_t* bits = dsm;
+    float* pr = reinterpret_cast<float*>(dsm + p.bit_words + 4 * p.hold);  // u / tau, then p_k
+    float* zk = pr + p.K;  // z of the slot's token in units of log2 (slots of this CTA's slice; all slots on CTA 0)
+    int* id = reinterpret_cast<int*>(zk + p.K);  // token or -1
 
-    const int tid = threadIdx.x, K = p.K, V = p.V, cl = p.cl;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, K = p.K, V = p.V, cl = p.cl;
     const int rank = cl > 1 ? (int)cluster_rank() : 0;
     const long long row = blockIdx.x / cl;
     const T* z = (const T*)p.z + row * p.ld;
     T* dz = MODE == M_LOSS ? nullptr : (T*)p.dz + row * p.ld_d;
     const float w = p.weight ? p.weight[row] : 1.f;
-    const float g = MODE == M_GRAD && p.grad ? p.grad[row * p.s_grad] : 1.f;
     if (cl > 1) cluster_arrive();  // paired with the wait before the exchange: every CTA of the row has started
 
     // the row's 16-byte vectors: `head` elements before the first, nb vectors, the tail; this CTA's are [v0, v1), and
@@ -145,7 +141,7 @@ __global__ void __launch_bounds__(D_THREADS) distill_kernel(const DistillParams 
         if (MODE != M_LOSS) {
             if (p.vec_out) {
                 for (int v = v0 + tid; v < v1; v += D_THREADS)
-                    *reinterpret_cast<uint4*>(dz + head + (long long)v * VEC) = make_uint4(0, 0, 0, 0);
+                    __stcs(reinterpret_cast<uint4*>(dz + head + (long long)v * VEC), make_uint4(0, 0, 0, 0));
                 if (rank == 0 && tid < head) dz[tid] = from_f<T>(0.f);
                 if (rank == cl - 1 && head + nb * VEC + tid < V) dz[head + nb * VEC + tid] = from_f<T>(0.f);
             } else
@@ -155,69 +151,47 @@ __global__ void __launch_bounds__(D_THREADS) distill_kernel(const DistillParams 
         return;
     }
 
-    // slots: ids, p, the student's logits at them, the bitmap
+    const uint4* zv = reinterpret_cast<const uint4*>(z + head);
+    // M_BOTH: the slice is on its way to shared memory (each thread copies and later reads its own vectors, so that no
+    // barrier is needed) in four batches while the slots are worked on
+    const uint32_t held = (uint32_t)__cvta_generic_to_shared(dsm + p.bit_words);
+    const int nh = MODE == M_BOTH ? min(v1 - v0, p.hold) : 0;
+    const int batch = MODE == M_BOTH ? (nh + 4 * D_THREADS - 1) / (4 * D_THREADS) * D_THREADS : 0;
+    if (MODE == M_BOTH) {
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            for (int i = b * batch + tid; i < min(nh, (b + 1) * batch); i += D_THREADS) cp16(held + 16 * i, zv + v0 + i);
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+        }
+    }
+
+    // slots: ids, teacher logits, the student's logits at them, the bitmap
     const float c = p.inv_tau * LOG2E;
     const int nwords = ((v1 - v0 + 2) * VEC + 31) / 32;
     for (int i = tid; i < nwords; i += D_THREADS) bits[i] = 0;
     if (tid == 0) dup = 0;
-    float um = -INFINITY;
+    __syncthreads();
     for (int k = tid; k < K; k += D_THREADS) {
         const long long i = p.idx64 ? ((const long long*)p.idx)[row * p.ld_idx + k] : ((const int*)p.idx)[row * p.ld_idx + k];
-        const bool live = i >= 0 && i < V;
-        const float u = live ? __fmul_rn(load_u(p.u, p.u_dt, row * p.ld_u + k), p.inv_tau) : -INFINITY;
+        const float u = load_u(p.u, p.u_dt, row * p.ld_u + k);
+        const bool live = i >= 0 && i < V, own = live && i >= j0 && i < j1;
         id[k] = live ? (int)i : -1;
-        pr[k] = u;
-        if (live && (rank == 0 || (i >= j0 && i < j1))) zk[k] = __fmul_rn(to_f(z[i]), c);
-        um = fmaxf(um, u);
-    }
-    float lt;  // the teacher's log-sum-exp
-    if (REST) {
-        lt = p.lse[row];
-        __syncthreads();
-    } else {
-        um = block_reduce<0>(um, red);
-        const float b = um == -INFINITY ? 0.f : um;
-        float s = 0.f;
-        for (int k = tid; k < K; k += D_THREADS) s += ex2(__fmul_rn(pr[k] - b, LOG2E));
-        s = block_reduce<1>(s, red);
-        lt = s == 0.f ? 0.f : b + logf(s);  // no live slot, or all of them -inf: p = 0
-    }
-    // pr: from u / tau to p; P and the entropy term need it all
-    float psum = 0.f, plogp = 0.f;
-    for (int k = tid; k < K; k += D_THREADS) {
-        if (id[k] >= 0) {
-            const float lp = pr[k] - lt, pk = ex2(__fmul_rn(lp, LOG2E));
-            pr[k] = pk;
-            psum += pk;
-            if (!(pk == 0.f)) plogp = __fmaf_rn(pk, lp, plogp);
-            const int b = id[k] - jb;
-            if (id[k] >= j0 && id[k] < j1)
-                if (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31) & 1u) dup = 1;
-        } else
-            pr[k] = 0.f;
-    }
-    psum = block_reduce<1>(psum, red);
-    float prest = REST ? fmaxf(1.f - psum, 0.f) : 0.f;
-    if (REST && K >= V) {  // slots that hold every token leave no rest
-        float distinct = 0.f;
-        for (int k = tid; k < K; k += D_THREADS) {
-            bool first = id[k] >= 0;
-            for (int q = 0; q < k && first; q++) first = id[q] != id[k];
-            distinct += first ? 1.f : 0.f;
+        pr[k] = live ? __fmul_rn(u, p.inv_tau) : -INFINITY;
+        if (live && (rank == 0 || own)) zk[k] = __fmul_rn(to_f(z[i]), c);
+        if (own) {
+            const int b = (int)i - jb;
+            if (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31) & 1u) dup = 1;
         }
-        if (block_reduce<1>(distinct, red) == (float)V) prest = 0.f;
     }
     __syncthreads();
-    // of slots with one id the lowest stands for the token
     const bool any_dup = dup != 0;
-    auto leads = [&](int k) {  // slot k is the first with its id
+    auto leads = [&](int k) {  // slot k is the first with its id: of slots with one id the lowest stands for the token
         if (any_dup)
             for (int q = 0; q < k; q++)
                 if (id[q] == id[k]) return false;
         return true;
     };
 
-    const uint4* zv = reinterpret_cast<const uint4*>(z + head);
     const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bits);
     auto member_bits = [&](int v) -> uint32_t {
         const int b = v - v0 + 1;
@@ -225,13 +199,12 @@ __global__ void __launch_bounds__(D_THREADS) distill_kernel(const DistillParams 
     };
     auto is_member = [&](int j) { return (bits[(j - jb) >> 5] >> ((j - jb) & 31)) & 1u; };
 
-    float log2S, log2qr;  // log2 of S and of q_r
+    // one pass: (m, s) with the running maximum, over the tokens outside the slots (REST) or all
+    float m = -INFINITY, s = 0.f;
     if (MODE != M_GRAD) {
-        // one pass: (m, s) with the running maximum, over the tokens outside the slots (REST) or all
-        float m = -INFINITY, s = 0.f;
-        for (int v = v0 + tid; v < v1; v += D_THREADS) {
+        auto add = [&](const uint4& raw, int v) {
             float x[VEC];
-            unpack16(__ldg(zv + v), x, T());
+            unpack16(raw, x, T());
             if (REST) {
                 const uint32_t mb = member_bits(v);
                 if (mb)
@@ -248,9 +221,43 @@ __global__ void __launch_bounds__(D_THREADS) distill_kernel(const DistillParams 
                 m = vm;
             }
             const float b = m == -INFINITY ? 0.f : m;
+            float t[VEC];
 #pragma unroll
-            for (int i = 0; i < VEC; i++) s += ex2(fmaf(x[i], c, -b));
+            for (int i = 0; i < VEC; i++) t[i] = ex2(fmaf(x[i], c, -b));
+#pragma unroll
+            for (int o = VEC / 2; o; o >>= 1)
+#pragma unroll
+                for (int i = 0; i < o; i++) t[i] += t[i + o];
+            s += t[0];
+        };
+        if (MODE == M_BOTH) {
+            auto held_batch = [&](int b) {
+                for (int i = b * batch + tid; i < min(nh, (b + 1) * batch); i += D_THREADS) {
+                    uint4 u;
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n"
+                                 : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                                 : "r"(held + 16 * i));
+                    add(u, v0 + i);
+                }
+            };
+            cp_wait<3>();
+            held_batch(0);
+            cp_wait<2>();
+            held_batch(1);
+            cp_wait<1>();
+            held_batch(2);
+            cp_wait<0>();
+            held_batch(3);
         }
+        int v = v0 + nh + tid;
+        for (; v + 3 * D_THREADS < v1; v += 4 * D_THREADS) {
+            uint4 u[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) u[q] = __ldg(zv + v + q * D_THREADS);
+#pragma unroll
+            for (int q = 0; q < 4; q++) add(u[q], v + q * D_THREADS);
+        }
+        for (; v < v1; v += D_THREADS) add(__ldg(zv + v), v);
         auto scalar = [&](int j) {
             if (!(REST && is_member(j))) {
                 const float x = __fmul_rn(to_f(z[j]), c);
@@ -261,13 +268,56 @@ __global__ void __launch_bounds__(D_THREADS) distill_kernel(const DistillParams 
         };
         if (rank == 0 && tid < head) scalar(tid);
         if (rank == cl - 1 && head + nb * VEC + tid < V) scalar(head + nb * VEC + tid);
-        block_join(m, s, red);
-        float mt = -INFINITY, st = 0.f;  // the slots' tokens of this CTA
-        if (REST) {
-            for (int k = tid; k < K; k += D_THREADS)
-                if (id[k] >= j0 && id[k] < j1 && leads(k)) join(mt, st, zk[k], 1.f);
-            block_join(mt, st, red);
+        warp_join(m, s);
+        if (lane == 0) red[0][warp] = m, red[1][warp] = s;
+    }
+    // the slots' sums, on the last warp: p_k into pr, P, the entropy term, the pair of this CTA's tokens
+    if (warp == WARPS - 1) {
+        float lt;  // the teacher's log-sum-exp
+        if (REST) lt = p.lse[row];
+        else {
+            float um = -INFINITY, t = 0.f;
+            for (int k = lane; k < K; k += 32) um = fmaxf(um, pr[k]);
+            um = warp_reduce<0>(um);
+            const float b = um == -INFINITY ? 0.f : um;
+            for (int k = lane; k < K; k += 32) t += ex2(__fmul_rn(pr[k] - b, LOG2E));
+            t = warp_reduce<1>(t);
+            lt = t == 0.f ? 0.f : b + logf(t);  // no live slot, or all of them -inf: p = 0
         }
+        float psum = 0.f, plogp = 0.f, mt = -INFINITY, st = 0.f, distinct = 0.f;
+        for (int k = lane; k < K; k += 32) {
+            const int i = id[k];
+            float pk = 0.f;
+            if (i >= 0) {
+                const float lp = pr[k] - lt;
+                pk = ex2(__fmul_rn(lp, LOG2E));
+                psum += pk;
+                if (!(pk == 0.f)) plogp = __fmaf_rn(pk, lp, plogp);
+                if (REST && MODE != M_GRAD && i >= j0 && i < j1 && leads(k)) join(mt, st, zk[k], 1.f);
+                if (REST && K >= V) {
+                    bool first = true;
+                    for (int q = 0; q < k && first; q++) first = id[q] != i;
+                    distinct += first ? 1.f : 0.f;
+                }
+            }
+            pr[k] = pk;
+        }
+        psum = warp_reduce<1>(psum);
+        plogp = warp_reduce<1>(plogp);
+        if (REST && MODE != M_GRAD) warp_join(mt, st);
+        float prest = REST ? fmaxf(1.f - psum, 0.f) : 0.f;
+        if (REST && K >= V && warp_reduce<1>(distinct) == (float)V) prest = 0.f;  // slots that hold every token leave no rest
+        if (lane == 0) slot_sums[0] = psum, slot_sums[1] = prest, slot_sums[2] = plogp, slot_sums[3] = mt, slot_sums[4] = st;
+    }
+    __syncthreads();
+    const float psum = slot_sums[0], prest = slot_sums[1];
+
+    float log2S, log2qr;  // log2 of S and of q_r
+    if (MODE != M_GRAD) {
+        m = lane < WARPS ? red[0][lane] : -INFINITY;
+        s = lane < WARPS ? red[1][lane] : 0.f;
+        warp_join(m, s);
+        float mt = slot_sums[3], st = slot_sums[4];
         if (cl > 1) {
             cluster_wait();
             if (tid < cl) {
@@ -285,13 +335,13 @@ __global__ void __launch_bounds__(D_THREADS) distill_kernel(const DistillParams 
         if (REST) join(ma, sa, mt, st);
         log2S = ma + log2f(sa);
         log2qr = !REST || s == 0.f ? -INFINITY : m + log2f(s) - log2S;
-        if (rank == 0) {
+        if (rank == 0 && warp == 0) {
             float l = 0.f;
             const float b = log2S == -INFINITY ? 0.f : log2S;
-            for (int k = tid; k < K; k += D_THREADS)
+            for (int k = lane; k < K; k += 32)
                 if (!(pr[k] == 0.f)) l = __fmaf_rn(-pr[k], __fmul_rn(zk[k] - b, LN2), l);
-            l = block_reduce<1>(l + plogp, red);
-            if (tid == 0) {
+            l = warp_reduce<1>(l) + slot_sums[2];
+            if (lane == 0) {
                 if (prest > 0.f) l = __fmaf_rn(prest, __fmaf_rn(-log2qr, LN2, logf(prest)), l);
                 p.loss[row] = __fmul_rn(w, l);
                 if (p.stats) p.stats[2 * row] = log2S * LN2, p.stats[2 * row + 1] = log2qr * LN2;
@@ -304,6 +354,7 @@ __global__ void __launch_bounds__(D_THREADS) distill_kernel(const DistillParams 
     }
 
     if (MODE != M_LOSS) {
+        const float g = MODE == M_GRAD && p.grad ? p.grad[row * p.s_grad] : 1.f;
         const float scale = g * w * p.inv_tau;
         const float P = psum + prest;
         // outside the slots: scale (P - p_r / q_r) 2^(z c - log2 S); a rest that the student gives nothing has q_j = 0
@@ -311,13 +362,30 @@ __global__ void __launch_bounds__(D_THREADS) distill_kernel(const DistillParams 
         const float b = log2S == -INFINITY ? 0.f : log2S;
         auto grad_of = [&](float x) { return cr * ex2(fmaf(x, c, -b)); };
         if (p.vec_out) {
-            for (int v = v0 + tid; v < v1; v += D_THREADS) {
+            auto put = [&](const uint4& raw, int v) {
                 float x[VEC];
-                unpack16(__ldg(zv + v), x, T());
+                unpack16(raw, x, T());
 #pragma unroll
                 for (int i = 0; i < VEC; i++) x[i] = grad_of(x[i]);
-                *reinterpret_cast<uint4*>(dz + head + (long long)v * VEC) = pack16(x, T());
+                __stcs(reinterpret_cast<uint4*>(dz + head + (long long)v * VEC), pack16(x, T()));
+            };
+            for (int i = tid; i < nh; i += D_THREADS) {
+                uint4 u;
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n"
+                             : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                             : "r"(held + 16 * i));
+                put(u, v0 + i);
             }
+            // plain loads: the rows may be overwritten (dz = z), each vector by the thread that has read it
+            int v = v0 + nh + tid;
+            for (; v + 3 * D_THREADS < v1; v += 4 * D_THREADS) {
+                uint4 u[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) u[q] = zv[v + q * D_THREADS];
+#pragma unroll
+                for (int q = 0; q < 4; q++) put(u[q], v + q * D_THREADS);
+            }
+            for (; v < v1; v += D_THREADS) put(zv[v], v);
             if (rank == 0 && tid < head) dz[tid] = from_f<T>(grad_of(to_f(z[tid])));
             if (rank == cl - 1 && head + nb * VEC + tid < V)
                 dz[head + nb * VEC + tid] = from_f<T>(grad_of(to_f(z[head + nb * VEC + tid])));
@@ -336,15 +404,25 @@ __global__ void __launch_bounds__(D_THREADS) distill_kernel(const DistillParams 
 }
 
 template <typename T, int MODE, bool REST>
-int launch(const DistillParams& p, int cl, cudaStream_t st)
+int launch(DistillParams p, int cl, cudaStream_t st)
 {
     constexpr int VEC = 16 / sizeof(T);
     const int per = (p.V / VEC + cl - 1) / cl;
-    const int smem = (((per + 2) * VEC + 31) / 32) * 4;
+    p.bit_words = (((per + 2) * VEC + 31) / 32 + 3) / 4 * 4;
+    p.hold = MODE == M_BOTH ? per : 0;
+    const int fixed = p.bit_words * 4 + p.K * 12;
+    if (fixed + p.hold * 16 > D_SMEM) p.hold = (D_SMEM - fixed) / 16;
+    const int smem = fixed + p.hold * 16;
     auto k = distill_kernel<T, MODE, REST>;
-    if (smem > 32768) {  // beyond the default 48 KB with the static arrays
-        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return (int)e;
+    if (smem > 46 * 1024) {  // beyond the default 48 KB with the static arrays
+        static std::atomic<int> ready[64];
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+        if (!ready[dev].load(std::memory_order_acquire)) {
+            const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, D_SMEM);
+            if (e != cudaSuccess) return (int)e;
+            ready[dev].store(1, std::memory_order_release);
+        }
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((long long)p.T * cl));
@@ -357,6 +435,18 @@ int launch(const DistillParams& p, int cl, cudaStream_t st)
     cfg.attrs = at;
     cfg.numAttrs = cl > 1 ? 1 : 0;
     return (int)cudaLaunchKernelEx(&cfg, k, p);
+}
+
+// CTAs of a row.  Loss and gradient: as few as let a slice stay in 72 KB of shared memory (three CTAs an SM, one row's
+// loads under another's exponentials and stores), so that the row is read from memory once; otherwise one.  Few rows: more, until
+// the GPU's SMs have one each.
+int row_ctas(long long T, int V, int es, int mode)
+{
+    int cl = 1;
+    if (mode == M_BOTH)
+        while (cl < D_MAXCL && (long long)V * es > 72 * 1024LL * cl) cl *= 2;
+    while (cl < D_MAXCL && T * cl < 148 && (long long)V * es / cl > 16 * 1024) cl *= 2;
+    return cl;
 }
 
 template <typename T>
@@ -390,7 +480,7 @@ extern "C" int ltq_distill_topk(const void* logits, int dtype, long long ld, con
     p.weight = weight, p.grad = grad, p.s_grad = grad_stride, p.loss = loss, p.stats = stats, p.dz = dlogits, p.ld_d = ld_d;
     p.T = T, p.V = V, p.K = K, p.idx64 = idx64 != 0, p.u_dt = teacher_dtype, p.inv_tau = 1.f / temperature;
     p.vec_out = mode != M_LOSS && ((uintptr_t)logits & 15) == ((uintptr_t)dlogits & 15) && ((ld - ld_d) * es) % 16 == 0;
-    const int cl = p.cl = 1;
+    const int cl = p.cl = row_ctas(T, V, es, mode);
     const cudaStream_t st = (cudaStream_t)stream;
     if (dtype == DT_F32) return dispatch<float>(p, mode, cl, st);
     if (dtype == DT_BF16) return dispatch<__nv_bfloat16>(p, mode, cl, st);
