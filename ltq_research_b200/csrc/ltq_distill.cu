@@ -20,8 +20,9 @@
 namespace {
 
 constexpr int DK_MAX = 1024;          // slots of a row
-constexpr int D_THREADS = 512;
+constexpr int D_THREADS = 256;
 constexpr int D_MAXCL = 8;
+constexpr long long D_ROW = 72 * 1024, D_SLICE = 52 * 1024;  // shared memory for a whole row of one CTA, for a cluster CTA's slice
 constexpr int D_SMEM = 200 * 1024;   // dynamic shared memory of a CTA at most
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 enum { M_LOSS = 0, M_BOTH = 1, M_GRAD = 2 };
@@ -43,10 +44,10 @@ struct DistillParams {
     long long ld_d;
     int T, V, K, idx64, u_dt;
     float inv_tau;
-    int cl;        // CTAs of a row (cluster size)
-    int hold;      // M_BOTH: vectors of a CTA's slice that stay in shared memory between the passes
-    int bit_words; // words of the bitmap, before the held vectors in shared memory
-    int vec_out;   // dz rows have the alignment of z rows
+    int cl;         // CTAs of a row (cluster size)
+    int hold;       // vectors of a slice that are held in shared memory (twice: this row's and the next one's)
+    int bit_words;  // words of the bitmap, before the held vectors in shared memory
+    int vec_out;    // dz rows have the alignment of z rows
 };
 
 // products and sums are written out (no contraction left to the compiler), so that every mode gives the same bits
@@ -85,13 +86,17 @@ __device__ __forceinline__ float warp_reduce(float v)
     }
     return v;
 }
+// joins the pairs of groups of N lanes; the maximum first (NaN pairs do not raise it), then one rescaling and a sum
+template <int N>
 __device__ __forceinline__ void warp_join(float& m, float& s)
 {
+    float M = m;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-        join(m, s, m2, s2);
-    }
+    for (int o = N / 2; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    s = __fmul_rn(s, ex2(m - (M == -INFINITY ? 0.f : M)));
+#pragma unroll
+    for (int o = N / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    m = M;
 }
 
 __device__ __forceinline__ float load_u(const void* u, int dt, long long i)
@@ -101,319 +106,420 @@ __device__ __forceinline__ float load_u(const void* u, int dt, long long i)
                            : __half2float(((const __half*)u)[i]);
 }
 
-template <typename T, int MODE, bool REST>
-__global__ void __launch_bounds__(D_THREADS, 3) distill_kernel(const DistillParams p)
+// The slice of a row that a CTA of the row's cluster works on: the row's 16-byte vectors begin `head` elements in, nb of them;
+// this CTA's are [v0, v1), its elements [j0, j1) (the elements before and behind the vectors belong to the first and last CTA).
+template <typename T>
+struct Slice {
+    const T* z;
+    int head, nb, v0, v1, j0, j1;
+    __device__ Slice(const DistillParams& p, long long row, int rank)
+    {
+        constexpr int VEC = 16 / sizeof(T);
+        z = (const T*)p.z + row * p.ld;
+        const int phase = (int)(((uintptr_t)z & 15) / sizeof(T));
+        head = min(p.V, (VEC - phase) % VEC);
+        nb = (p.V - head) / VEC;
+        const int per = (nb + p.cl - 1) / p.cl;
+        v0 = min(nb, rank * per), v1 = min(nb, v0 + per);
+        j0 = rank == 0 ? 0 : head + v0 * VEC;
+        j1 = rank == p.cl - 1 ? p.V : head + v1 * VEC;
+    }
+    __device__ int tail() const { return head + nb * (16 / (int)sizeof(T)); }
+};
+
+__device__ __forceinline__ void load_slot(const DistillParams& p, long long row, int k, int& id, float& u)
 {
-    constexpr int VEC = 16 / sizeof(T), WARPS = D_THREADS / 32;
-    extern __shared__ __align__(16) uint32_t dsm[];  // bitmap, held vectors, slots
+    const long long i = p.idx64 ? ((const long long*)p.idx)[row * p.ld_idx + k] : ((const int*)p.idx)[row * p.ld_idx + k];
+    const float t = load_u(p.u, p.u_dt, row * p.ld_u + k);
+    id = i >= 0 && i < p.V ? (int)i : -1;
+    u = id >= 0 ? __fmul_rn(t, p.inv_tau) : -INFINITY;
+}
+
+// p_k into pr (from u / tau) on one warp; returns P's two parts and sum p log p
+template <bool REST>
+__device__ __forceinline__ void teacher_probabilities(const DistillParams& p, float lse, float* pr, const int* id, int lane,
+                                                      float& psum, float& prest, float& plogp)
+{
+    const int K = p.K;
+    float lt = lse;  // the teacher's log-sum-exp
+    if (!REST) {
+        float um = -INFINITY, t = 0.f;
+        for (int k = lane; k < K; k += 32) um = fmaxf(um, pr[k]);
+        um = warp_reduce<0>(um);
+        const float b = um == -INFINITY ? 0.f : um;
+        for (int k = lane; k < K; k += 32) t += ex2(__fmul_rn(pr[k] - b, LOG2E));
+        t = warp_reduce<1>(t);
+        lt = t == 0.f ? 0.f : b + logf(t);  // no live slot, or all of them -inf: p = 0
+    }
+    float distinct = 0.f;
+    psum = plogp = 0.f;
+    for (int k = lane; k < K; k += 32) {
+        float pk = 0.f;
+        if (id[k] >= 0) {
+            const float lp = pr[k] - lt;
+            pk = ex2(__fmul_rn(lp, LOG2E));
+            psum += pk;
+            if (!(pk == 0.f)) plogp = __fmaf_rn(pk, lp, plogp);
+            if (REST && K >= p.V) {
+                bool first = true;
+                for (int q = 0; q < k && first; q++) first = id[q] != id[k];
+                distinct += first ? 1.f : 0.f;
+            }
+        }
+        pr[k] = pk;
+    }
+    psum = warp_reduce<1>(psum);
+    plogp = warp_reduce<1>(plogp);
+    prest = REST ? fmaxf(1.f - psum, 0.f) : 0.f;
+    if (REST && K >= p.V && warp_reduce<1>(distinct) == (float)p.V) prest = 0.f;  // slots that hold every token leave no rest
+}
+
+// slot k is the first with its id: of slots with one id the lowest stands for the token
+__device__ __forceinline__ bool leads(const int* id, int k)
+{
+    for (int q = 0; q < k; q++)
+        if (id[q] == id[k]) return false;
+    return true;
+}
+
+// what the gradient of a row needs: outside the slots cr 2^(z c - b), for a slot's token scale (P 2^(z c - b) - sum p)
+struct GradScale {
+    float scale, P, cr, b;
+    __device__ GradScale(float scale_, float psum, float prest, float log2S, float log2qr) : scale(scale_), P(psum + prest)
+    {
+        // a rest that the student gives nothing has q_j = 0 throughout
+        cr = scale * (prest > 0.f ? (log2qr == -INFINITY ? 0.f : P - prest * ex2(-log2qr)) : P);
+        b = log2S == -INFINITY ? 0.f : log2S;
+    }
+};
+template <typename T>
+__device__ __forceinline__ uint4 grad16(const uint4& raw, uint64_t cc, uint64_t bb, uint64_t rr)
+{
+    constexpr int VEC = 16 / sizeof(T);
+    float x[VEC];
+    unpack16(raw, x, T());
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+        const float2 e = unpair(fma2(pair(x[i], x[i + 1]), cc, bb));
+        const float2 d = unpair(mul2(rr, pair(ex2(e.x), ex2(e.y))));
+        x[i] = d.x, x[i + 1] = d.y;
+    }
+    return pack16(x, T());
+}
+template <typename T>
+__device__ __forceinline__ void zero_slice(const DistillParams& p, const Slice<T>& w, T* dz, int rank, int tid, int threads)
+{
+    constexpr int VEC = 16 / sizeof(T);
+    if (p.vec_out) {
+        for (int v = w.v0 + tid; v < w.v1; v += threads)
+            __stcs(reinterpret_cast<uint4*>(dz + w.head + (long long)v * VEC), make_uint4(0, 0, 0, 0));
+        if (rank == 0 && tid < w.head) dz[tid] = from_f<T>(0.f);
+        if (rank == p.cl - 1 && w.tail() + tid < p.V) dz[w.tail() + tid] = from_f<T>(0.f);
+    } else
+        for (int j = w.j0 + tid; j < w.j1; j += threads) dz[j] = from_f<T>(0.f);
+}
+
+// Losses, and with GRAD their gradients.  A cluster per row, each CTA a slice of it; with GRAD the slice stays in shared memory
+// between the two passes, so that the row is read from memory once.  Several small CTAs an SM, not one large one: a row has
+// latencies in a chain (its weight, its slots, the sums, the cluster's barrier) and only other rows can fill them.  The last warp
+// works on the slots alone, while the others are in their first pass.
+// Bound: the logits read once and the gradient written once; two exponentials an element (16 a clock and SM) take about half
+// of that time.
+template <typename T, bool GRAD, bool REST>
+__global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const DistillParams p)
+{
+    constexpr int VEC = 16 / sizeof(T), WARPS = D_THREADS / 32, ALL = D_THREADS + 32;
+    extern __shared__ __align__(16) uint32_t dsm[];  // bitmap, held slice, slots
     __shared__ float red[2][WARPS];
-    __shared__ float slot_sums[6];  // sum p, p_r, sum p log p, and the pair of the slots' tokens in this CTA's slice
+    __shared__ float slot_sums[5];  // sum p, p_r, sum p log p, the pair of the slots' tokens in the slice
     __shared__ float xch[4][D_MAXCL];
     __shared__ int dup;
     uint32_t* bits = dsm;
     float* pr = reinterpret_cast<float*>(dsm + p.bit_words + 4 * p.hold);  // u / tau, then p_k
-    float* zk = pr + p.K;  // z of the slot's token in units of log2 (slots of this CTA's slice; all slots on CTA 0)
+    float* zk = pr + p.K;  // z of the slot's token in units of log2 (slots of the slice; all of them on the first CTA)
     int* id = reinterpret_cast<int*>(zk + p.K);  // token or -1
+    const uint32_t held = (uint32_t)__cvta_generic_to_shared(dsm + p.bit_words);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, K = p.K, V = p.V, cl = p.cl;
     const int rank = cl > 1 ? (int)cluster_rank() : 0;
     const long long row = blockIdx.x / cl;
-    const T* z = (const T*)p.z + row * p.ld;
-    T* dz = MODE == M_LOSS ? nullptr : (T*)p.dz + row * p.ld_d;
     const float w = p.weight ? p.weight[row] : 1.f;
-    if (cl > 1) cluster_arrive();  // paired with the wait before the exchange: every CTA of the row has started
-
-    // the row's 16-byte vectors: `head` elements before the first, nb vectors, the tail; this CTA's are [v0, v1), and
-    // its elements [j0, j1)
-    const int phase = (int)(((uintptr_t)z & 15) / sizeof(T));
-    const int head = min(V, (VEC - phase) % VEC);
-    const int nb = (V - head) / VEC;
-    const int per = (nb + cl - 1) / cl;
-    const int v0 = min(nb, rank * per), v1 = min(nb, v0 + per);
-    const int j0 = rank == 0 ? 0 : head + v0 * VEC, j1 = rank == cl - 1 ? V : head + v1 * VEC;
-    const int jb = head + (v0 - 1) * VEC;  // element of bit 0: vector v's bits start at (v - v0 + 1) VEC
-
+    int id0 = -1;
+    float u0 = 0.f;
+    if (tid < K) load_slot(p, row, tid, id0, u0);  // in flight together with the weight
+    if (cl > 1) cluster_arrive_relaxed();          // paired with the wait before the exchange: every CTA of the row has started
+    const Slice<T> sl(p, row, rank);
+    T* dz = GRAD ? (T*)p.dz + row * p.ld_d : nullptr;
     if (w == 0.f) {  // no loss, no gradient; the logits may be anything
-        if (MODE != M_GRAD && rank == 0 && tid == 0) {
+        if (rank == 0 && tid == 0) {
             p.loss[row] = 0.f;
             if (p.stats) p.stats[2 * row] = 0.f, p.stats[2 * row + 1] = 0.f;
         }
-        if (MODE != M_LOSS) {
-            if (p.vec_out) {
-                for (int v = v0 + tid; v < v1; v += D_THREADS)
-                    __stcs(reinterpret_cast<uint4*>(dz + head + (long long)v * VEC), make_uint4(0, 0, 0, 0));
-                if (rank == 0 && tid < head) dz[tid] = from_f<T>(0.f);
-                if (rank == cl - 1 && head + nb * VEC + tid < V) dz[head + nb * VEC + tid] = from_f<T>(0.f);
-            } else
-                for (int j = j0 + tid; j < j1; j += D_THREADS) dz[j] = from_f<T>(0.f);
-        }
+        if (GRAD) zero_slice(p, sl, dz, rank, tid, ALL);
         if (cl > 1) cluster_wait();
         return;
     }
-
-    const uint4* zv = reinterpret_cast<const uint4*>(z + head);
-    // M_BOTH: the slice is on its way to shared memory (each thread copies and later reads its own vectors, so that no
-    // barrier is needed) in four batches while the slots are worked on
-    const uint32_t held = (uint32_t)__cvta_generic_to_shared(dsm + p.bit_words);
-    const int nh = MODE == M_BOTH ? min(v1 - v0, p.hold) : 0;
-    const int batch = MODE == M_BOTH ? (nh + 4 * D_THREADS - 1) / (4 * D_THREADS) * D_THREADS : 0;
-    if (MODE == M_BOTH) {
+    // The slice is on its way to shared memory (each thread copies and later reads its own vectors: no barrier for them) in
+    // four batches while the slots are set up.
+    const int nvec = sl.v1 - sl.v0, nh = GRAD ? min(nvec, p.hold) : 0;
+    const int bt = GRAD ? (nh + 4 * D_THREADS - 1) / (4 * D_THREADS) : 0;  // a thread's vectors in a batch
+    const uint4* zt = reinterpret_cast<const uint4*>(sl.z + sl.head) + sl.v0 + tid;
+    if (GRAD && tid < D_THREADS) {
 #pragma unroll
         for (int b = 0; b < 4; b++) {
-            for (int i = b * batch + tid; i < min(nh, (b + 1) * batch); i += D_THREADS) cp16(held + 16 * i, zv + v0 + i);
+            for (int t = b * bt; t < (b + 1) * bt && tid + t * D_THREADS < nh; t++)
+                cp16(held + 16 * tid + t * (16 * D_THREADS), zt + t * D_THREADS);
             asm volatile("cp.async.commit_group;\n" ::: "memory");
         }
     }
-
-    // slots: ids, teacher logits, the student's logits at them, the bitmap
-    const float c = p.inv_tau * LOG2E;
-    const int nwords = ((v1 - v0 + 2) * VEC + 31) / 32;
-    for (int i = tid; i < nwords; i += D_THREADS) bits[i] = 0;
+    const int jb = sl.head + (sl.v0 - 1) * VEC;  // element of bit 0: vector v's bits start at (v - v0 + 1) VEC
+    for (int i = tid; i < ((nvec + 2) * VEC + 31) / 32; i += ALL) bits[i] = 0;
     if (tid == 0) dup = 0;
     __syncthreads();
-    for (int k = tid; k < K; k += D_THREADS) {
-        const long long i = p.idx64 ? ((const long long*)p.idx)[row * p.ld_idx + k] : ((const int*)p.idx)[row * p.ld_idx + k];
-        const float u = load_u(p.u, p.u_dt, row * p.ld_u + k);
-        const bool live = i >= 0 && i < V, own = live && i >= j0 && i < j1;
-        id[k] = live ? (int)i : -1;
-        pr[k] = live ? __fmul_rn(u, p.inv_tau) : -INFINITY;
-        if (live && (rank == 0 || own)) zk[k] = __fmul_rn(to_f(z[i]), c);
+    const float c = p.inv_tau * LOG2E;
+    for (int k = tid; k < K; k += ALL) {
+        if (k != tid) load_slot(p, row, k, id0, u0);
+        const bool own = id0 >= 0 && id0 >= sl.j0 && id0 < sl.j1;
+        id[k] = id0, pr[k] = u0;
+        if (own || (rank == 0 && id0 >= 0)) zk[k] = __fmul_rn(to_f(sl.z[id0]), c);
         if (own) {
-            const int b = (int)i - jb;
+            const int b = id0 - jb;
             if (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31) & 1u) dup = 1;
         }
     }
     __syncthreads();
     const bool any_dup = dup != 0;
-    auto leads = [&](int k) {  // slot k is the first with its id: of slots with one id the lowest stands for the token
-        if (any_dup)
-            for (int q = 0; q < k; q++)
-                if (id[q] == id[k]) return false;
-        return true;
-    };
 
-    const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bits);
-    auto member_bits = [&](int v) -> uint32_t {
-        const int b = v - v0 + 1;
-        return VEC == 8 ? bytes[b] : (bytes[b >> 1] >> ((b & 1) * 4)) & 15u;
+    const uint64_t cc = pair(c, c);
+    auto held_vec = [&](int t) {
+        uint4 u;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n"
+                     : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                     : "r"(held + 16 * tid + t * (16 * D_THREADS)));
+        return u;
     };
-    auto is_member = [&](int j) { return (bits[(j - jb) >> 5] >> ((j - jb) & 31)) & 1u; };
+    // this thread's vectors: v0 + tid + t * D_THREADS for t < nt, the first nth of them in shared memory
+    const int nt = tid < D_THREADS ? (nvec - tid + D_THREADS - 1) / D_THREADS : 0;
+    const int nth = tid < D_THREADS ? max(0, (nh - tid + D_THREADS - 1) / D_THREADS) : 0;
 
-    // one pass: (m, s) with the running maximum, over the tokens outside the slots (REST) or all
-    float m = -INFINITY, s = 0.f;
-    if (MODE != M_GRAD) {
-        auto add = [&](const uint4& raw, int v) {
-            float x[VEC];
-            unpack16(raw, x, T());
+    if (warp < WARPS) {
+        // one pass: (m, s) with the running maximum, over the tokens outside the slots (REST) or all
+        float m = -INFINITY, s;
+        uint64_t s2 = 0;  // two sums, by the elements' parity
+        // the bits of this thread's vectors: at a fixed step (and, of four-element vectors, a fixed half of a byte)
+        const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bits) + (VEC == 8 ? tid + 1 : (tid + 1) >> 1);
+        constexpr int step = VEC == 8 ? D_THREADS : D_THREADS / 2;
+        auto add = [&](uint4 raw, int t) {
             if (REST) {
-                const uint32_t mb = member_bits(v);
-                if (mb)
-#pragma unroll
-                    for (int i = 0; i < VEC; i++)
-                        if (mb >> i & 1u) x[i] = -INFINITY;
+                const uint32_t by = bytes[t * step], mb = VEC == 8 ? by : by >> (((tid + 1) & 1) * 4) & 15u;
+                if (mb) raw = mask16(raw, mb, T());
             }
-            float vm = x[0];
-#pragma unroll
-            for (int i = 1; i < VEC; i++) vm = fmaxf(vm, x[i]);
-            vm = __fmul_rn(vm, c);
+            const float vm = __fmul_rn(max16(raw, T()), c);
             if (vm > m) {
-                s *= ex2(m - vm);
+                const float f = ex2(m - vm);
+                s2 = mul2(s2, pair(f, f));
                 m = vm;
             }
-            const float b = m == -INFINITY ? 0.f : m;
-            float t[VEC];
+            const float b = m == -INFINITY ? 0.f : -m;
+            const uint64_t bb = pair(b, b);
+            float x[VEC];
+            unpack16(raw, x, T());
 #pragma unroll
-            for (int i = 0; i < VEC; i++) t[i] = ex2(fmaf(x[i], c, -b));
-#pragma unroll
-            for (int o = VEC / 2; o; o >>= 1)
-#pragma unroll
-                for (int i = 0; i < o; i++) t[i] += t[i + o];
-            s += t[0];
+            for (int i = 0; i < VEC; i += 2) {
+                const float2 e = unpair(fma2(pair(x[i], x[i + 1]), cc, bb));
+                s2 = add2(s2, pair(ex2(e.x), ex2(e.y)));
+            }
         };
-        if (MODE == M_BOTH) {
-            auto held_batch = [&](int b) {
-                for (int i = b * batch + tid; i < min(nh, (b + 1) * batch); i += D_THREADS) {
-                    uint4 u;
-                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n"
-                                 : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
-                                 : "r"(held + 16 * i));
-                    add(u, v0 + i);
-                }
-            };
+        int t = 0;
+        if (GRAD) {
             cp_wait<3>();
-            held_batch(0);
+            for (const int e = min(nth, bt); t < e; t++) add(held_vec(t), t);
             cp_wait<2>();
-            held_batch(1);
+            for (const int e = min(nth, 2 * bt); t < e; t++) add(held_vec(t), t);
             cp_wait<1>();
-            held_batch(2);
+            for (const int e = min(nth, 3 * bt); t < e; t++) add(held_vec(t), t);
             cp_wait<0>();
-            held_batch(3);
+            for (; t < nth; t++) add(held_vec(t), t);
         }
-        int v = v0 + nh + tid;
-        for (; v + 3 * D_THREADS < v1; v += 4 * D_THREADS) {
+        for (; t + 4 <= nt; t += 4) {
             uint4 u[4];
 #pragma unroll
-            for (int q = 0; q < 4; q++) u[q] = __ldg(zv + v + q * D_THREADS);
+            for (int q = 0; q < 4; q++) u[q] = __ldg(zt + (t + q) * D_THREADS);
 #pragma unroll
-            for (int q = 0; q < 4; q++) add(u[q], v + q * D_THREADS);
+            for (int q = 0; q < 4; q++) add(u[q], t + q);
         }
-        for (; v < v1; v += D_THREADS) add(__ldg(zv + v), v);
+        for (; t < nt; t++) add(__ldg(zt + t * D_THREADS), t);
+        const float2 e = unpair(s2);
+        s = e.x + e.y;
         auto scalar = [&](int j) {
-            if (!(REST && is_member(j))) {
-                const float x = __fmul_rn(to_f(z[j]), c);
-                const float M = fmaxf(m, x), b = M == -INFINITY ? 0.f : M;
-                s = __fmaf_rn(s, ex2(m - b), ex2(x - b));
-                m = M;
-            }
+            if (REST && (bits[(j - jb) >> 5] >> ((j - jb) & 31) & 1u)) return;
+            join(m, s, __fmul_rn(to_f(sl.z[j]), c), 1.f);
         };
-        if (rank == 0 && tid < head) scalar(tid);
-        if (rank == cl - 1 && head + nb * VEC + tid < V) scalar(head + nb * VEC + tid);
-        warp_join(m, s);
+        if (rank == 0 && tid < sl.head) scalar(tid);
+        if (rank == cl - 1 && sl.tail() + tid < V) scalar(sl.tail() + tid);
+        warp_join<32>(m, s);
         if (lane == 0) red[0][warp] = m, red[1][warp] = s;
-    }
-    // the slots' sums, on the last warp: p_k into pr, P, the entropy term, the pair of this CTA's tokens
-    if (warp == WARPS - 1) {
-        float lt;  // the teacher's log-sum-exp
-        if (REST) lt = p.lse[row];
-        else {
-            float um = -INFINITY, t = 0.f;
-            for (int k = lane; k < K; k += 32) um = fmaxf(um, pr[k]);
-            um = warp_reduce<0>(um);
-            const float b = um == -INFINITY ? 0.f : um;
-            for (int k = lane; k < K; k += 32) t += ex2(__fmul_rn(pr[k] - b, LOG2E));
-            t = warp_reduce<1>(t);
-            lt = t == 0.f ? 0.f : b + logf(t);  // no live slot, or all of them -inf: p = 0
+    } else {  // the slots' sums
+        float psum, prest, plogp, mt = -INFINITY, st = 0.f;
+        teacher_probabilities<REST>(p, REST ? p.lse[row] : 0.f, pr, id, lane, psum, prest, plogp);
+        if (REST) {
+            for (int k = lane; k < K; k += 32)
+                if (id[k] >= 0 && id[k] >= sl.j0 && id[k] < sl.j1 && (!any_dup || leads(id, k))) join(mt, st, zk[k], 1.f);
+            warp_join<32>(mt, st);
         }
-        float psum = 0.f, plogp = 0.f, mt = -INFINITY, st = 0.f, distinct = 0.f;
-        for (int k = lane; k < K; k += 32) {
-            const int i = id[k];
-            float pk = 0.f;
-            if (i >= 0) {
-                const float lp = pr[k] - lt;
-                pk = ex2(__fmul_rn(lp, LOG2E));
-                psum += pk;
-                if (!(pk == 0.f)) plogp = __fmaf_rn(pk, lp, plogp);
-                if (REST && MODE != M_GRAD && i >= j0 && i < j1 && leads(k)) join(mt, st, zk[k], 1.f);
-                if (REST && K >= V) {
-                    bool first = true;
-                    for (int q = 0; q < k && first; q++) first = id[q] != i;
-                    distinct += first ? 1.f : 0.f;
-                }
-            }
-            pr[k] = pk;
-        }
-        psum = warp_reduce<1>(psum);
-        plogp = warp_reduce<1>(plogp);
-        if (REST && MODE != M_GRAD) warp_join(mt, st);
-        float prest = REST ? fmaxf(1.f - psum, 0.f) : 0.f;
-        if (REST && K >= V && warp_reduce<1>(distinct) == (float)V) prest = 0.f;  // slots that hold every token leave no rest
         if (lane == 0) slot_sums[0] = psum, slot_sums[1] = prest, slot_sums[2] = plogp, slot_sums[3] = mt, slot_sums[4] = st;
     }
     __syncthreads();
     const float psum = slot_sums[0], prest = slot_sums[1];
-
-    float log2S, log2qr;  // log2 of S and of q_r
-    if (MODE != M_GRAD) {
-        m = lane < WARPS ? red[0][lane] : -INFINITY;
-        s = lane < WARPS ? red[1][lane] : 0.f;
-        warp_join(m, s);
-        float mt = slot_sums[3], st = slot_sums[4];
-        if (cl > 1) {
-            cluster_wait();
-            if (tid < cl) {
-                st_cluster_u32(&xch[0][rank], tid, __float_as_uint(m));
-                st_cluster_u32(&xch[1][rank], tid, __float_as_uint(s));
-                st_cluster_u32(&xch[2][rank], tid, __float_as_uint(mt));
-                st_cluster_u32(&xch[3][rank], tid, __float_as_uint(st));
-            }
-            cluster_arrive();
-            cluster_wait();
-            m = mt = -INFINITY, s = st = 0.f;
-            for (int q = 0; q < cl; q++) join(m, s, xch[0][q], xch[1][q]), join(mt, st, xch[2][q], xch[3][q]);
+    float m = red[0][lane & (WARPS - 1)], s = red[1][lane & (WARPS - 1)], mt = slot_sums[3], st = slot_sums[4];
+    warp_join<WARPS>(m, s);
+    if (cl > 1) {
+        cluster_wait();
+        if (tid < cl) {
+            st_cluster_u32(&xch[0][rank], tid, __float_as_uint(m));
+            st_cluster_u32(&xch[1][rank], tid, __float_as_uint(s));
+            st_cluster_u32(&xch[2][rank], tid, __float_as_uint(mt));
+            st_cluster_u32(&xch[3][rank], tid, __float_as_uint(st));
         }
-        float ma = m, sa = s;
-        if (REST) join(ma, sa, mt, st);
-        log2S = ma + log2f(sa);
-        log2qr = !REST || s == 0.f ? -INFINITY : m + log2f(s) - log2S;
-        if (rank == 0 && warp == 0) {
-            float l = 0.f;
-            const float b = log2S == -INFINITY ? 0.f : log2S;
-            for (int k = lane; k < K; k += 32)
-                if (!(pr[k] == 0.f)) l = __fmaf_rn(-pr[k], __fmul_rn(zk[k] - b, LN2), l);
-            l = warp_reduce<1>(l) + slot_sums[2];
-            if (lane == 0) {
-                if (prest > 0.f) l = __fmaf_rn(prest, __fmaf_rn(-log2qr, LN2, logf(prest)), l);
-                p.loss[row] = __fmul_rn(w, l);
-                if (p.stats) p.stats[2 * row] = log2S * LN2, p.stats[2 * row + 1] = log2qr * LN2;
-            }
+        if (warp == 0) cluster_arrive();
+        else cluster_arrive_relaxed();
+        cluster_wait();
+        const int q = lane & (D_MAXCL - 1);
+        m = q < cl ? xch[0][q] : -INFINITY, s = q < cl ? xch[1][q] : 0.f;
+        warp_join<D_MAXCL>(m, s);
+        if (REST) {
+            mt = q < cl ? xch[2][q] : -INFINITY, st = q < cl ? xch[3][q] : 0.f;
+            warp_join<D_MAXCL>(mt, st);
         }
-    } else {
-        log2S = p.stats[2 * row] * LOG2E;
-        log2qr = p.stats[2 * row + 1] * LOG2E;
-        if (cl > 1) cluster_wait();
     }
-
-    if (MODE != M_LOSS) {
-        const float g = MODE == M_GRAD && p.grad ? p.grad[row * p.s_grad] : 1.f;
-        const float scale = g * w * p.inv_tau;
-        const float P = psum + prest;
-        // outside the slots: scale (P - p_r / q_r) 2^(z c - log2 S); a rest that the student gives nothing has q_j = 0
-        const float cr = scale * (prest > 0.f ? (log2qr == -INFINITY ? 0.f : P - prest * ex2(-log2qr)) : P);
+    float ma = m, sa = s;
+    if (REST) join(ma, sa, mt, st);
+    const float log2S = ma + log2f(sa);
+    const float log2qr = !REST || s == 0.f ? -INFINITY : m + log2f(s) - log2S;
+    if (rank == 0 && warp == WARPS) {
+        float l = 0.f;
         const float b = log2S == -INFINITY ? 0.f : log2S;
-        auto grad_of = [&](float x) { return cr * ex2(fmaf(x, c, -b)); };
+        for (int k = lane; k < K; k += 32)
+            if (!(pr[k] == 0.f)) l = __fmaf_rn(-pr[k], __fmul_rn(zk[k] - b, LN2), l);
+        l = warp_reduce<1>(l) + slot_sums[2];
+        if (lane == 0) {
+            if (prest > 0.f) l = __fmaf_rn(prest, __fmaf_rn(-log2qr, LN2, logf(prest)), l);
+            p.loss[row] = __fmul_rn(w, l);
+            if (p.stats) p.stats[2 * row] = log2S * LN2, p.stats[2 * row + 1] = log2qr * LN2;
+        }
+    }
+    if (GRAD) {
+        const GradScale g(__fmul_rn(w, p.inv_tau), psum, prest, log2S, log2qr);
         if (p.vec_out) {
-            auto put = [&](const uint4& raw, int v) {
-                float x[VEC];
-                unpack16(raw, x, T());
-#pragma unroll
-                for (int i = 0; i < VEC; i++) x[i] = grad_of(x[i]);
-                __stcs(reinterpret_cast<uint4*>(dz + head + (long long)v * VEC), pack16(x, T()));
-            };
-            for (int i = tid; i < nh; i += D_THREADS) {
-                uint4 u;
-                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n"
-                             : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
-                             : "r"(held + 16 * i));
-                put(u, v0 + i);
-            }
+            const uint64_t bb = pair(-g.b, -g.b), rr = pair(g.cr, g.cr);
+            uint4* dt = reinterpret_cast<uint4*>(dz + sl.head) + sl.v0 + tid;
+            int t = 0;
+#pragma unroll 2
+            for (; t < nth; t++) __stcs(dt + t * D_THREADS, grad16<T>(held_vec(t), cc, bb, rr));
             // plain loads: the rows may be overwritten (dz = z), each vector by the thread that has read it
-            int v = v0 + nh + tid;
-            for (; v + 3 * D_THREADS < v1; v += 4 * D_THREADS) {
-                uint4 u[4];
-#pragma unroll
-                for (int q = 0; q < 4; q++) u[q] = zv[v + q * D_THREADS];
-#pragma unroll
-                for (int q = 0; q < 4; q++) put(u[q], v + q * D_THREADS);
-            }
-            for (; v < v1; v += D_THREADS) put(zv[v], v);
-            if (rank == 0 && tid < head) dz[tid] = from_f<T>(grad_of(to_f(z[tid])));
-            if (rank == cl - 1 && head + nb * VEC + tid < V)
-                dz[head + nb * VEC + tid] = from_f<T>(grad_of(to_f(z[head + nb * VEC + tid])));
+#pragma unroll 4
+            for (; t < nt; t++) __stcs(dt + t * D_THREADS, grad16<T>(zt[t * D_THREADS], cc, bb, rr));
+            auto scalar = [&](int j) { dz[j] = from_f<T>(g.cr * ex2(fmaf(to_f(sl.z[j]), c, -g.b))); };
+            if (rank == 0 && tid < sl.head) scalar(tid);
+            if (rank == cl - 1 && sl.tail() + tid < V) scalar(sl.tail() + tid);
         } else
-            for (int j = j0 + tid; j < j1; j += D_THREADS) dz[j] = from_f<T>(grad_of(to_f(z[j])));
+            for (int j = sl.j0 + tid; j < sl.j1; j += ALL) dz[j] = from_f<T>(g.cr * ex2(fmaf(to_f(sl.z[j]), c, -g.b)));
         __syncthreads();
-        for (int k = tid; k < K; k += D_THREADS) {
-            if (id[k] < 0 || id[k] < j0 || id[k] >= j1 || !leads(k)) continue;
+        for (int k = tid; k < K; k += ALL) {
+            if (id[k] < 0 || id[k] < sl.j0 || id[k] >= sl.j1 || (any_dup && !leads(id, k))) continue;
             float pk = pr[k];
             if (any_dup)
                 for (int q = k + 1; q < K; q++)
                     if (id[q] == id[k]) pk += pr[q];
-            dz[id[k]] = from_f<T>(scale * (P * ex2(zk[k] - b) - pk));
+            dz[id[k]] = from_f<T>(g.scale * (g.P * ex2(zk[k] - g.b) - pk));
         }
     }
 }
 
-template <typename T, int MODE, bool REST>
-int launch(DistillParams p, int cl, cudaStream_t st)
+// the gradient alone, from the statistics: one pass, a CTA per row
+template <typename T, bool REST>
+__global__ void __launch_bounds__(D_THREADS) distill_grad_kernel(const DistillParams p)
+{
+    extern __shared__ __align__(16) uint32_t dsm[];
+    __shared__ float sums[2];
+    float* pr = reinterpret_cast<float*>(dsm);
+    int* id = reinterpret_cast<int*>(pr + p.K);
+    const int tid = threadIdx.x, lane = tid & 31, K = p.K, V = p.V;
+    const long long row = blockIdx.x;
+    const Slice<T> sl(p, row, 0);
+    T* dz = (T*)p.dz + row * p.ld_d;
+    const float w = p.weight ? p.weight[row] : 1.f;
+    if (w == 0.f) {
+        zero_slice(p, sl, dz, 0, tid, D_THREADS);
+        return;
+    }
+    const float c = p.inv_tau * LOG2E;
+    float* zk = reinterpret_cast<float*>(id + K);
+    for (int k = tid; k < K; k += D_THREADS) {
+        load_slot(p, row, k, id[k], pr[k]);
+        if (id[k] >= 0) zk[k] = __fmul_rn(to_f(sl.z[id[k]]), c);
+    }
+    __syncthreads();
+    if (tid < 32) {
+        float psum, prest, plogp;
+        teacher_probabilities<REST>(p, REST ? p.lse[row] : 0.f, pr, id, lane, psum, prest, plogp);
+        if (lane == 0) sums[0] = psum, sums[1] = prest;
+    }
+    __syncthreads();
+    const float up = p.grad ? p.grad[row * p.s_grad] : 1.f;
+    const GradScale g(up * w * p.inv_tau, sums[0], sums[1], p.stats[2 * row] * LOG2E, p.stats[2 * row + 1] * LOG2E);
+    if (p.vec_out) {
+        const uint64_t cc = pair(c, c), bb = pair(-g.b, -g.b), rr = pair(g.cr, g.cr);
+        // plain loads: the rows may be overwritten (dz = z), each vector by the thread that has read it
+        const uint4* zt = reinterpret_cast<const uint4*>(sl.z + sl.head);
+        uint4* dt = reinterpret_cast<uint4*>(dz + sl.head);
+        int v = tid;
+        for (; v + 3 * D_THREADS < sl.nb; v += 4 * D_THREADS) {
+            uint4 u[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) u[q] = zt[v + q * D_THREADS];
+#pragma unroll
+            for (int q = 0; q < 4; q++) __stcs(dt + v + q * D_THREADS, grad16<T>(u[q], cc, bb, rr));
+        }
+        for (; v < sl.nb; v += D_THREADS) __stcs(dt + v, grad16<T>(zt[v], cc, bb, rr));
+        auto scalar = [&](int j) { dz[j] = from_f<T>(g.cr * ex2(fmaf(to_f(sl.z[j]), c, -g.b))); };
+        if (tid < sl.head) scalar(tid);
+        if (sl.tail() + tid < V) scalar(sl.tail() + tid);
+    } else
+        for (int j = tid; j < V; j += D_THREADS) dz[j] = from_f<T>(g.cr * ex2(fmaf(to_f(sl.z[j]), c, -g.b)));
+    __syncthreads();
+    for (int k = tid; k < K; k += D_THREADS) {
+        if (id[k] < 0 || !leads(id, k)) continue;
+        float pk = pr[k];
+        for (int q = k + 1; q < K; q++)
+            if (id[q] == id[k]) pk += pr[q];
+        dz[id[k]] = from_f<T>(g.scale * (g.P * ex2(zk[k] - g.b) - pk));
+    }
+}
+
+// CTAs of a row.  With gradient one where the row fits D_ROW (three CTAs an SM and no cluster barrier: 4096 x 32000 fp16 111 us,
+// two CTAs of half a row 123 us), else as few as let a slice stay in D_SLICE (four an SM: 4096 x 128256 bf16 384 us with 52 KB
+// slices, 397 us with 36, 395 us with 66 KB).  Without gradient one.  Few rows: more, until the GPU's SMs have one each.
+int row_ctas(long long T, int V, int es, bool grad)
+{
+    const long long bytes = (long long)V * es;
+    int cl = grad && bytes > D_ROW ? (int)((bytes + D_SLICE - 1) / D_SLICE) : 1;
+    while (cl < D_MAXCL && T * cl < 148 && bytes / cl > 16 * 1024) cl *= 2;
+    return cl < D_MAXCL ? cl : D_MAXCL;
+}
+
+template <typename T, bool GRAD, bool REST>
+int launch_rows(DistillParams p, cudaStream_t st)
 {
     constexpr int VEC = 16 / sizeof(T);
-    const int per = (p.V / VEC + cl - 1) / cl;
+    auto k = distill_rows_kernel<T, GRAD, REST>;
+    p.cl = row_ctas(p.T, p.V, sizeof(T), GRAD);
+    const int per = (p.V / VEC + p.cl - 1) / p.cl;
     p.bit_words = (((per + 2) * VEC + 31) / 32 + 3) / 4 * 4;
-    p.hold = MODE == M_BOTH ? per : 0;
     const int fixed = p.bit_words * 4 + p.K * 12;
+    p.hold = GRAD ? per : 0;
     if (fixed + p.hold * 16 > D_SMEM) p.hold = (D_SMEM - fixed) / 16;
     const int smem = fixed + p.hold * 16;
-    auto k = distill_kernel<T, MODE, REST>;
     if (smem > 46 * 1024) {  // beyond the default 48 KB with the static arrays
         static std::atomic<int> ready[64];
         int dev = 0;
@@ -425,37 +531,33 @@ int launch(DistillParams p, int cl, cudaStream_t st)
         }
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((long long)p.T * cl));
-    cfg.blockDim = dim3(D_THREADS);
+    cfg.gridDim = dim3((unsigned)((long long)p.T * p.cl));
+    cfg.blockDim = dim3(D_THREADS + 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim = {(unsigned)cl, 1, 1};
+    at[0].val.clusterDim = {(unsigned)p.cl, 1, 1};
     cfg.attrs = at;
-    cfg.numAttrs = cl > 1 ? 1 : 0;
+    cfg.numAttrs = p.cl > 1 ? 1 : 0;
     return (int)cudaLaunchKernelEx(&cfg, k, p);
 }
 
-// CTAs of a row.  Loss and gradient: as few as let a slice stay in 72 KB of shared memory (three CTAs an SM, one row's
-// loads under another's exponentials and stores), so that the row is read from memory once; otherwise one.  Few rows: more, until
-// the GPU's SMs have one each.
-int row_ctas(long long T, int V, int es, int mode)
+template <typename T, bool REST>
+int launch_grad(DistillParams p, cudaStream_t st)
 {
-    int cl = 1;
-    if (mode == M_BOTH)
-        while (cl < D_MAXCL && (long long)V * es > 72 * 1024LL * cl) cl *= 2;
-    while (cl < D_MAXCL && T * cl < 148 && (long long)V * es / cl > 16 * 1024) cl *= 2;
-    return cl;
+    p.cl = 1;
+    distill_grad_kernel<T, REST><<<p.T, D_THREADS, p.K * 12, st>>>(p);
+    return (int)cudaGetLastError();
 }
 
 template <typename T>
-int dispatch(const DistillParams& p, int mode, int cl, cudaStream_t st)
+int dispatch(const DistillParams& p, int mode, cudaStream_t st)
 {
     const bool rest = p.lse != nullptr;
-    if (mode == M_LOSS) return rest ? launch<T, M_LOSS, true>(p, cl, st) : launch<T, M_LOSS, false>(p, cl, st);
-    if (mode == M_BOTH) return rest ? launch<T, M_BOTH, true>(p, cl, st) : launch<T, M_BOTH, false>(p, cl, st);
-    return rest ? launch<T, M_GRAD, true>(p, cl, st) : launch<T, M_GRAD, false>(p, cl, st);
+    if (mode == M_LOSS) return rest ? launch_rows<T, false, true>(p, st) : launch_rows<T, false, false>(p, st);
+    if (mode == M_BOTH) return rest ? launch_rows<T, true, true>(p, st) : launch_rows<T, true, false>(p, st);
+    return rest ? launch_grad<T, true>(p, st) : launch_grad<T, false>(p, st);
 }
 
 }  // namespace
@@ -480,9 +582,8 @@ extern "C" int ltq_distill_topk(const void* logits, int dtype, long long ld, con
     p.weight = weight, p.grad = grad, p.s_grad = grad_stride, p.loss = loss, p.stats = stats, p.dz = dlogits, p.ld_d = ld_d;
     p.T = T, p.V = V, p.K = K, p.idx64 = idx64 != 0, p.u_dt = teacher_dtype, p.inv_tau = 1.f / temperature;
     p.vec_out = mode != M_LOSS && ((uintptr_t)logits & 15) == ((uintptr_t)dlogits & 15) && ((ld - ld_d) * es) % 16 == 0;
-    const int cl = p.cl = row_ctas(T, V, es, mode);
     const cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == DT_F32) return dispatch<float>(p, mode, cl, st);
-    if (dtype == DT_BF16) return dispatch<__nv_bfloat16>(p, mode, cl, st);
-    return dispatch<__half>(p, mode, cl, st);
+    if (dtype == DT_F32) return dispatch<float>(p, mode, st);
+    if (dtype == DT_BF16) return dispatch<__nv_bfloat16>(p, mode, st);
+    return dispatch<__half>(p, mode, st);
 }

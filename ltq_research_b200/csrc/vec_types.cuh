@@ -48,6 +48,75 @@ __device__ __forceinline__ void unpack16(const uint4& u, float (&f)[8], __half)
         f[2 * i] = p.x, f[2 * i + 1] = p.y;
     }
 }
+// two fp32 values in a 64-bit register pair, and products and sums of both in one instruction
+__device__ __forceinline__ uint64_t pair(float x, float y)
+{
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v)
+{
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// the largest element of 16 bytes of T (NaN only where all are)
+__device__ __forceinline__ float max16(const uint4& u, float)
+{
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+}
+__device__ __forceinline__ float max16(const uint4& u, __nv_bfloat16)
+{
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float max16(const uint4& u, __half)
+{
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+// 16 bytes of T with the elements of `mask` (bit i: element i) replaced by -infinity
+__device__ __forceinline__ uint4 mask16(uint4 u, uint32_t mask, float)
+{
+    uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (mask >> i & 1u) w[i] = 0xff800000u;
+    return u;
+}
+__device__ __forceinline__ uint4 mask16_16(uint4 u, uint32_t mask, uint32_t inf)
+{
+    uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (mask >> (2 * i) & 1u) w[i] = (w[i] & 0xffff0000u) | inf;
+        if (mask >> (2 * i + 1) & 1u) w[i] = (w[i] & 0xffffu) | inf << 16;
+    }
+    return u;
+}
+__device__ __forceinline__ uint4 mask16(uint4 u, uint32_t mask, __nv_bfloat16) { return mask16_16(u, mask, 0xff80u); }
+__device__ __forceinline__ uint4 mask16(uint4 u, uint32_t mask, __half) { return mask16_16(u, mask, 0xfc00u); }
 __device__ __forceinline__ uint4 pack16(const float (&f)[4], float)
 {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
@@ -73,13 +142,15 @@ __device__ __forceinline__ uint4 pack16(const float (&f)[8], __half)
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// barrier of the cluster's CTAs: shared and global writes before it are seen by all of them after it
+// barrier of the cluster's CTAs: shared and global writes before it are seen by all of them after it (those of a thread that
+// arrives relaxed need not be)
 __device__ __forceinline__ uint32_t cluster_rank()
 {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
     return r;
 }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
 // writes a 32-bit word at `p` of this CTA's shared memory into the same place of CTA `rank`
