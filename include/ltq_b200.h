@@ -343,6 +343,14 @@ size_t ltq_fp8_gemm_workspace_bytes(int M, int N, int K);
 int ltq_fp8_gemm(const uint8_t* A, long long lda, const float* sa, long long ld_sa, const uint8_t* B, long long ldb,
                  const float* sb, long long ld_sb, void* C, int dtype, long long ldc, int M, int N, int K,
                  void* workspace, size_t workspace_bytes, int* err, void* stream);
+/*
+ * ltq_fp8_few: y[m, n] = sum_b sx[m, b] sw[(n / 128) * ld_sw + b] sum_{k in block b} xq[m, k] W[n, k] for 1 to 64 rows x [M, K]
+ *   (dtype), quantized in the call as ltq_fp8_quant_rows does; y [M, N] of out_dtype.  One launch, no workspace.  For shapes that
+ *   ltq_fp8_few_supported names (1; else 0: use ltq_fp8_quant_rows and ltq_fp8_gemm).
+ */
+int ltq_fp8_few_supported(int M, int N, int K);
+int ltq_fp8_few(const void* x, int dtype, long long ldx, const uint8_t* W, long long ldw, const float* sw, long long ld_sw,
+                void* y, int out_dtype, long long ldy, int M, int N, int K, int* err, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,48 @@
+// Pieces of the e4m3 tensor-core products (sm_100a).
+#pragma once
+#include "tc_pipe.cuh"
+#include "fp8_quant.cuh"
+
+namespace {
+
+constexpr uint32_t WAIT_LIMIT = 1u << 24;
+
+// instruction descriptor, kind::f8f6f4: D fp32 (bits 4-5 = 1), A and B e4m3 (bits 7-9, 10-12 = 0), both K-major
+__host__ __device__ constexpr uint32_t idesc_f8(int m, int n)
+{
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// one lane of a converged warp, always the same
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
+}
+
+inline bool make_map_8(CUtensorMap* m, const void* base, long long rows, long long cols, long long ld, int box_rows)
+{
+    auto f = encode_fn();
+    if (!f) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld};
+    cuuint32_t box[2] = {QB, (cuuint32_t)box_rows}, one[2] = {1, 1};
+    return f(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+inline int sm_count()
+{
+    static std::atomic<int> n[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    int v = n[dev].load(std::memory_order_relaxed);
+    if (!v) {
+        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+        n[dev].store(v, std::memory_order_relaxed);
+    }
+    return v;
+}
+
+inline bool bad_operand(const void* q, long long ld, int K) { return !q || (uintptr_t)q % 16 || ld % 16 || ld < K; }
+
+}  // namespace

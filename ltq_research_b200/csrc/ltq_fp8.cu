@@ -3,27 +3,17 @@
 //
 // 128 values: s = max |x| / 448 (at least 2^-126), q = e4m3(x / s), an fp32 quotient rounded to nearest even; a block with a
 // NaN or an infinity becomes NaN.  Activations: one scale per row and 128 columns; weights: one per 128 x 128 block.
-#include <cuda_fp8.h>
 #include "ltq_b200.h"
-#include "vec_types.cuh"
+#include "fp8_quant.cuh"
 
 namespace {
 
-constexpr int QB = 128;
-constexpr float E4M3_MAX = 448.f, S_MIN = 1.17549435e-38f;
-
-__device__ __forceinline__ float block_scale(uint32_t amax_bits)  // the largest |x| by its bits: NaN above infinity
-{
-    const float s = __fdiv_rn(__uint_as_float(amax_bits), E4M3_MAX);
-    return s < S_MIN ? S_MIN : s;
-}
 __device__ __forceinline__ uint32_t quant4(const float (&x)[4], float s)
 {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x[0], s), __fdiv_rn(x[1], s)), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x[2], s), __fdiv_rn(x[3], s)), __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
 }
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 // four elements of a row from column c on (zeros beyond K)
 template <typename T>
@@ -47,41 +37,6 @@ __device__ __forceinline__ void store4(uint8_t* row, int c, int K, uint32_t q)
 // Activations.  A warp takes 1024 columns of ROWS rows, eight columns a lane and load (16 bytes of a 16-bit type), so a block
 // of 128 is half a warp's load and the maximum four exchanges; a row's loads are in flight while the row before it is worked on.  The scales of a
 // CTA's rows are gathered in shared memory and leave as one run of rows per block, the layout the products read.
-// The quotient x / s is rounded correctly without a division each: with r = 1 / s correctly rounded, q = x r and then
-// q + (x - q s) r is the correctly rounded quotient (Markstein's correction, IBM J. Res. Dev. 34, 1990) while the remainder
-// stays above the smallest normal number, which 2^-80 <= s guarantees for every quotient that e4m3 does not round to 0;
-// smaller scales take the division.  128 MB of bf16 in, 64 MB out: see the measured rate at the launch.
-__device__ __forceinline__ float quotient(float x, float s, float r)
-{
-    const float q = __fmul_rn(x, r);
-    return __fmaf_rn(__fmaf_rn(-q, s, x), r, q);
-}
-// eight elements of a row from column c on (zeros beyond K), as they are
-template <typename T>
-struct Raw8 {
-    uint4 u[sizeof(T) / 2];
-};
-template <typename T>
-__device__ __forceinline__ void load8(const T* row, int c, int K, bool aligned, Raw8<T>& x)
-{
-    if (aligned && c + 8 <= K) {
-#pragma unroll
-        for (int h = 0; h < (int)sizeof(T) / 2; h++) x.u[h] = __ldg(reinterpret_cast<const uint4*>(row + c) + h);
-    } else {
-        T t[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) t[i] = c + i < K ? row[c + i] : from_f<T>(0.f);
-        memcpy(&x, t, sizeof(x));
-    }
-}
-__device__ __forceinline__ void unpack8(const Raw8<float>& x, float (&f)[8])
-{
-    f[0] = __uint_as_float(x.u[0].x), f[1] = __uint_as_float(x.u[0].y), f[2] = __uint_as_float(x.u[0].z), f[3] = __uint_as_float(x.u[0].w);
-    f[4] = __uint_as_float(x.u[1].x), f[5] = __uint_as_float(x.u[1].y), f[6] = __uint_as_float(x.u[1].z), f[7] = __uint_as_float(x.u[1].w);
-}
-__device__ __forceinline__ void unpack8(const Raw8<__nv_bfloat16>& x, float (&f)[8]) { unpack16(x.u[0], f, __nv_bfloat16()); }
-__device__ __forceinline__ void unpack8(const Raw8<__half>& x, float (&f)[8]) { unpack16(x.u[0], f, __half()); }
-
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) quant_rows_kernel(const T* __restrict__ x, long long ld, int M, int K,
                                                          uint8_t* __restrict__ q, long long ld_q, float* __restrict__ s,
@@ -106,28 +61,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) quant_rows_kernel
         for (int j = 0; j < 4; j++) {
             float v[8];
             unpack8(cur[j], v);
-            uint32_t a = 0;
-#pragma unroll
-            for (int i = 0; i < 8; i++) a = max(a, abs_bits(v[i]));
-#pragma unroll
-            for (int o = 8; o; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-            const float scale = block_scale(a), r = __frcp_rn(scale);
-            if (!(scale >= 0x1p-80f)) {  // a tiny scale, or NaN
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = __fdiv_rn(v[i], scale);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = quotient(v[i], scale, r);
-            }
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                w[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+            const float scale = block_scale(half_warp_amax(v));
+            const uint2 w = quant8(v, scale);
             const int c = c0 + 256 * j + 8 * lane;
             uint8_t* o = q + m * ld_q + c;
-            if (c + 8 <= K) *reinterpret_cast<uint2*>(o) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+            if (c + 8 <= K) *reinterpret_cast<uint2*>(o) = w;
             else
-                for (int i = 0; c + i < K; i++) o[i] = (uint8_t)(w[i >> 1] >> (8 * (i & 1)));
+                for (int i = 0; c + i < K; i++) o[i] = (uint8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
             if ((lane & 15) == 0) sc[2 * j + (lane >> 4)][m - mb] = scale;
         }
     }

@@ -19,13 +19,10 @@
 // along K into equal shares (a share may end inside a tile); the parts go to a workspace and join_parts_kernel adds them in the
 // order of K.  Every wait is bounded: when one runs out *err is set, the role stops and the CTAs still meet at their last barrier.
 #include "ltq_b200.h"
-#include "tc_pipe.cuh"
+#include "fp8_tc.cuh"
 #include "vec_types.cuh"
 
 namespace {
-
-constexpr int QB = 128;  // K block: the width of a scale
-constexpr uint32_t WAIT_LIMIT = 1u << 24;
 
 // ------------------------------------------------------------------------------------------------ cta_group::2 pieces
 
@@ -56,11 +53,6 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar)  // arrives on both C
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(smem_u32(bar)),
         "h"((uint16_t)3)
         : "memory");
-}
-// instruction descriptor, kind::f8f6f4: D fp32 (bits 4-5 = 1), A and B e4m3 (bits 7-9, 10-12 = 0), both K-major
-__host__ __device__ constexpr uint32_t idesc_f8(int m, int n)
-{
-    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 __device__ __forceinline__ void mma_f8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {
@@ -152,13 +144,6 @@ struct Walk {
         return true;
     }
 };
-
-__device__ __forceinline__ bool elect_one()
-{
-    uint32_t p;
-    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
-    return p != 0;
-}
 
 template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
@@ -410,16 +395,6 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const WideArgs g)
 
 // ---------------------------------------------------------------------------------------------------------- host side
 
-bool make_map_8(CUtensorMap* m, const void* base, long long rows, long long cols, long long ld, int box_rows)
-{
-    auto f = encode_fn();
-    if (!f) return false;
-    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)ld};
-    cuuint32_t box[2] = {QB, (cuuint32_t)box_rows}, one[2] = {1, 1};
-    return f(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
 bool make_map_out(CUtensorMap* m, void* base, int es, long long rows, long long cols, long long ld)
 {
     auto f = encode_fn();
@@ -430,19 +405,6 @@ bool make_map_out(CUtensorMap* m, void* base, int es, long long rows, long long 
     return f(m, es == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, dims, strides, box, one,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-int sm_count()
-{
-    static std::atomic<int> n[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-    int v = n[dev].load(std::memory_order_relaxed);
-    if (!v) {
-        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-        n[dev].store(v, std::memory_order_relaxed);
-    }
-    return v;
 }
 
 struct WidePlan {
@@ -487,8 +449,6 @@ int run_wide(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc
     join_parts_kernel<T><<<dim3(p.tiles - p.whole, 8), 256, 0, st>>>(g);
     return (int)cudaGetLastError();
 }
-
-bool bad_operand(const void* q, long long ld, int K) { return !q || (uintptr_t)q % 16 || ld % 16 || ld < K; }
 
 }  // namespace
 

@@ -94,6 +94,13 @@ inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn()
 {
     static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> fn{nullptr};
     PFN_cuTensorMapEncodeTiled_v12000 f = fn.load(std::memory_order_acquire);
+    // the encoder is a driver call: a thread whose first CUDA call it is (autograd's, say) has no context current yet
+    static thread_local bool bound = false;
+    if (!bound) {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return nullptr;
+        bound = true;
+    }
     if (!f) {
         void* ptr = nullptr;
         cudaDriverEntryPointQueryResult q;

@@ -23,6 +23,14 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return
 template <>
 __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
 
+// y[i] = v in the type of the code
+__device__ __forceinline__ void store_as(void* y, int dt, long long i, float v)
+{
+    if (dt == DT_F32) ((float*)y)[i] = v;
+    else if (dt == DT_BF16) ((__nv_bfloat16*)y)[i] = from_f<__nv_bfloat16>(v);
+    else ((__half*)y)[i] = from_f<__half>(v);
+}
+
 // V elements of T moved as one access of V * sizeof(T) bytes (2, 4, 8, 16 or 32: two of 16)
 template <typename T, int V>
 struct alignas(V * sizeof(T) > 16 ? 16 : V * sizeof(T)) Vec {

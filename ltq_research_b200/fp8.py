@@ -21,6 +21,7 @@ from . import _lib
 from ._lib import DTYPES, ptr
 
 BLOCK = 128
+FEW = 64  # rows up to which one launch quantizes them and streams the weight (ltq_fp8_few)
 E4M3 = torch.float8_e4m3fn
 
 
@@ -137,6 +138,10 @@ def _product(x: torch.Tensor, q: torch.Tensor, s: torch.Tensor, N: int, K: int, 
     from .liqk_v2 import gemm_error_flag
     L = _lib.lib()
     with _lib.on_device(dev):
+        if M <= FEW and L.ltq_fp8_few_supported(M, N, K):
+            _check(L.ltq_fp8_few(ptr(x2), DTYPES[x2.dtype], ld, ptr(q), q.stride(0), ptr(s), s.shape[1], ptr(y), DTYPES[dtype],
+                                 N, M, N, K, ptr(gemm_error_flag(dev)), _lib.stream_ptr(dev)), "ltq_fp8_few")
+            return y
         xq, xs = _quantize_rows(x2, ld)
         nws = L.ltq_fp8_gemm_workspace_bytes(M, N, K)
         ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
