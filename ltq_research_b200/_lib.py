@@ -153,7 +153,10 @@ def exported_symbols() -> list[str]:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream's handle on `device`."""
+    if device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)  # the same handle without a Stream object around it
 
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:
@@ -175,7 +178,10 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
 
 def on_device(device: torch.device):
     """Context with `device` current, as a launch on its streams needs."""
-    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _SAME if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+_SAME = nullcontext()
 
 
 def ptr(t) -> int | None:

@@ -32,19 +32,23 @@ LOSS, LOSS_AND_GRAD, GRAD = 0, 1, 2
 
 def _rows(t: torch.Tensor, what: str) -> int:
     """Row stride of a 2-D tensor with unit column stride and rows that do not overlap."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    if t.dim() != 2:
         raise ValueError(f"distill: {what} must be 2-D with unit column stride")
-    if t.shape[0] <= 1:
-        return max(t.shape[1], 1)
-    if t.stride(0) < t.shape[1]:
+    rows, cols = t.shape
+    ld, step = t.stride()
+    if cols > 1 and step != 1:
+        raise ValueError(f"distill: {what} must be 2-D with unit column stride")
+    if rows <= 1:
+        return max(cols, 1)
+    if ld < cols:
         raise ValueError(f"distill: the rows of {what} overlap")
-    return t.stride(0)
+    return ld
 
 
 def _vector(t: Optional[torch.Tensor], T: int, what: str) -> Optional[torch.Tensor]:
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.shape != (T,):
+    if t.dtype is not torch.float32 or t.shape != (T,):
         raise ValueError(f"distill: {what} must be fp32 of shape [{T}]")
     return t if t.is_contiguous() else t.contiguous()
 
@@ -118,7 +122,6 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
-@torch.no_grad()
 def topk_loss(logits: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor, *,
               teacher_lse: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
               temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -128,7 +131,6 @@ def topk_loss(logits: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor, *,
     return loss, stats
 
 
-@torch.no_grad()
 def topk_loss_grad(logits: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor, *,
                    teacher_lse: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
                    temperature: float = 1.0, out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -138,7 +140,6 @@ def topk_loss_grad(logits: torch.Tensor, idx: torch.Tensor, teacher: torch.Tenso
     return loss, d
 
 
-@torch.no_grad()
 def topk_grad(logits: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor, stats: torch.Tensor, *,
               grad: Optional[torch.Tensor] = None, teacher_lse: Optional[torch.Tensor] = None,
               weight: Optional[torch.Tensor] = None, temperature: float = 1.0,

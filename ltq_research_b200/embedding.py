@@ -34,7 +34,6 @@ def _row_stride(t: torch.Tensor, what: str) -> int:
     return t.stride(0)
 
 
-@torch.no_grad()
 def lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """scale * table[tokens]: table [V, D] fp32, bf16 or fp16, tokens of any shape -> [*tokens.shape, D]."""
@@ -59,7 +58,6 @@ def lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
     return out
 
 
-@torch.no_grad()
 def lookup_grad(tokens: torch.Tensor, dout: torch.Tensor, num_rows: int, scale: float = 1.0,
                 padding_idx: Optional[int] = None, out: Optional[torch.Tensor] = None, accumulate: bool = False,
                 dtype: torch.dtype = torch.float32) -> torch.Tensor:

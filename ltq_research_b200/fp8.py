@@ -33,6 +33,11 @@ def _pad16(n: int) -> int:
     return (n + 15) // 16 * 16
 
 
+def _error_flag(dev: torch.device) -> torch.Tensor:
+    from .liqk_v2 import gemm_error_flag  # the tensor-core products' common flag
+    return gemm_error_flag(dev)
+
+
 def _check(rc: int, what: str):
     if rc != 0:
         raise RuntimeError(f"{what}: error code {rc}")
@@ -124,41 +129,40 @@ def _product(x: torch.Tensor, q: torch.Tensor, s: torch.Tensor, N: int, K: int, 
     dtype = x.dtype if dtype is None else dtype
     if dtype not in DTYPES:
         raise TypeError("fp8: the output must be fp32, bf16 or fp16")
-    if x.dim() < 1 or x.shape[-1] != K:
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] != K:
         raise ValueError(f"fp8: the last dimension must be {K}")
     dev = _lib.require_cuda(x, q)
-    x2 = x if x.dim() == 2 else x.reshape(-1, K)
-    if (K > 1 and x2.stride(1) != 1) or (x2.shape[0] > 1 and x2.stride(0) < K):
+    x2 = x if len(shape) == 2 else x.reshape(-1, K)
+    M = x2.shape[0]
+    ld, step = x2.stride()
+    if (K > 1 and step != 1) or (M > 1 and ld < K):
         x2 = x2.contiguous()
     ld = _rows(x2, "x")
-    M = x2.shape[0]
-    y = torch.empty((*x.shape[:-1], N), dtype=dtype, device=dev)
+    y = torch.empty((*shape[:-1], N), dtype=dtype, device=dev)
     if M == 0:
         return y
-    from .liqk_v2 import gemm_error_flag
     L = _lib.lib()
     with _lib.on_device(dev):
+        st, err = _lib.stream_ptr(dev), ptr(_error_flag(dev))
         if M <= FEW and L.ltq_fp8_few_supported(M, N, K):
             _check(L.ltq_fp8_few(ptr(x2), DTYPES[x2.dtype], ld, ptr(q), q.stride(0), ptr(s), s.shape[1], ptr(y), DTYPES[dtype],
-                                 N, M, N, K, ptr(gemm_error_flag(dev)), _lib.stream_ptr(dev)), "ltq_fp8_few")
+                                 N, M, N, K, err, st), "ltq_fp8_few")
             return y
         xq, xs = _quantize_rows(x2, ld)
         nws = L.ltq_fp8_gemm_workspace_bytes(M, N, K)
         ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
         _check(L.ltq_fp8_gemm(ptr(xq), xq.shape[1], ptr(xs), xs.shape[1], ptr(q), q.stride(0), ptr(s), s.shape[1], ptr(y),
-                              DTYPES[dtype], N, M, N, K, ptr(ws), nws, ptr(gemm_error_flag(dev)), _lib.stream_ptr(dev)),
-               "ltq_fp8_gemm")
+                              DTYPES[dtype], N, M, N, K, ptr(ws), nws, err, st), "ltq_fp8_gemm")
     return y
 
 
-@torch.no_grad()
 def linear(x: torch.Tensor, W: BlockWeight, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """x W^T: x [..., K] fp32, bf16 or fp16 -> [..., N] in `dtype` (x's by default)."""
     N, K = W.shape
     return _product(x, W.q, W.s, N, K, dtype)
 
 
-@torch.no_grad()
 def linear_grad(dy: torch.Tensor, W: BlockWeight, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """dy W: the gradient [..., K] of linear's input by dy [..., N], dy quantized per row and 128 columns."""
     if W.qt is None:
