@@ -303,7 +303,7 @@ int ltq_viterbi_tb_noalloc(const float* x, const float* w, int w_stride, const f
  *   log-sum-exp of all the teacher's logits / temperature) p_k = exp(u_k / temperature - lse) and the remaining mass
  *   p_r = max(0, 1 - sum p) is one outcome, against the student's mass q_r outside the slots.  weight [T] (or NULL: 1):
  *       loss = weight (sum p (log p - log q) + p_r (log p_r - log q_r))
- *   mode 0: loss [T], and stats [T, 2] = (log-sum-exp of z / temperature, log q_r) when not NULL; mode 1: the same and
+ *   mode 0: loss [T], and stats [T, 3] = (m, s, r) when not NULL: sum exp(z / temperature) = s 2^m, q_r = 2^r; mode 1: the same and
  *   dlogits = d loss / d logits (dtype, row stride ld_d; may be `logits` itself with ld_d = ld); mode 2: dlogits alone, from
  *   stats, times grad[t * grad_stride] (or NULL: 1).  Terms with p = 0 are 0; a row without a live slot has loss and gradient
  *   0, as has a row of weight 0, whose logits are not read; slots that name one token add up.  V <= 2^20, K <= 1024.

@@ -39,7 +39,7 @@ struct DistillParams {
     const float* grad;    // M_GRAD: upstream gradient of the loss, or NULL
     long long s_grad;
     float* loss;
-    float* stats;  // [T][2]: log S, log q_r (natural logarithms)
+    float* stats;  // [T][3]: S as sa 2^ma (ma, sa), log2 q_r
     void* dz;
     long long ld_d;
     int T, V, K, idx64, u_dt;
@@ -132,32 +132,35 @@ __device__ __forceinline__ void load_slot(const DistillParams& p, long long row,
     const long long i = p.idx64 ? ((const long long*)p.idx)[row * p.ld_idx + k] : ((const int*)p.idx)[row * p.ld_idx + k];
     const float t = load_u(p.u, p.u_dt, row * p.ld_u + k);
     id = i >= 0 && i < p.V ? (int)i : -1;
-    u = id >= 0 ? __fmul_rn(t, p.inv_tau) : -INFINITY;
+    u = id >= 0 ? t : -INFINITY;
 }
 
-// p_k into pr (from u / tau) on one warp; returns P's two parts and sum p log p
+// p_k into pr (from u) on one warp; returns P's two parts and sum p log p.  log p is formed from differences, small where p is
+// large: u / tau and the log-sum-exp alone would each be rounded to their own size.
 template <bool REST>
 __device__ __forceinline__ void teacher_probabilities(const DistillParams& p, float lse, float* pr, const int* id, int lane,
                                                       float& psum, float& prest, float& plogp)
 {
     const int K = p.K;
-    float lt = lse;  // the teacher's log-sum-exp
+    float um = 0.f, lt = 0.f, inv = 0.f;  // without rest: the largest u, log and reciprocal of the sum relative to it
     if (!REST) {
-        float um = -INFINITY, t = 0.f;
+        um = -INFINITY;
         for (int k = lane; k < K; k += 32) um = fmaxf(um, pr[k]);
         um = warp_reduce<0>(um);
-        const float b = um == -INFINITY ? 0.f : um;
-        for (int k = lane; k < K; k += 32) t += ex2(__fmul_rn(pr[k] - b, LOG2E));
+        if (um == -INFINITY) um = 0.f;
+        float t = 0.f;
+        for (int k = lane; k < K; k += 32) t += expf(__fmul_rn(pr[k] - um, p.inv_tau));
         t = warp_reduce<1>(t);
-        lt = t == 0.f ? 0.f : b + logf(t);  // no live slot, or all of them -inf: p = 0
+        if (t != 0.f) lt = logf(t), inv = 1.f / t;  // else no live slot, or all of them -inf: p = 0
     }
     float distinct = 0.f;
     psum = plogp = 0.f;
     for (int k = lane; k < K; k += 32) {
         float pk = 0.f;
         if (id[k] >= 0) {
-            const float lp = pr[k] - lt;
-            pk = ex2(__fmul_rn(lp, LOG2E));
+            const float d = REST ? __fmaf_rn(pr[k], p.inv_tau, -lse) : __fmul_rn(pr[k] - um, p.inv_tau);
+            const float lp = REST ? d : d - lt;
+            pk = REST ? expf(d) : __fmul_rn(expf(d), inv);
             psum += pk;
             if (!(pk == 0.f)) plogp = __fmaf_rn(pk, lp, plogp);
             if (REST && K >= p.V) {
@@ -182,14 +185,16 @@ __device__ __forceinline__ bool leads(const int* id, int k)
     return true;
 }
 
-// what the gradient of a row needs: outside the slots cr 2^(z c - b), for a slot's token scale (P 2^(z c - b) - sum p)
+// what the gradient of a row needs, S = sa 2^ma: outside the slots cr 2^(z c - b), for a slot's token Pq 2^(z c - b) - scale sum p
 struct GradScale {
-    float scale, P, cr, b;
-    __device__ GradScale(float scale_, float psum, float prest, float log2S, float log2qr) : scale(scale_), P(psum + prest)
+    float scale, Pq, cr, b;
+    __device__ GradScale(float scale_, float psum, float prest, float ma, float sa, float log2qr) : scale(scale_)
     {
+        const float P = psum + prest, inv = sa == 0.f ? 0.f : 1.f / sa;
+        Pq = scale * P * inv;
         // a rest that the student gives nothing has q_j = 0 throughout
-        cr = scale * (prest > 0.f ? (log2qr == -INFINITY ? 0.f : P - prest * ex2(-log2qr)) : P);
-        b = log2S == -INFINITY ? 0.f : log2S;
+        cr = scale * (prest > 0.f ? (log2qr == -INFINITY ? 0.f : P - prest * ex2(-log2qr)) : P) * inv;
+        b = ma == -INFINITY ? 0.f : ma;
     }
 };
 template <typename T>
@@ -235,8 +240,8 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
     __shared__ float xch[4][D_MAXCL];
     __shared__ int dup;
     uint32_t* bits = dsm;
-    float* pr = reinterpret_cast<float*>(dsm + p.bit_words + 4 * p.hold);  // u / tau, then p_k
-    float* zk = pr + p.K;  // z of the slot's token in units of log2 (slots of the slice; all of them on the first CTA)
+    float* pr = reinterpret_cast<float*>(dsm + p.bit_words + 4 * p.hold);  // u, then p_k
+    float* zk = pr + p.K;  // z of the slot's token (slots of the slice; all of them on the first CTA)
     int* id = reinterpret_cast<int*>(zk + p.K);  // token or -1
     const uint32_t held = (uint32_t)__cvta_generic_to_shared(dsm + p.bit_words);
 
@@ -253,7 +258,7 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
     if (w == 0.f) {  // no loss, no gradient; the logits may be anything
         if (rank == 0 && tid == 0) {
             p.loss[row] = 0.f;
-            if (p.stats) p.stats[2 * row] = 0.f, p.stats[2 * row + 1] = 0.f;
+            if (p.stats) p.stats[3 * row] = p.stats[3 * row + 1] = p.stats[3 * row + 2] = 0.f;
         }
         if (GRAD) zero_slice(p, sl, dz, rank, tid, ALL);
         if (cl > 1) cluster_wait();
@@ -281,7 +286,7 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
         if (k != tid) load_slot(p, row, k, id0, u0);
         const bool own = id0 >= 0 && id0 >= sl.j0 && id0 < sl.j1;
         id[k] = id0, pr[k] = u0;
-        if (own || (rank == 0 && id0 >= 0)) zk[k] = __fmul_rn(to_f(sl.z[id0]), c);
+        if (own || (rank == 0 && id0 >= 0)) zk[k] = to_f(sl.z[id0]);
         if (own) {
             const int b = id0 - jb;
             if (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31) & 1u) dup = 1;
@@ -353,7 +358,9 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
         s = e.x + e.y;
         auto scalar = [&](int j) {
             if (REST && (bits[(j - jb) >> 5] >> ((j - jb) & 31) & 1u)) return;
-            join(m, s, __fmul_rn(to_f(sl.z[j]), c), 1.f);
+            const float z = to_f(sl.z[j]), M = fmaxf(m, __fmul_rn(z, c)), b = M == -INFINITY ? 0.f : M;
+            s = __fmaf_rn(s, ex2(m - b), ex2(__fmaf_rn(z, c, -b)));
+            m = M;
         };
         if (rank == 0 && tid < sl.head) scalar(tid);
         if (rank == cl - 1 && sl.tail() + tid < V) scalar(sl.tail() + tid);
@@ -363,9 +370,13 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
         float psum, prest, plogp, mt = -INFINITY, st = 0.f;
         teacher_probabilities<REST>(p, REST ? p.lse[row] : 0.f, pr, id, lane, psum, prest, plogp);
         if (REST) {
+            auto counts = [&](int k) { return id[k] >= 0 && id[k] >= sl.j0 && id[k] < sl.j1 && (!any_dup || leads(id, k)); };
             for (int k = lane; k < K; k += 32)
-                if (id[k] >= 0 && id[k] >= sl.j0 && id[k] < sl.j1 && (!any_dup || leads(id, k))) join(mt, st, zk[k], 1.f);
-            warp_join<32>(mt, st);
+                if (counts(k)) mt = fmaxf(mt, __fmul_rn(zk[k], c));
+            mt = warp_reduce<0>(mt);
+            for (int k = lane; k < K; k += 32)
+                if (counts(k)) st += ex2(__fmaf_rn(zk[k], c, mt == -INFINITY ? 0.f : -mt));
+            st = warp_reduce<1>(st);
         }
         if (lane == 0) slot_sums[0] = psum, slot_sums[1] = prest, slot_sums[2] = plogp, slot_sums[3] = mt, slot_sums[4] = st;
     }
@@ -394,22 +405,22 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
     }
     float ma = m, sa = s;
     if (REST) join(ma, sa, mt, st);
-    const float log2S = ma + log2f(sa);
-    const float log2qr = !REST || s == 0.f ? -INFINITY : m + log2f(s) - log2S;
+    // S = sa 2^ma: the two stay apart, for log2 S itself would be rounded to the size of the logits
+    const float ls = log2f(sa), base = ma == -INFINITY ? 0.f : ma;
+    const float log2qr = !REST || s == 0.f ? -INFINITY : (m - base) + (log2f(s) - ls);
     if (rank == 0 && warp == WARPS) {
         float l = 0.f;
-        const float b = log2S == -INFINITY ? 0.f : log2S;
         for (int k = lane; k < K; k += 32)
-            if (!(pr[k] == 0.f)) l = __fmaf_rn(-pr[k], __fmul_rn(zk[k] - b, LN2), l);
+            if (!(pr[k] == 0.f)) l = __fmaf_rn(-pr[k], __fmul_rn(__fmaf_rn(zk[k], c, -base) - (ma == -INFINITY ? 0.f : ls), LN2), l);
         l = warp_reduce<1>(l) + slot_sums[2];
         if (lane == 0) {
             if (prest > 0.f) l = __fmaf_rn(prest, __fmaf_rn(-log2qr, LN2, logf(prest)), l);
             p.loss[row] = __fmul_rn(w, l);
-            if (p.stats) p.stats[2 * row] = log2S * LN2, p.stats[2 * row + 1] = log2qr * LN2;
+            if (p.stats) p.stats[3 * row] = ma, p.stats[3 * row + 1] = sa, p.stats[3 * row + 2] = log2qr;
         }
     }
     if (GRAD) {
-        const GradScale g(__fmul_rn(w, p.inv_tau), psum, prest, log2S, log2qr);
+        const GradScale g(__fmul_rn(w, p.inv_tau), psum, prest, ma, sa, log2qr);
         if (p.vec_out) {
             const uint64_t bb = pair(-g.b, -g.b), rr = pair(g.cr, g.cr);
             uint4* dt = reinterpret_cast<uint4*>(dz + sl.head) + sl.v0 + tid;
@@ -431,7 +442,7 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
             if (any_dup)
                 for (int q = k + 1; q < K; q++)
                     if (id[q] == id[k]) pk += pr[q];
-            dz[id[k]] = from_f<T>(g.scale * (g.P * ex2(zk[k] - g.b) - pk));
+            dz[id[k]] = from_f<T>(__fmaf_rn(g.Pq, ex2(__fmaf_rn(zk[k], c, -g.b)), -__fmul_rn(g.scale, pk)));
         }
     }
 }
@@ -457,7 +468,7 @@ __global__ void __launch_bounds__(D_THREADS) distill_grad_kernel(const DistillPa
     float* zk = reinterpret_cast<float*>(id + K);
     for (int k = tid; k < K; k += D_THREADS) {
         load_slot(p, row, k, id[k], pr[k]);
-        if (id[k] >= 0) zk[k] = __fmul_rn(to_f(sl.z[id[k]]), c);
+        if (id[k] >= 0) zk[k] = to_f(sl.z[id[k]]);
     }
     __syncthreads();
     if (tid < 32) {
@@ -467,7 +478,7 @@ __global__ void __launch_bounds__(D_THREADS) distill_grad_kernel(const DistillPa
     }
     __syncthreads();
     const float up = p.grad ? p.grad[row * p.s_grad] : 1.f;
-    const GradScale g(up * w * p.inv_tau, sums[0], sums[1], p.stats[2 * row] * LOG2E, p.stats[2 * row + 1] * LOG2E);
+    const GradScale g(up * w * p.inv_tau, sums[0], sums[1], p.stats[3 * row], p.stats[3 * row + 1], p.stats[3 * row + 2]);
     if (p.vec_out) {
         const uint64_t cc = pair(c, c), bb = pair(-g.b, -g.b), rr = pair(g.cr, g.cr);
         // plain loads: the rows may be overwritten (dz = z), each vector by the thread that has read it
@@ -493,7 +504,7 @@ __global__ void __launch_bounds__(D_THREADS) distill_grad_kernel(const DistillPa
         float pk = pr[k];
         for (int q = k + 1; q < K; q++)
             if (id[q] == id[k]) pk += pr[q];
-        dz[id[k]] = from_f<T>(g.scale * (g.P * ex2(zk[k] - g.b) - pk));
+        dz[id[k]] = from_f<T>(__fmaf_rn(g.Pq, ex2(__fmaf_rn(zk[k], c, -g.b)), -__fmul_rn(g.scale, pk)));
     }
 }
 

@@ -85,10 +85,10 @@ def _call(logits, idx, teacher, teacher_lse, weight, temperature, mode, stats=No
     ld_d = s_grad = 0
     if mode != GRAD:
         loss = torch.empty(T, dtype=torch.float32, device=dev)
-        stats = torch.empty((T, 2), dtype=torch.float32, device=dev) if want_stats else None
+        stats = torch.empty((T, 3), dtype=torch.float32, device=dev) if want_stats else None
     else:
-        if stats.dtype != torch.float32 or stats.shape != (T, 2) or not stats.is_contiguous():
-            raise ValueError(f"distill: stats must be the [{T}, 2] that topk_loss returned")
+        if stats.dtype != torch.float32 or stats.shape != (T, 3) or not stats.is_contiguous():
+            raise ValueError(f"distill: stats must be the [{T}, 3] that topk_loss returned")
         if grad is not None:
             if grad.dtype != torch.float32 or grad.shape != (T,):
                 raise ValueError(f"distill: grad must be fp32 of shape [{T}]")
@@ -125,8 +125,8 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 def topk_loss(logits: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor, *,
               teacher_lse: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
               temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(loss [T], stats [T, 2]) of logits [T, V] against teacher [T, K] at the tokens idx [T, K]; stats are the student's
-    log-sum-exp at the temperature and the logarithm of its mass outside the slots, which topk_grad takes."""
+    """(loss [T], stats [T, 3]) of logits [T, V] against teacher [T, K] at the tokens idx [T, K].  stats = (m, s, r), which
+    topk_grad takes: the student's sum of exponentials is s 2^m, its mass outside the slots 2^r."""
     loss, stats, _ = _call(logits, idx, teacher, teacher_lse, weight, temperature, LOSS, want_stats=True)
     return loss, stats
 
