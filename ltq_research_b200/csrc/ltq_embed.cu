@@ -5,8 +5,9 @@
 //
 // A token outside [0, V) reads as a row of zeros and takes no gradient; neither does the padding token.
 //
-// The gradient runs in three launches.  (1) One cluster of 8 CTAs sorts the positions by token (stable, least digit
-// first, 10 bits a pass); the other CTAs meanwhile write zeros to the table rows that no token names.  (2) The sorted
+// The gradient runs in three launches.  (1) The positions are sorted by token (stable) and zeros written to the table rows
+// that no token names.  Up to 8192 positions every CTA counts the ranks of a few positions and then writes its zeros; beyond,
+// one cluster of 8 CTAs sorts (least digit first, 10 bits a pass) while the other CTAs write the zeros.  (2) The sorted
 // list is cut into chunks of equal length; a warp sums one chunk's rows over 32 vectors of the width and writes the rows
 // whose positions all lie in the chunk, and the sums of the rows that reach over its ends to a workspace.  (3) Those
 // sums are joined from the row's first chunk to its last.  Nothing depends on the order in which CTAs run.
@@ -66,11 +67,13 @@ int lookup_launch(const void* E, long long ld, const void* tok, int t64, long lo
 
 // -------------------------------------------------------------------------------------------------------- gradient
 
-constexpr int S_THREADS = 1024, S_WARPS = 32, S_CL = 8;
+constexpr int S_THREADS = 512, S_WARPS = 16, S_CL = 8;  // two CTAs an SM, so that the fill uses all of them
 constexpr int DIGIT = 10, BINS = 1 << DIGIT;
-constexpr int FILL_ROWS = 1 << 17;  // rows of a fill CTA's bitmap at a time
-constexpr int SORT_SMEM = (S_WARPS * BINS + S_CL * BINS + 64) * 4;
-static_assert(BINS == S_THREADS, "one thread per bin");
+constexpr int FILL_ROWS = 1 << 15;  // rows of a fill CTA's bitmap at a time
+constexpr int RANK_BITS = FILL_ROWS / 32;
+constexpr int SORT_SMEM = (S_WARPS * BINS + S_CL * BINS + BINS + 64) * 4;
+constexpr int KEPT = 4;  // groups of 32 positions that a warp keeps in registers between counting and scattering
+static_assert(BINS == 2 * S_THREADS, "two bins a thread");
 static_assert(FILL_ROWS / 32 <= S_WARPS * BINS, "the fill's bitmap fits the histograms' memory");
 
 struct SortParams {
@@ -99,69 +102,98 @@ __device__ void sort_cluster(const SortParams& p, uint32_t* sm)
 {
     uint32_t* hist = sm;                        // [warp][bin]
     uint32_t* all = sm + S_WARPS * BINS;        // [CTA of the cluster][bin]
-    uint32_t* wsum = all + S_CL * BINS;         // 32 warp sums
+    uint32_t* base = all + S_CL * BINS;         // first place of this CTA's keys of a bin
+    uint32_t* wsum = base + BINS;               // warp sums
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = (int)cluster_rank();
     const int gw = rank * S_WARPS + warp;
     const int per = (p.n + S_CL * S_WARPS * 32 - 1) / (S_CL * S_WARPS * 32) * 32;  // positions of a warp
     const long long a = (long long)gw * per;
     const int i0 = (int)(a < p.n ? a : p.n), i1 = (int)(a + per < p.n ? a + per : p.n);
+    const bool kept = per <= 32 * KEPT;
     uint32_t* mine = hist + warp * BINS;
     for (int pass = 0; pass < p.passes; pass++) {
         const int shift = pass * DIGIT;
         const uint32_t* ik = p.key[(pass & 1) ^ 1];
         const uint32_t* ip = p.pos[(pass & 1) ^ 1];
         uint32_t *ok = p.key[pass & 1], *op = p.pos[pass & 1];
-        for (int w = 0; w < S_WARPS; w++) hist[w * BINS + tid] = 0;
-        __syncthreads();
-        for (int i = i0 + lane; i < i1; i += 32) {
-            const uint32_t k = pass == 0 ? sort_key(p, i) : ik[i];
-            atomicAdd(&mine[(k >> shift) & (BINS - 1)], 1u);
+        uint32_t kr[KEPT], pr[KEPT];
+        if (kept) {
+#pragma unroll
+            for (int q = 0; q < KEPT; q++) {
+                const int i = i0 + 32 * q + lane;
+                kr[q] = i < i1 ? (pass == 0 ? sort_key(p, i) : ik[i]) : 0;
+                pr[q] = i < i1 ? (pass == 0 ? (uint32_t)i : ip[i]) : 0;
+            }
         }
+        for (int i = tid; i < S_WARPS * BINS / 4; i += S_THREADS) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        uint32_t run = 0;  // thread = bin: the warps' counts become offsets within the CTA
+        if (kept) {
+#pragma unroll
+            for (int q = 0; q < KEPT; q++)
+                if (i0 + 32 * q + lane < i1) atomicAdd(&mine[(kr[q] >> shift) & (BINS - 1)], 1u);
+        } else
+            for (int i = i0 + lane; i < i1; i += 32) {
+                const uint32_t k = pass == 0 ? sort_key(p, i) : ik[i];
+                atomicAdd(&mine[(k >> shift) & (BINS - 1)], 1u);
+            }
+        __syncthreads();
+        // a thread's two bins (adjacent): the warps' counts become offsets within the CTA
+        uint2 run = make_uint2(0, 0), c[S_WARPS];
+#pragma unroll
+        for (int w = 0; w < S_WARPS; w++) c[w] = reinterpret_cast<const uint2*>(hist + w * BINS)[tid];
+#pragma unroll
         for (int w = 0; w < S_WARPS; w++) {
-            const uint32_t c = hist[w * BINS + tid];
-            hist[w * BINS + tid] = run;
-            run += c;
+            reinterpret_cast<uint2*>(hist + w * BINS)[tid] = run;
+            run.x += c[w].x, run.y += c[w].y;
         }
-        for (int q = 0; q < S_CL; q++) st_cluster_u32(&all[rank * BINS + tid], q, run);
+        for (int q = 0; q < S_CL; q++) {
+            st_cluster_u32(&all[rank * BINS + 2 * tid], q, run.x);
+            st_cluster_u32(&all[rank * BINS + 2 * tid + 1], q, run.y);
+        }
         cluster_arrive();
         cluster_wait();
-        uint32_t tot = 0, before = 0;
+        uint2 tot = make_uint2(0, 0), before = make_uint2(0, 0);
+#pragma unroll
         for (int q = 0; q < S_CL; q++) {
-            const uint32_t c = all[q * BINS + tid];
-            before += q < rank ? c : 0;
-            tot += c;
+            const uint2 v = reinterpret_cast<const uint2*>(all + q * BINS)[tid];
+            if (q < rank) before.x += v.x, before.y += v.y;
+            tot.x += v.x, tot.y += v.y;
         }
-        uint32_t inc = tot;  // exclusive scan of the totals over the bins
+        uint32_t inc = tot.x + tot.y;  // exclusive scan of the totals over the bins
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t x = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += x;
         }
         if (lane == 31) wsum[warp] = inc;
         __syncthreads();
-        uint32_t base = 0;
-        for (int w = 0; w < warp; w++) base += wsum[w];
-        base += inc - tot + before;
-        for (int w = 0; w < S_WARPS; w++) hist[w * BINS + tid] += base;
+        uint32_t first = inc - tot.x - tot.y;
+        for (int w = 0; w < warp; w++) first += wsum[w];
+        base[2 * tid] = first + before.x;
+        base[2 * tid + 1] = first + tot.x + before.y;
         __syncthreads();
-        for (int g = i0; g < i1; g += 32) {  // in the order of the list: stable
-            const int i = g + lane;
-            const bool on = i < i1;
-            const uint32_t k = on ? (pass == 0 ? sort_key(p, i) : ik[i]) : 0;
-            const uint32_t ps = on ? (pass == 0 ? (uint32_t)i : ip[i]) : 0;
+        auto scatter = [&](bool on, uint32_t k, uint32_t ps) {  // 32 positions in the order of the list: stable
             const uint32_t d = on ? (k >> shift) & (BINS - 1) : BINS;
             const uint32_t peers = __match_any_sync(0xffffffffu, d);
             const int leader = __ffs(peers) - 1;
             uint32_t at = 0;
             if (on && lane == leader) {
-                at = mine[d];
-                mine[d] = at + __popc(peers);
+                const uint32_t o = mine[d];
+                at = o + base[d];
+                mine[d] = o + __popc(peers);
             }
             at = __shfl_sync(0xffffffffu, at, leader) + __popc(peers & ((1u << lane) - 1));
             if (on) ok[at] = k, op[at] = ps;
             __syncwarp();
-        }
+        };
+        if (kept) {
+#pragma unroll
+            for (int q = 0; q < KEPT; q++) scatter(i0 + 32 * q + lane < i1, kr[q], pr[q]);
+        } else
+            for (int g = i0; g < i1; g += 32) {
+                const int i = g + lane;
+                const bool on = i < i1;
+                scatter(on, on ? (pass == 0 ? sort_key(p, i) : ik[i]) : 0, on ? (pass == 0 ? (uint32_t)i : ip[i]) : 0);
+            }
         cluster_arrive();  // the pass's list is written, and `all` is free again
         cluster_wait();
     }
@@ -171,13 +203,14 @@ template <int B>  // bytes of a store
 __device__ void zero_row(uint8_t* row, long long bytes, int lane)
 {
     for (long long o = lane * B; o < bytes; o += 32 * B) {
-        if (B == 16) *reinterpret_cast<uint4*>(row + o) = make_uint4(0, 0, 0, 0);
+        if (B == 16) __stcs(reinterpret_cast<uint4*>(row + o), make_uint4(0, 0, 0, 0));
         else if (B == 4) *reinterpret_cast<uint32_t*>(row + o) = 0;
         else *reinterpret_cast<uint16_t*>(row + o) = 0;
     }
 }
 
-__device__ void fill_rows(const SortParams& p, uint32_t* bits, int f)
+// zeros to this CTA's share of the rows that no token names; keys: all sort keys in shared memory, or NULL to read the tokens
+__device__ void fill_rows(const SortParams& p, uint32_t* bits, int f, const uint32_t* keys)
 {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const long long per = (p.V + p.fill_ctas - 1) / p.fill_ctas;
@@ -190,8 +223,8 @@ __device__ void fill_rows(const SortParams& p, uint32_t* bits, int f)
         for (int i = tid; i < (nr + 31) / 32; i += S_THREADS) bits[i] = 0;
         __syncthreads();
         for (int i = tid; i < p.n; i += S_THREADS) {
-            const long long t = load_token(p.tok, p.t64, i);
-            if (t >= r0 && t < r0 + nr && t != p.pad) atomicOr(&bits[(t - r0) >> 5], 1u << ((t - r0) & 31));
+            const long long t = keys ? (long long)keys[i] : (long long)sort_key(p, i);
+            if (t >= r0 && t < r0 + nr) atomicOr(&bits[(t - r0) >> 5], 1u << ((t - r0) & 31));
         }
         __syncthreads();
         for (int r = warp; r < nr; r += S_WARPS) {
@@ -205,12 +238,41 @@ __device__ void fill_rows(const SortParams& p, uint32_t* bits, int f)
     }
 }
 
-__global__ void __cluster_dims__(S_CL, 1, 1) __launch_bounds__(S_THREADS, 1) sort_fill_kernel(const SortParams p)
+// Few positions: a position's place in the sorted list is the number of smaller keys and of equal keys before it, counted by a
+// warp over all keys in shared memory.  At 4099 positions and 50003 rows this takes 2 us of a launch where the digit passes'
+// barriers would take 17.
+constexpr int RANK_MAX = 8192;
+__global__ void __launch_bounds__(S_THREADS, 2) rank_fill_kernel(const SortParams p)
+{
+    __shared__ __align__(16) uint32_t key[RANK_MAX];
+    __shared__ uint32_t bits[RANK_BITS];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n4 = (p.n + 3) / 4;
+    for (int i = tid; i < 4 * n4; i += S_THREADS) key[i] = i < p.n ? sort_key(p, i) : 0xffffffffu;
+    __syncthreads();
+    for (int i = blockIdx.x * S_WARPS + warp; i < p.n; i += gridDim.x * S_WARPS) {
+        const uint32_t k = key[i];
+        int below = 0;
+        for (int j = lane; j < n4; j += 32) {
+            const uint4 q = reinterpret_cast<const uint4*>(key)[j];
+            const int e = 4 * j;
+            below += (q.x < k || (q.x == k && e < i)) + (q.y < k || (q.y == k && e + 1 < i)) + (q.z < k || (q.z == k && e + 2 < i)) +
+                     (q.w < k || (q.w == k && e + 3 < i));
+        }
+        below = __reduce_add_sync(0xffffffffu, below);
+        if (lane == 0) p.key[0][below] = k, p.pos[0][below] = i;
+    }
+    if (p.fill_ctas) {
+        __syncthreads();
+        fill_rows(p, bits, blockIdx.x, key);
+    }
+}
+
+__global__ void __cluster_dims__(S_CL, 1, 1) __launch_bounds__(S_THREADS, 2) sort_fill_kernel(const SortParams p)
 {
     extern __shared__ uint32_t sm[];
     const int cluster = blockIdx.x / S_CL;
     if (cluster == 0) sort_cluster(p, sm);
-    else fill_rows(p, sm, blockIdx.x - S_CL);
+    else fill_rows(p, sm, blockIdx.x - S_CL, nullptr);
 }
 
 struct SumParams {
@@ -226,18 +288,21 @@ struct SumParams {
 };
 
 template <typename TO, int VEC>
-__device__ __forceinline__ void write_row(const SumParams& p, uint32_t row, int v, const float (&a)[VEC])
+__device__ __forceinline__ Vec<TO, VEC>* out_vec(const SumParams& p, uint32_t row, int v)
 {
-    TO* o = (TO*)p.out + (long long)row * p.ld_out + (long long)v * VEC;
-    Vec<TO, VEC> x;
-    if (p.accumulate) {
-        x = *reinterpret_cast<const Vec<TO, VEC>*>(o);
+    return reinterpret_cast<Vec<TO, VEC>*>((TO*)p.out + (long long)row * p.ld_out + (long long)v * VEC);
+}
+// x: with ACC, what the row holds
+template <typename TO, int VEC, bool ACC>
+__device__ __forceinline__ void write_row(const SumParams& p, uint32_t row, int v, const float (&a)[VEC], Vec<TO, VEC> x)
+{
+    if (ACC) {
 #pragma unroll
         for (int q = 0; q < VEC; q++) x.v[q] = from_f<TO>(fmaf(p.scale, a[q], to_f(x.v[q])));
     } else
 #pragma unroll
         for (int q = 0; q < VEC; q++) x.v[q] = from_f<TO>(p.scale * a[q]);
-    *reinterpret_cast<Vec<TO, VEC>*>(o) = x;
+    *out_vec<TO, VEC>(p, row, v) = x;
 }
 
 template <int VEC>
@@ -249,81 +314,181 @@ __device__ __forceinline__ void store_part(float* part, const float (&a)[VEC])
     *reinterpret_cast<Vec<float, VEC>*>(part) = x;
 }
 
-template <typename TI, typename TO, int VEC>
+// a warp per chunk and 32 vectors of the width; four rows' loads in flight
+template <typename TI, typename TO, int VEC, bool ACC>
 __global__ void __launch_bounds__(128) sum_chunks_kernel(const SumParams p)
 {
     const int lane = threadIdx.x, ch = blockIdx.x * 4 + threadIdx.y, v = blockIdx.y * 32 + lane, nv = p.D / VEC;
     if (ch >= p.nchunks) return;
     const int c0 = ch * p.chunk, c1 = min(p.n, c0 + p.chunk);
-    uint32_t cur = p.key[c0];
+    // keys and positions of up to 32 places, a lane each, and the keys beside the chunk: one round of loads
+    uint32_t kk = c0 + lane < c1 ? p.key[c0 + lane] : (uint32_t)p.V, pp = c0 + lane < c1 ? p.pos[c0 + lane] : 0;
+    const uint32_t before = c0 > 0 ? p.key[c0 - 1] : (uint32_t)p.V, after = c1 < p.n ? p.key[c1] : (uint32_t)p.V;
+    uint32_t cur = __shfl_sync(0xffffffffu, kk, 0);
     if (cur >= (uint32_t)p.V) return;  // from here on nothing takes a gradient
     const bool on = v < nv;
-    const bool open = c0 > 0 && p.key[c0 - 1] == cur;  // the first row was begun in an earlier chunk
+    const bool open = before == cur;  // the first row was begun in an earlier chunk
     bool first = true;
     float a[VEC];
 #pragma unroll
     for (int q = 0; q < VEC; q++) a[q] = 0.f;
     float* part = p.part + (long long)ch * 2 * p.D + (long long)v * VEC;
-    for (int i = c0; i < c1; i++) {
-        const uint32_t k = p.key[i];
-        if (k != cur) {
-            if (on) {
-                if (first && open) store_part<VEC>(part, a);
-                else write_row<TO, VEC>(p, cur, v, a);
+    const TI* d = (const TI*)p.d + (long long)v * VEC;
+    for (int g = c0; g < c1; g += 32) {
+        if (g > c0) kk = g + lane < c1 ? p.key[g + lane] : (uint32_t)p.V, pp = g + lane < c1 ? p.pos[g + lane] : 0;
+        const int m = min(32, c1 - g);
+        for (int i = 0; i < m; i += 4) {
+            Vec<TI, VEC> x[4];
+            Vec<TO, VEC> old[4];  // ACC: the row that ends at this place, if one does
+            uint32_t k[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                k[q] = __shfl_sync(0xffffffffu, kk, i + q);
+                const uint32_t row = __shfl_sync(0xffffffffu, pp, i + q);
+                if (on && k[q] < (uint32_t)p.V) x[q] = *reinterpret_cast<const Vec<TI, VEC>*>(d + (long long)row * p.ld_d);
             }
-            first = false;
-            cur = k;
+            if (ACC) {
+                uint32_t k0 = cur;  // the row before each place: written when the place's key differs
 #pragma unroll
-            for (int q = 0; q < VEC; q++) a[q] = 0.f;
-            if (cur >= (uint32_t)p.V) return;
-        }
-        if (on) {
-            const Vec<TI, VEC> x =
-                *reinterpret_cast<const Vec<TI, VEC>*>((const TI*)p.d + (long long)p.pos[i] * p.ld_d + (long long)v * VEC);
+                for (int q = 0; q < 4; q++) {
+                    if (on && k[q] != k0) old[q] = *out_vec<TO, VEC>(p, k0, v);
+                    k0 = k[q];
+                    if (k0 >= (uint32_t)p.V) break;
+                }
+            }
 #pragma unroll
-            for (int q = 0; q < VEC; q++) a[q] += to_f(x.v[q]);
+            for (int q = 0; q < 4; q++) {
+                if (i + q >= m) break;
+                if (k[q] != cur) {
+                    if (on) {
+                        if (first && open) store_part<VEC>(part, a);
+                        else write_row<TO, VEC, ACC>(p, cur, v, a, old[q]);
+                    }
+                    first = false;
+                    cur = k[q];
+                    if (cur >= (uint32_t)p.V) return;
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) a[e] = 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < VEC; e++) a[e] += to_f(x[q].v[e]);
+            }
         }
     }
     if (!on) return;
     if (first && open) store_part<VEC>(part, a);  // the chunk is the middle or the end of a row begun earlier
-    else if (c1 < p.n && p.key[c1] == cur) store_part<VEC>(part + p.D, a);
-    else write_row<TO, VEC>(p, cur, v, a);
+    else if (after == cur) store_part<VEC>(part + p.D, a);
+    else {
+        Vec<TO, VEC> x;
+        if (ACC) x = *out_vec<TO, VEC>(p, cur, v);
+        write_row<TO, VEC, ACC>(p, cur, v, a, x);
+    }
 }
 
-template <typename TO, int VEC>
-__global__ void __launch_bounds__(128) join_chunks_kernel(const SumParams p)
+// sum of chunks q0 .. q1 - 1 of a row whose first chunk is `part`'s: that chunk's sum lies in its second place, the others' in their first
+template <int VEC>
+__device__ __forceinline__ void add_parts(float (&a)[VEC], const float* part, int q0, int q1, int D)
 {
-    const int ch = blockIdx.x * 4 + threadIdx.y, v = blockIdx.y * 32 + threadIdx.x;
-    if (ch >= p.nchunks - 1 || v >= p.D / VEC) return;
-    const int c0 = ch * p.chunk, c1 = c0 + p.chunk;
-    const uint32_t k = p.key[c1 - 1];
-    if (k >= (uint32_t)p.V || p.key[c1] != k) return;               // no row goes on into the next chunk
-    if (c0 > 0 && p.key[c0] == k && p.key[c0 - 1] == k) return;     // it was begun earlier: joined from there
-    float a[VEC];
-    const float* part = p.part + (long long)ch * 2 * p.D + (long long)v * VEC;
+#pragma unroll 4
+    for (int q = q0; q < q1; q++) {
+        const Vec<float, VEC> x = *reinterpret_cast<const Vec<float, VEC>*>(part + (long long)q * 2 * D + (q == 0 ? D : 0));
 #pragma unroll
-    for (int q = 0; q < VEC; q++) a[q] = part[p.D + q];
-    for (int c = ch + 1; c < p.nchunks && p.key[c * p.chunk] == k; c++) {
-        part += 2 * p.D;
-#pragma unroll
-        for (int q = 0; q < VEC; q++) a[q] += part[q];
+        for (int i = 0; i < VEC; i++) a[i] += x.v[i];
     }
-    write_row<TO, VEC>(p, k, v, a);
+}
+
+// Rows that go on over chunks.  A CTA looks at 32 chunks; a warp joins a row of up to SHORT chunks, the whole CTA (eight stretches,
+// added in order) a longer one.
+template <typename TO, int VEC, bool ACC>
+__global__ void __launch_bounds__(256) join_chunks_kernel(const SumParams p)
+{
+    constexpr int SHORT = 8;
+    __shared__ float stretch[8][32][VEC + 1];
+    __shared__ int ends[32];  // the last chunk of a long row that begins in chunk i, or -1
+    const int lane = threadIdx.x, warp = threadIdx.y, v = blockIdx.y * 32 + lane, nv = p.D / VEC, base = blockIdx.x * 32;
+    // those whose last row goes on into the next chunk and was not begun in an earlier one
+    const int mine = base + lane, c0 = mine * p.chunk, c1 = c0 + p.chunk;
+    uint32_t k1 = (uint32_t)p.V;
+    bool b = mine < p.nchunks - 1;
+    if (b) {
+        const uint32_t at = p.key[c0], before = c0 > 0 ? p.key[c0 - 1] : (uint32_t)p.V, after = p.key[c1];
+        k1 = p.key[c1 - 1];
+        b = k1 < (uint32_t)p.V && after == k1 && !(at == k1 && before == k1);
+    }
+    const uint32_t begins = __ballot_sync(0xffffffffu, b);
+    if (warp == 0) ends[lane] = -1;
+    __syncthreads();
+    int nth = 0;
+    for (uint32_t rest = begins; rest; rest &= rest - 1, nth++) {
+        if ((nth & 7) != warp) continue;
+        const int i = __ffs(rest) - 1, ch = base + i;
+        const uint32_t k = __shfl_sync(0xffffffffu, k1, i);
+        int last = ch + 1;  // the last chunk that begins with it
+        while (true) {
+            const bool same = last + lane < p.nchunks && p.key[(long long)(last + lane) * p.chunk] == k;
+            const uint32_t no = ~__ballot_sync(0xffffffffu, same);
+            if (no) {
+                last += __ffs(no) - 2;
+                break;
+            }
+            last += 32;
+        }
+        if (last - ch >= SHORT) {
+            if (lane == 0) ends[i] = last;
+        } else if (v < nv) {
+            float a[VEC];
+#pragma unroll
+            for (int q = 0; q < VEC; q++) a[q] = 0.f;
+            add_parts<VEC>(a, p.part + (long long)ch * 2 * p.D + (long long)v * VEC, 0, last - ch + 1, p.D);
+            Vec<TO, VEC> x;
+            if (ACC) x = *out_vec<TO, VEC>(p, k, v);
+            write_row<TO, VEC, ACC>(p, k, v, a, x);
+        }
+    }
+    __syncthreads();
+    for (uint32_t rest = begins; rest; rest &= rest - 1) {
+        const int i = __ffs(rest) - 1, ch = base + i, last = ends[i];
+        if (last < 0) continue;  // uniform
+        const int count = last - ch + 1, each = (count + 7) / 8, q0 = min(count, warp * each);
+        float a[VEC];
+#pragma unroll
+        for (int q = 0; q < VEC; q++) a[q] = 0.f;
+        if (v < nv) add_parts<VEC>(a, p.part + (long long)ch * 2 * p.D + (long long)v * VEC, q0, min(count, q0 + each), p.D);
+#pragma unroll
+        for (int q = 0; q < VEC; q++) stretch[warp][lane][q] = a[q];
+        __syncthreads();
+        if (warp == 0 && v < nv) {
+#pragma unroll
+            for (int w = 1; w < 8; w++)
+#pragma unroll
+                for (int q = 0; q < VEC; q++) a[q] += stretch[w][lane][q];
+            const uint32_t k = p.key[(long long)(ch + 1) * p.chunk];
+            Vec<TO, VEC> x;
+            if (ACC) x = *out_vec<TO, VEC>(p, k, v);
+            write_row<TO, VEC, ACC>(p, k, v, a, x);
+        }
+        __syncthreads();
+    }
 }
 
 constexpr long long N_MAX = 1LL << 30;  // positions of a gradient call
 constexpr int D_MAX = 1 << 20;
 
-// positions of a chunk: about a thousand chunks, 8 positions at least
-int chunk_of(long long n) { return (int)(n <= 8192 ? 8 : (n + 1023) / 1024); }
+// Positions of a chunk, a multiple of 4: 8 at least, and so many that about 8192 warps (a chunk times 32 vectors of the width,
+// eight elements each) share the sums, 1024 chunks at least.
+int chunk_of(long long n, int D)
+{
+    const int slices = (D + 255) / 256, target = slices >= 8 ? 1024 : 8192 / slices;
+    return n <= 8LL * target ? 8 : (int)(((n + target - 1) / target + 3) / 4 * 4);
+}
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 
-template <typename TI, typename TO, int VEC>
+template <typename TI, typename TO, int VEC, bool ACC>
 int sum_launch(const SumParams& p, cudaStream_t st)
 {
-    const dim3 grid((p.nchunks + 3) / 4, (p.D / VEC + 31) / 32), block(32, 4);
-    sum_chunks_kernel<TI, TO, VEC><<<grid, block, 0, st>>>(p);
-    if (p.nchunks > 1) join_chunks_kernel<TO, VEC><<<grid, block, 0, st>>>(p);
+    const unsigned slices = (p.D / VEC + 31) / 32;
+    sum_chunks_kernel<TI, TO, VEC, ACC><<<dim3((p.nchunks + 3) / 4, slices), dim3(32, 4), 0, st>>>(p);
+    if (p.nchunks > 1) join_chunks_kernel<TO, VEC, ACC><<<dim3((p.nchunks + 30) / 32, slices), dim3(32, 8), 0, st>>>(p);
     return (int)cudaGetLastError();
 }
 template <typename TI, typename TO>
@@ -331,8 +496,8 @@ int sum_dispatch(const SumParams& p, cudaStream_t st)
 {
     constexpr int W = 16 / sizeof(TI);
     if (p.D % W == 0 && p.ld_d % W == 0 && p.ld_out % W == 0 && (uintptr_t)p.d % 16 == 0 && (uintptr_t)p.out % 16 == 0)
-        return sum_launch<TI, TO, W>(p, st);
-    return sum_launch<TI, TO, 1>(p, st);
+        return p.accumulate ? sum_launch<TI, TO, W, true>(p, st) : sum_launch<TI, TO, W, false>(p, st);
+    return p.accumulate ? sum_launch<TI, TO, 1, true>(p, st) : sum_launch<TI, TO, 1, false>(p, st);
 }
 template <typename TI>
 int sum_type(const SumParams& p, int odt, cudaStream_t st)
@@ -373,7 +538,7 @@ extern "C" int ltq_embed_lookup(const void* table, int dtype, long long ld, cons
 extern "C" size_t ltq_embed_grad_workspace_bytes(long long n, int D)
 {
     if (n <= 0 || n > N_MAX || D < 1 || D > D_MAX) return 0;
-    const int c = chunk_of(n);
+    const int c = chunk_of(n, D);
     return 4 * align256(4 * (size_t)n) + align256(8 * (size_t)((n + c - 1) / c) * D);
 }
 
@@ -397,28 +562,39 @@ extern "C" int ltq_embed_grad(const void* tokens, int tok64, long long n, int V,
     const size_t a = align256(4 * (size_t)n);
     for (int i = 0; i < 2; i++) s.key[i] = (uint32_t*)(ws + 2 * i * a), s.pos[i] = (uint32_t*)(ws + (2 * i + 1) * a);
     s.out = (uint8_t*)out, s.ld_bytes = ld_out * eo, s.row_bytes = (long long)D * eo;
-    static std::atomic<int> clusters[64];  // clusters of the sort kernel that a device holds at once
+    static std::atomic<int> clusters[64], sms[64];  // clusters of the sort kernel that a device holds at once
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
     int nc = clusters[dev].load(std::memory_order_acquire);
+    cudaError_t e;
     if (nc == 0) {
-        cudaError_t e = cudaFuncSetAttribute(sort_fill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_SMEM);
+        e = cudaFuncSetAttribute(sort_fill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_SMEM);
         if (e != cudaSuccess) return (int)e;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(S_CL), cfg.blockDim = dim3(S_THREADS), cfg.dynamicSmemBytes = SORT_SMEM;
         if ((e = cudaOccupancyMaxActiveClusters(&nc, sort_fill_kernel, &cfg)) != cudaSuccess) return (int)e;
+        int m = 0;
+        if ((e = cudaDeviceGetAttribute(&m, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return (int)e;
+        sms[dev].store(m, std::memory_order_relaxed);
         if (nc < 2) nc = 2;
         clusters[dev].store(nc, std::memory_order_release);
     }
-    s.fill_ctas = accumulate ? 0 : (nc - 1) * S_CL;
-    sort_fill_kernel<<<S_CL + s.fill_ctas, S_THREADS, SORT_SMEM, st>>>(s);
-    cudaError_t e = cudaGetLastError();
+    if (n <= RANK_MAX) {
+        s.passes = 1;
+        const int all = 2 * sms[dev].load(std::memory_order_relaxed), need = (int)((n + S_WARPS - 1) / S_WARPS);
+        s.fill_ctas = accumulate ? 0 : all;
+        rank_fill_kernel<<<accumulate && need < all ? need : all, S_THREADS, 0, st>>>(s);
+    } else {
+        s.fill_ctas = accumulate ? 0 : (nc - 1) * S_CL;
+        sort_fill_kernel<<<S_CL + s.fill_ctas, S_THREADS, SORT_SMEM, st>>>(s);
+    }
+    e = cudaGetLastError();
     if (e != cudaSuccess || n == 0) return (int)e;
     SumParams p{};
     const int b = sorted_buffer(s.passes);
     p.key = s.key[b], p.pos = s.pos[b], p.d = dout, p.ld_d = ld_d, p.out = out, p.ld_out = ld_out;
     p.part = (float*)(ws + 4 * a);
-    p.n = (int)n, p.V = V, p.D = D, p.chunk = chunk_of(n), p.accumulate = accumulate != 0, p.scale = scale;
+    p.n = (int)n, p.V = V, p.D = D, p.chunk = chunk_of(n, D), p.accumulate = accumulate != 0, p.scale = scale;
     p.nchunks = (int)((n + p.chunk - 1) / p.chunk);
     if (dtype == DT_F32) return sum_type<float>(p, out_dtype, st);
     if (dtype == DT_BF16) return sum_type<__nv_bfloat16>(p, out_dtype, st);
