@@ -339,6 +339,9 @@ int ltq_fp8_quant_rows(const void* x, int dtype, long long ld, int M, int K, uin
                        long long ld_s, void* stream);
 int ltq_fp8_quant_blocks(const void* w, int dtype, long long ld, int N, int K, uint8_t* q, long long ld_q, float* s,
                          long long ld_s, void* stream);
+/* out [C, ld_out] = the transpose of the 8-bit q [R, C] (rows 4-byte aligned), zeros behind column R (R <= ld_out, at most the next
+ * multiple of 64): a weight's other layout, for the gradient by the input. */
+int ltq_fp8_transpose(const uint8_t* q, long long ld, int R, int C, uint8_t* out, long long ld_out, void* stream);
 size_t ltq_fp8_gemm_workspace_bytes(int M, int N, int K);
 int ltq_fp8_gemm(const uint8_t* A, long long lda, const float* sa, long long ld_sa, const uint8_t* B, long long ldb,
                  const float* sb, long long ld_sb, void* C, int dtype, long long ldc, int M, int N, int K,

@@ -67,6 +67,7 @@ SIGNATURES = {
     "ltq_embed_grad": (I, [P, I, LL, I, LL, P, I, LL, I, ctypes.c_float, P, I, LL, I, P, SZ, P]),
     "ltq_fp8_quant_rows": (I, [P, I, LL, I, I, P, LL, P, LL, P]),
     "ltq_fp8_quant_blocks": (I, [P, I, LL, I, I, P, LL, P, LL, P]),
+    "ltq_fp8_transpose": (I, [P, LL, I, I, P, LL, P]),
     "ltq_fp8_gemm_workspace_bytes": (SZ, [I, I, I]),
     "ltq_fp8_few_supported": (I, [I, I, I]),
     "ltq_fp8_few": (I, [P, I, LL, P, LL, P, LL, P, I, LL, I, I, I, P, P]),
@@ -94,6 +95,7 @@ KERNELS_PER_CALL = {
     "ltq_distill_topk": lambda a: int(a[13] > 0), "ltq_embed_lookup": lambda a: int(a[5] > 0),
     "ltq_embed_grad": lambda a: 3 if a[2] > 8 else (2 if a[2] > 0 else int(not a[13])),
     "ltq_fp8_quant_rows": lambda a: int(a[3] > 0), "ltq_fp8_quant_blocks": lambda a: int(a[3] > 0),
+    "ltq_fp8_transpose": 1,
     "ltq_fp8_few": lambda a: int(a[10] > 0 and a[11] > 0),
     "ltq_fp8_gemm": lambda a: int(a[11] > 0 and a[12] > 0) + int(a[15] > 0),  # with a workspace also the parts' join
 }

@@ -104,6 +104,33 @@ __global__ void __launch_bounds__(256) quant_blocks_kernel(const T* __restrict__
     if (threadIdx.x == 0) s[blockIdx.y * ld_s + blockIdx.x] = sc;
 }
 
+// 8-bit transpose, 64 x 64 bytes through shared memory
+__global__ void __launch_bounds__(256) transpose8_kernel(const uint8_t* __restrict__ q, long long ld, int R, int C,
+                                                         uint8_t* __restrict__ out, long long ld_out)
+{
+    __shared__ uint8_t t[64][68];
+    const long long r0 = blockIdx.y * 64LL, c0 = blockIdx.x * 64LL;
+    const int x = (threadIdx.x & 15) * 4, y = threadIdx.x >> 4;
+#pragma unroll
+    for (int i = y; i < 64; i += 16) {
+        if (r0 + i >= R) break;
+        const uint8_t* p = q + (r0 + i) * ld + c0 + x;
+        if (c0 + x + 4 <= C) *reinterpret_cast<uint32_t*>(&t[i][x]) = *reinterpret_cast<const uint32_t*>(p);
+        else
+            for (int e = 0; c0 + x + e < C; e++) t[i][x + e] = p[e];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = y; i < 64; i += 16) {
+        if (c0 + i >= C) break;
+        uint32_t w = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) w |= (uint32_t)(r0 + x + e < R ? t[x + e][i] : 0) << (8 * e);
+        // a row's padding up to ld_out is written too, as zeros
+        if (r0 + x < ld_out) *reinterpret_cast<uint32_t*>(out + (c0 + i) * ld_out + r0 + x) = w;
+    }
+}
+
 template <typename T, int ROWS>
 int quant_rows(const void* x, long long ld, int M, int K, uint8_t* q, long long ld_q, float* s, long long ld_s, cudaStream_t st)
 {
@@ -152,4 +179,13 @@ extern "C" int ltq_fp8_quant_blocks(const void* w, int dtype, long long ld, int 
     if (dtype == DT_F32) return quant_blocks<float>(w, ld, N, K, q, ld_q, s, ld_s, st);
     if (dtype == DT_BF16) return quant_blocks<__nv_bfloat16>(w, ld, N, K, q, ld_q, s, ld_s, st);
     return quant_blocks<__half>(w, ld, N, K, q, ld_q, s, ld_s, st);
+}
+
+extern "C" int ltq_fp8_transpose(const uint8_t* q, long long ld, int R, int C, uint8_t* out, long long ld_out, void* stream)
+{
+    if (R < 1 || C < 1 || ld < C || ld % 4 || ld_out < R || ld_out % 16 || !q || (uintptr_t)q % 4 || !out || (uintptr_t)out % 16 ||
+        R > 65535 * 64 || ld_out > ((long long)R + 63) / 64 * 64)
+        return -1;
+    transpose8_kernel<<<dim3((C + 63) / 64, (R + 63) / 64), 256, 0, (cudaStream_t)stream>>>(q, ld, R, C, out, ld_out);
+    return (int)cudaGetLastError();
 }

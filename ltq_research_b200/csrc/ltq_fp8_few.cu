@@ -109,31 +109,33 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
         for (int j = issued > g.stages ? issued - g.stages : 0; j < issued; j++)
             mbar_wait(&empty[j % g.stages], (j / g.stages) & 1, g.err, F_WAIT);
     } else {
-        // x, rows M .. BN - 1 as zeros: a warp per row and two blocks
-        const int pairs = (nb + 1) / 2, units = pairs * BN;
+        // x, a warp per row and two blocks, four of those in flight; rows M .. BN - 1 are zeros
+        const int pairs = (nb + 1) / 2, piece = lane & 15;
         const T* x = (const T*)g.x;
-        Raw8<T> next;
-        auto fetch = [&](int u) {
-            const int m = u % BN, c = (kb0 + 2 * (u / BN)) * QB + 8 * lane;
-            if (u < units && m < g.M) load8(x + m * g.ldx, c, g.K, g.aligned, next);
-        };
-        fetch(warp - 1);
-        for (int u = warp - 1; u < units; u += F_WARPS - 1) {
-            const int m = u % BN, b = 2 * (u / BN) + (lane >> 4);
-            const Raw8<T> cur = next;
-            fetch(u + F_WARPS - 1);
-            uint2 q = make_uint2(0, 0);
-            float scale = 0.f;
-            if (m < g.M) {
-                float v[8];
-                unpack8(cur, v);
-                scale = block_scale(half_warp_amax(v));
-                q = quant8(v, scale);
+        for (int i = tid - 32; i < nb * BN * (QB / 16); i += F_THREADS - 32)
+            if (i / (QB / 16) % BN >= g.M) reinterpret_cast<uint4*>(xq)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = tid - 32; i < nb * BN; i += F_THREADS - 32)
+            if (i % BN >= g.M) xs[i] = 0.f;
+        constexpr int AHEAD = sizeof(T) == 2 ? 4 : 2, STEP = F_WARPS - 1;
+        for (int u0 = warp - 1; u0 < pairs * g.M; u0 += AHEAD * STEP) {
+            Raw8<T> raw[AHEAD];
+#pragma unroll
+            for (int q = 0; q < AHEAD; q++) {
+                const int u = u0 + q * STEP, m = u % g.M, c = (kb0 + 2 * (u / g.M)) * QB + 8 * lane;
+                if (u < pairs * g.M) load8(x + m * g.ldx, c, g.K, g.aligned, raw[q]);
             }
-            if (b < nb) {
-                const int piece = lane & 15;  // eight bytes; 16-byte chunks are swizzled by the row
-                *reinterpret_cast<uint2*>(xq + b * BN * QB + m * QB + (((piece >> 1) ^ (m & 7)) << 4) + (piece & 1) * 8) = q;
-                if (piece == 0) xs[b * BN + m] = scale;
+#pragma unroll
+            for (int q = 0; q < AHEAD; q++) {
+                const int u = u0 + q * STEP, m = u % g.M, b = 2 * (u / g.M) + (lane >> 4);
+                if (u >= pairs * g.M) break;
+                float v[8];
+                unpack8(raw[q], v);
+                const float scale = block_scale(half_warp_amax(v));
+                const uint2 w = quant8(v, scale);
+                if (b < nb) {  // eight bytes; 16-byte chunks are swizzled by the row
+                    *reinterpret_cast<uint2*>(xq + b * BN * QB + m * QB + (((piece >> 1) ^ (m & 7)) << 4) + (piece & 1) * 8) = w;
+                    if (piece == 0) xs[b * BN + m] = scale;
+                }
             }
         }
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // written here, read by the MMAs

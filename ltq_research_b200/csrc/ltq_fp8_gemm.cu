@@ -361,36 +361,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
     }
 }
 
-// tiles whose K was cut: the parts of 32 rows of a CTA's half, summed in the order of K
+// Tiles whose K was cut: the parts of 32 rows and 64 columns, summed in the order of K.
+constexpr int J_COLS = 64;
 template <typename T>
 __global__ void __launch_bounds__(256) join_parts_kernel(const WideArgs g)
 {
-    __shared__ float rows[32][WT + 1];
-    const int tile = g.whole + blockIdx.x, rank = blockIdx.y >> 2, r0 = (blockIdx.y & 3) * 32;
-    const int m0 = (tile % g.mt) * WT + rank * 128 + r0, n0 = (tile / g.mt) * WT;
-    if (m0 >= g.M) return;
+    __shared__ float rows[32][J_COLS + 1];
+    const int tile = g.whole + blockIdx.x, rank = blockIdx.y >> 2, r0 = (blockIdx.y & 3) * 32, col0 = blockIdx.z * J_COLS;
+    const int m0 = (tile % g.mt) * WT + rank * 128 + r0, n0 = (tile / g.mt) * WT + col0;
+    if (m0 >= g.M || n0 >= g.N) return;
     const long long a = (long long)blockIdx.x * g.nkb, b = a + g.nkb, U = g.shared_units;
     const int npairs = g.sharers;
     int c0 = (int)(a * npairs / U);  // the pair whose share holds block a, or the one before it
     while (U * (c0 + 1) / npairs <= a) c0++;
     if (U * c0 / npairs <= a && U * (c0 + 1) / npairs >= b) return;  // one pair did all of the tile
-    const int r = threadIdx.x & 31;
-    for (int c4 = threadIdx.x >> 5; c4 < WT / 4; c4 += 8) {
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c = c0; c < npairs && U * c / npairs < b; c++) {
-            // a share that begins inside the tile left part 0, one that begins at its first block or before it part 1
-            const long long u0 = U * c / npairs;
-            const int slot = u0 > a ? 0 : 1;
-            const float4 x = *reinterpret_cast<const float4*>(
-                g.parts + (((long long)c * 2 + slot) * 2 + rank) * PART_FLOATS + ((long long)c4 * 128 + r0 + r) * 4);
-            v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+    const int r = threadIdx.x & 31, q = threadIdx.x >> 5;
+    float4 v[2] = {};
+    for (int c = c0; c < npairs && U * c / npairs < b; c++) {
+        // a share that begins inside the tile left part 0, one that begins at its first block or before it part 1
+        const int slot = U * c / npairs > a ? 0 : 1;
+        const float* part = g.parts + (((long long)c * 2 + slot) * 2 + rank) * PART_FLOATS + (col0 / 4 * 128LL + r0 + r) * 4;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const float4 x = *reinterpret_cast<const float4*>(part + (q + 8 * h) * 512);
+            v[h].x += x.x, v[h].y += x.y, v[h].z += x.z, v[h].w += x.w;
         }
-        rows[r][4 * c4] = v.x, rows[r][4 * c4 + 1] = v.y, rows[r][4 * c4 + 2] = v.z, rows[r][4 * c4 + 3] = v.w;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        float* o = &rows[r][4 * (q + 8 * h)];
+        o[0] = v[h].x, o[1] = v[h].y, o[2] = v[h].z, o[3] = v[h].w;
     }
     __syncthreads();
-    for (int q = threadIdx.x >> 5; q < 32 && m0 + q < g.M; q += 8)
-        for (int e = threadIdx.x & 31; e < WT && n0 + e < g.N; e += 32)
-            ((T*)g.C)[(long long)(m0 + q) * g.ldc + n0 + e] = from_f<T>(rows[q][e]);
+    for (int i = threadIdx.x; i < 32 * J_COLS; i += 256) {
+        const int m = i / J_COLS, e = i % J_COLS;
+        if (m0 + m < g.M && n0 + e < g.N) ((T*)g.C)[(long long)(m0 + m) * g.ldc + n0 + e] = from_f<T>(rows[m][e]);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------- host side
@@ -446,7 +452,7 @@ int run_wide(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc
     gemm_wide_kernel<T><<<2 * p.pairs, W_THREADS, W_SMEM, st>>>(ta, tb, tc, g);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || p.whole == p.tiles) return (int)e;
-    join_parts_kernel<T><<<dim3(p.tiles - p.whole, 8), 256, 0, st>>>(g);
+    join_parts_kernel<T><<<dim3(p.tiles - p.whole, 8, WT / J_COLS), 256, 0, st>>>(g);
     return (int)cudaGetLastError();
 }
 

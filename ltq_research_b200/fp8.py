@@ -100,8 +100,8 @@ class BlockWeight:
         N, K = self.shape = tuple(q.shape)
         if s.dtype != torch.float32 or tuple(s.shape) != (_blocks(N), _blocks(K)):
             raise ValueError(f"BlockWeight: the scales must be fp32 [{_blocks(N)}, {_blocks(K)}]")
-        self.q, self.s = self._lay(q), s.contiguous()
-        self.qt = self._lay(q.t()) if backward else None
+        self.q, self.s = self._lay(q), s.contiguous()  # before the transpose, which reads them
+        self.qt = self._transposed(N, K) if backward else None
         self.st = s.t().contiguous() if backward else None
 
     @classmethod
@@ -117,6 +117,13 @@ class BlockWeight:
         out = torch.zeros((rows, _pad16(cols)), dtype=torch.uint8, device=q.device)
         out[:, :cols] = u
         return out
+
+    def _transposed(self, N: int, K: int) -> torch.Tensor:
+        qt = torch.empty((K, _pad16(N)), dtype=torch.uint8, device=self.device)
+        with _lib.on_device(self.device):
+            _check(_lib.lib().ltq_fp8_transpose(ptr(self.q), self.q.stride(0), N, K, ptr(qt), qt.shape[1],
+                                                _lib.stream_ptr(self.device)), "ltq_fp8_transpose")
+        return qt
 
     def dequantize(self) -> torch.Tensor:
         """The weight's values in fp32."""
