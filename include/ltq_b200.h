@@ -347,7 +347,7 @@ int ltq_fp8_gemm(const uint8_t* A, long long lda, const float* sa, long long ld_
                  const float* sb, long long ld_sb, void* C, int dtype, long long ldc, int M, int N, int K,
                  void* workspace, size_t workspace_bytes, int* err, void* stream);
 /*
- * ltq_fp8_few: y[m, n] = sum_b sx[m, b] sw[(n / 128) * ld_sw + b] sum_{k in block b} xq[m, k] W[n, k] for 1 to 64 rows x [M, K]
+ * ltq_fp8_few: y[m, n] = sum_b sx[m, b] sw[(n / 128) * ld_sw + b] sum_{k in block b} xq[m, k] W[n, k] for 1 to 32 rows x [M, K]
  *   (dtype), quantized in the call as ltq_fp8_quant_rows does; y [M, N] of out_dtype.  One launch, no workspace.  For shapes that
  *   ltq_fp8_few_supported names (1; else 0: use ltq_fp8_quant_rows and ltq_fp8_gemm).
  */

@@ -115,11 +115,13 @@ class _CountingLib:
         if k is None:
             return fn
 
+        lock, varies = self._lock, callable(k)
+
         def call(*a):
             rc = fn(*a)
             if rc == 0:
-                n = k(a) if callable(k) else k
-                with self._lock:
+                n = k(a) if varies else k
+                with lock:
                     self.kernels += n
             return rc
         call.__name__ = name
@@ -169,9 +171,10 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
             continue
         if not t.is_cuda:
             raise RuntimeError("ltq_research_b200: inputs must be CUDA tensors (there is no CPU implementation)")
+        d = t.device
         if dev is None:
-            dev = t.device
-        elif t.device != dev:
+            dev = d
+        elif d != dev:
             raise RuntimeError("ltq_research_b200: all inputs must be on the same CUDA device")
     if dev is None:
         raise RuntimeError("ltq_research_b200: no CUDA tensor given")
@@ -180,7 +183,7 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
 
 def on_device(device: torch.device):
     """Context with `device` current, as a launch on its streams needs."""
-    return _SAME if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _SAME if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 _SAME = nullcontext()

@@ -20,6 +20,24 @@ __device__ __forceinline__ bool elect_one()
     return p != 0;
 }
 
+// 16 columns of tensor memory of this warp's lanes; the registers may be used after tmem_ld_done
+__device__ __forceinline__ void tmem_ld16_start(uint32_t taddr, uint32_t* r)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+template <int N>
+__device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[N])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+r"(r[i]));  // no use of a register moves above the wait
+}
+
 inline bool make_map_8(CUtensorMap* m, const void* base, long long rows, long long cols, long long ld, int box_rows)
 {
     auto f = encode_fn();

@@ -1,12 +1,12 @@
-// y = x W^T for few rows x (at most 64) and a block-scaled e4m3 weight, in one launch (B200, sm_100a).
+// y = x W^T for few rows x (at most 32) and a block-scaled e4m3 weight, in one launch (B200, sm_100a).
 //
 // The weight is read once and is all of the traffic, so the kernel is a stream of weight blocks with everything else kept out
 // of its way.  The roles of the operands are exchanged: 128 rows of the weight are the M side of tcgen05.mma and the rows of x,
-// padded to 16, 32 or 64, its N side, so a block of 128 x 128 weights costs a fraction of its load's time.  A CTA quantizes its
+// padded to 16 or 32, its N side, so a block of 128 x 128 weights costs a fraction of its load's time.  A CTA quantizes its
 // share of x once, into shared memory in the layout the MMAs read, while the first weight blocks are on their way.
 //
 //   warp 0        TMA producer: weight blocks [128 rows][128 of K] into a ring
-//   warp 1        MMA issuer: four tcgen05.mma a block into one of 4 or 8 tensor-memory buffers
+//   warp 1        MMA issuer: four tcgen05.mma a block into tensor-memory buffers of two blocks
 //   warps 2 .. 5  epilogue: lane = weight row; each block's sums times sw sx added to fp32 registers
 //   warps 1 ..    first quantize x
 //
@@ -18,6 +18,7 @@
 
 namespace {
 
+constexpr int F_ROWS = 32;
 constexpr int F_THREADS = 384, F_WARPS = F_THREADS / 32;
 constexpr int F_STAGES = 12, F_MIN_STAGES = 4, F_STAGE = 128 * QB;  // weight blocks of 16 KB on their way
 constexpr int F_SMEM = 226 * 1024;
@@ -51,7 +52,8 @@ __device__ __forceinline__ void arrive(uint64_t* b)
 template <typename T, int BN>
 __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(const __grid_constant__ CUtensorMap tmW, const FewArgs g)
 {
-    constexpr int F_BUFS = BN <= 32 ? 8 : 4;
+    constexpr int PER = 2;                    // blocks whose sums are handed over together
+    constexpr int F_BUFS = BN == 16 ? 8 : 4;  // tensor-memory buffers
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* ring = smem;
@@ -63,7 +65,7 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
     uint64_t* accfull = empty + F_STAGES;
     uint64_t* accempty = accfull + F_BUFS;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accempty + F_BUFS);
-    constexpr int COLS = F_BUFS * BN;  // tensor memory: 128 or 256 columns
+    constexpr int COLS = F_BUFS * PER * BN;  // 256 columns
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = g.splits > 1 ? (int)cluster_rank() : 0;
@@ -116,7 +118,7 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
             if (i / (QB / 16) % BN >= g.M) reinterpret_cast<uint4*>(xq)[i] = make_uint4(0, 0, 0, 0);
         for (int i = tid - 32; i < nb * BN; i += F_THREADS - 32)
             if (i % BN >= g.M) xs[i] = 0.f;
-        constexpr int AHEAD = sizeof(T) == 2 ? 4 : 2, STEP = F_WARPS - 1;
+        constexpr int AHEAD = 4, STEP = F_WARPS - 1;
         for (int u0 = warp - 1; u0 < pairs * g.M; u0 += AHEAD * STEP) {
             Raw8<T> raw[AHEAD];
 #pragma unroll
@@ -149,20 +151,22 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
             bool ok = true;
             for (int tile = worker; tile < g.tiles && ok; tile += workers)
                 for (int k = 0; k < nb; k++) {
-                    ok = mbar_wait(&full[st], full_parity, g.err, F_WAIT) && mbar_wait(&accempty[buf], free_parity, g.err, F_WAIT);
+                    ok = mbar_wait(&full[st], full_parity, g.err, F_WAIT) &&
+                         (k % PER || mbar_wait(&accempty[buf], free_parity, g.err, F_WAIT));
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t a = wdesc + (uint32_t)(st * (F_STAGE >> 4)), b = xdesc + (uint32_t)(k * (BN * QB >> 4));
+                    const bool last = k % PER == PER - 1 || k + 1 == nb;  // the buffer is complete
                     if (elect_one()) {
 #pragma unroll
-                        for (int kk = 0; kk < 4; kk++) mma_f8<BN>(tm + buf * BN, a + 2 * kk, b + 2 * kk, kk != 0);
-                        umma_commit(&accfull[buf]);
+                        for (int kk = 0; kk < 4; kk++) mma_f8<BN>(tm + (PER * buf + k % PER) * BN, a + 2 * kk, b + 2 * kk, kk != 0);
+                        if (last) umma_commit(&accfull[buf]);
                         umma_commit(&empty[st]);
                     }
                     __syncwarp();
                     if (++st == g.stages) st = 0, full_parity ^= 1;
-                    if (++buf == F_BUFS) buf = 0, free_parity ^= 1;
+                    if (last && ++buf == F_BUFS) buf = 0, free_parity ^= 1;
                 }
         } else if (warp < 6) {
             const int quarter = warp & 3, row = 32 * quarter + lane;
@@ -176,27 +180,35 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
                 for (int j = 0; j < BN; j++) acc[j] = 0.f;
                 const float* sb = g.sb + (long long)tile * g.ld_sb + kb0;
                 float sw32 = 0.f;
-                for (int k = 0; k < nb; k++) {
+                for (int k = 0; k < nb; k += PER) {
                     if ((k & 31) == 0) sw32 = k + lane < nb ? sb[k + lane] : 0.f;  // a lane each for 32 blocks
-                    const float sw = __shfl_sync(0xffffffffu, sw32, k & 31);
+                    float sw[PER];
+#pragma unroll
+                    for (int h = 0; h < PER; h++) sw[h] = __shfl_sync(0xffffffffu, sw32, (k + h) & 31);
                     ok = __all_sync(0xffffffffu, mbar_wait(&accfull[buf], parity, g.err, F_WAIT));
                     if (!ok) break;
                     tc_fence_after();
-                    float part[BN];
+                    uint32_t part[PER * BN];  // behind a single last block the second half is not used
 #pragma unroll
-                    for (int c = 0; c < BN; c += 16) tmem_ld16(tl + buf * BN + c, *reinterpret_cast<float (*)[16]>(part + c));
+                    for (int c = 0; c < PER * BN; c += 16) tmem_ld16_start(tl + buf * PER * BN + c, part + c);
+                    tmem_ld_done(part);
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) arrive(&accempty[buf]);
                     if (++buf == F_BUFS) buf = 0, parity ^= 1;
-                    const float4* s4 = reinterpret_cast<const float4*>(xs + k * BN);
 #pragma unroll
-                    for (int j = 0; j < BN; j += 4) {
-                        const float4 s = s4[j / 4];
-                        acc[j] = fmaf(part[j], sw * s.x, acc[j]);
-                        acc[j + 1] = fmaf(part[j + 1], sw * s.y, acc[j + 1]);
-                        acc[j + 2] = fmaf(part[j + 2], sw * s.z, acc[j + 2]);
-                        acc[j + 3] = fmaf(part[j + 3], sw * s.w, acc[j + 3]);
+                    for (int h = 0; h < PER; h++) {
+                        if (k + h >= nb) break;
+                        const float4* s4 = reinterpret_cast<const float4*>(xs + (k + h) * BN);
+#pragma unroll
+                        for (int j = 0; j < BN; j += 4) {
+                            const float4 s = s4[j / 4];
+                            const uint32_t* q = part + h * BN + j;
+                            acc[j] = fmaf(__uint_as_float(q[0]), sw[h] * s.x, acc[j]);
+                            acc[j + 1] = fmaf(__uint_as_float(q[1]), sw[h] * s.y, acc[j + 1]);
+                            acc[j + 2] = fmaf(__uint_as_float(q[2]), sw[h] * s.z, acc[j + 2]);
+                            acc[j + 3] = fmaf(__uint_as_float(q[3]), sw[h] * s.w, acc[j + 3]);
+                        }
                     }
                 }
                 if (!ok) break;
@@ -250,16 +262,18 @@ struct FewPlan {
 };
 // The quantized x of a CTA's share of K stays in its shared memory beside at least four weight blocks.  K is cut (2, 4 or 8 ways)
 // where that takes it, and further while the CTAs all run at once (two an SM of at most 16 rows) with four blocks of K or more
-// each.  False, for the other kernels, where more CTAs than that would each have to quantize their x, and for more than 64 rows.
+// each.  False, for the other kernels, where more CTAs than that would each have to quantize their x, and for more than 32 rows:
+// at 64 (one block a buffer, 88 us for 128256 x 2048) the 256-row tiles behind a separate quantization are as fast (83 us).
 bool plan_few(int M, int N, int K, int sms, FewPlan& p)
 {
-    if (M < 1 || M > 64 || N < 1 || K < 1 || sms < 1) return false;
-    p.bn = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+    if (M < 1 || M > F_ROWS || N < 1 || K < 1 || sms < 1) return false;
+    p.bn = M <= 16 ? 16 : 32;
     p.nkb = (int)(((long long)K + QB - 1) / QB);
     p.tiles = (int)(((long long)N + 127) / 128);
     const int block = p.bn * (QB + 4), hand = p.bn * 512, fixed = 512 + 1024;  // bytes: x and its scales of a block; joined columns
     auto share = [&](int splits) { return (p.nkb + splits - 1) / splits; };
     auto need = [&](int splits, int stages) { return stages * F_STAGE + share(splits) * block + (splits > 1 ? hand : 0) + fixed; };
+    if (p.bn > 16 && p.tiles < sms) return false;  // quantizing so much in every CTA pays where each then reads a row tile or more
     p.splits = 1;
     while (p.splits < 8 && need(p.splits, F_MIN_STAGES) > F_SMEM) p.splits *= 2;
     if (need(p.splits, F_MIN_STAGES) > F_SMEM || (p.splits > 1 && (long long)p.tiles * p.splits > sms)) return false;
@@ -304,9 +318,7 @@ int run_few(const CUtensorMap& tw, const FewArgs& g, const FewPlan& p, cudaStrea
 template <typename T>
 int few_type(const CUtensorMap& tw, const FewArgs& g, const FewPlan& p, cudaStream_t st)
 {
-    if (p.bn == 16) return run_few<T, 16>(tw, g, p, st);
-    if (p.bn == 32) return run_few<T, 32>(tw, g, p, st);
-    return run_few<T, 64>(tw, g, p, st);
+    return p.bn == 16 ? run_few<T, 16>(tw, g, p, st) : run_few<T, 32>(tw, g, p, st);
 }
 
 }  // namespace

@@ -66,26 +66,30 @@ def _like(logits: torch.Tensor, ld: int) -> torch.Tensor:
 
 def _call(logits, idx, teacher, teacher_lse, weight, temperature, mode, stats=None, grad=None, out=None, want_stats=False):
     dev = _lib.require_cuda(logits, idx, teacher, teacher_lse, weight, stats, grad, out)
-    if logits.dtype not in DTYPES or teacher.dtype not in DTYPES:
+    code, tcode, itype = DTYPES.get(logits.dtype), DTYPES.get(teacher.dtype), idx.dtype
+    if code is None or tcode is None:
         raise TypeError("distill: logits and teacher must be fp32, bf16 or fp16")
-    if idx.dtype not in (torch.int32, torch.int64):
+    if itype is not torch.int64 and itype is not torch.int32:
         raise TypeError("distill: idx must be int32 or int64")
     ld = _rows(logits, "logits")
-    T, V = logits.shape
-    if idx.dim() != 2 or idx.shape[0] != T or teacher.shape != idx.shape:
+    ld_i, ld_u = _rows(idx, "idx"), _rows(teacher, "teacher")
+    (T, V), (Ti, K) = logits.shape, idx.shape
+    if Ti != T or teacher.shape != idx.shape:
         raise ValueError(f"distill: idx and teacher must both be [{T}, K]")
-    K = idx.shape[1]
     if not 1 <= K <= MAX_K or not 1 <= V <= MAX_VOCAB:
         raise ValueError(f"distill: between 1 and {MAX_K} slots and between 1 and {MAX_VOCAB} tokens are supported")
     if not 0.0 < temperature < float("inf"):
         raise ValueError("distill: the temperature must be positive and finite")
-    ld_i, ld_u = _rows(idx, "idx"), _rows(teacher, "teacher")
-    teacher_lse, weight = _vector(teacher_lse, T, "teacher_lse"), _vector(weight, T, "weight")
+    if teacher_lse is not None:
+        teacher_lse = _vector(teacher_lse, T, "teacher_lse")
+    if weight is not None:
+        weight = _vector(weight, T, "weight")
     loss = dlogits = None
     ld_d = s_grad = 0
     if mode != GRAD:
         loss = torch.empty(T, dtype=torch.float32, device=dev)
-        stats = torch.empty((T, 3), dtype=torch.float32, device=dev) if want_stats else None
+        if want_stats:
+            stats = torch.empty((T, 3), dtype=torch.float32, device=dev)
     else:
         if stats.dtype != torch.float32 or stats.shape != (T, 3) or not stats.is_contiguous():
             raise ValueError(f"distill: stats must be the [{T}, 3] that topk_loss returned")
@@ -106,9 +110,9 @@ def _call(logits, idx, teacher, teacher_lse, weight, temperature, mode, stats=No
         ld_d = _rows(dlogits, "out")
     with _lib.on_device(dev):
         rc = _lib.lib().ltq_distill_topk(
-            ptr(logits), DTYPES[logits.dtype], ld, ptr(idx), int(idx.dtype == torch.int64), ld_i, ptr(teacher),
-            DTYPES[teacher.dtype], ld_u, ptr(teacher_lse), ptr(weight), ptr(grad), s_grad, T, V, K, float(temperature),
-            mode, ptr(loss), ptr(stats), ptr(dlogits), ld_d, _lib.stream_ptr(dev))
+            logits.data_ptr(), code, ld, idx.data_ptr(), itype is torch.int64, ld_i, teacher.data_ptr(), tcode, ld_u,
+            ptr(teacher_lse), ptr(weight), ptr(grad), s_grad, T, V, K, temperature, mode, ptr(loss), ptr(stats),
+            ptr(dlogits), ld_d, _lib.stream_ptr(dev))
     if rc != 0:
         raise RuntimeError(f"ltq_distill_topk: error code {rc}")
     return loss, stats, dlogits

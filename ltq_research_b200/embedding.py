@@ -25,34 +25,38 @@ def _tokens(tokens: torch.Tensor) -> torch.Tensor:
 
 
 def _row_stride(t: torch.Tensor, what: str) -> int:
-    if t.dim() != 2 or t.shape[1] < 1 or (t.shape[1] > 1 and t.stride(1) != 1):
+    if t.dim() != 2:
         raise ValueError(f"embedding: {what} must be 2-D with unit column stride")
-    if t.shape[0] <= 1:
-        return t.shape[1]
-    if t.stride(0) < t.shape[1]:
+    rows, cols = t.shape
+    ld, step = t.stride()
+    if cols < 1 or (cols > 1 and step != 1):
+        raise ValueError(f"embedding: {what} must be 2-D with unit column stride")
+    if rows <= 1:
+        return cols
+    if ld < cols:
         raise ValueError(f"embedding: the rows of {what} overlap")
-    return t.stride(0)
+    return ld
 
 
 def lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """scale * table[tokens]: table [V, D] fp32, bf16 or fp16, tokens of any shape -> [*tokens.shape, D]."""
     dev = _lib.require_cuda(table, tokens, out)
-    if table.dtype not in DTYPES:
+    code = DTYPES.get(table.dtype)
+    if code is None:
         raise TypeError("embedding: the table must be fp32, bf16 or fp16")
     ld = _row_stride(table, "the table")
     V, D = table.shape
     if V < 1:
         raise ValueError("embedding: the table has no rows")
     tok = _tokens(tokens)
-    shape = (*tokens.shape, D)
     if out is None:
-        out = torch.empty(shape, dtype=table.dtype, device=dev)
-    elif out.dtype != table.dtype or out.shape != shape or not out.is_contiguous():
+        out = torch.empty((*tokens.shape, D), dtype=table.dtype, device=dev)
+    elif out.dtype != table.dtype or out.shape != (*tokens.shape, D) or not out.is_contiguous():
         raise ValueError("embedding: out must be contiguous, of the table's type and shape [*tokens.shape, D]")
     with _lib.on_device(dev):
-        rc = _lib.lib().ltq_embed_lookup(ptr(table), DTYPES[table.dtype], ld, ptr(tok), int(tok.dtype == torch.int64),
-                                         tok.numel(), V, D, float(scale), ptr(out), D, _lib.stream_ptr(dev))
+        rc = _lib.lib().ltq_embed_lookup(table.data_ptr(), code, ld, tok.data_ptr(), tok.dtype is torch.int64, tok.numel(), V, D,
+                                         scale, out.data_ptr(), D, _lib.stream_ptr(dev))
     if rc != 0:
         raise RuntimeError(f"ltq_embed_lookup: error code {rc}")
     return out

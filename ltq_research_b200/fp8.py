@@ -21,7 +21,7 @@ from . import _lib
 from ._lib import DTYPES, ptr
 
 BLOCK = 128
-FEW = 64  # rows up to which one launch quantizes them and streams the weight (ltq_fp8_few)
+FEW = 32  # rows up to which one launch quantizes them and streams the weight (ltq_fp8_few)
 E4M3 = torch.float8_e4m3fn
 
 
@@ -33,9 +33,16 @@ def _pad16(n: int) -> int:
     return (n + 15) // 16 * 16
 
 
+_FLAGS = {}
+
+
 def _error_flag(dev: torch.device) -> torch.Tensor:
-    from .liqk_v2 import gemm_error_flag  # the tensor-core products' common flag
-    return gemm_error_flag(dev)
+    """The tensor-core products' common flag of a device."""
+    flag = _FLAGS.get(dev)
+    if flag is None:
+        from .liqk_v2 import gemm_error_flag
+        flag = _FLAGS[dev] = gemm_error_flag(dev)
+    return flag
 
 
 def _check(rc: int, what: str):
@@ -134,7 +141,8 @@ class BlockWeight:
 
 def _product(x: torch.Tensor, q: torch.Tensor, s: torch.Tensor, N: int, K: int, dtype: Optional[torch.dtype]) -> torch.Tensor:
     dtype = x.dtype if dtype is None else dtype
-    if dtype not in DTYPES:
+    code = DTYPES.get(dtype)
+    if code is None:
         raise TypeError("fp8: the output must be fp32, bf16 or fp16")
     shape = x.shape
     if len(shape) < 1 or shape[-1] != K:
@@ -145,7 +153,12 @@ def _product(x: torch.Tensor, q: torch.Tensor, s: torch.Tensor, N: int, K: int, 
     ld, step = x2.stride()
     if (K > 1 and step != 1) or (M > 1 and ld < K):
         x2 = x2.contiguous()
-    ld = _rows(x2, "x")
+        ld = K
+    if M <= 1:
+        ld = K
+    xcode = DTYPES.get(x2.dtype)
+    if xcode is None:
+        raise TypeError("fp8: x must be fp32, bf16 or fp16")
     y = torch.empty((*shape[:-1], N), dtype=dtype, device=dev)
     if M == 0:
         return y
@@ -153,14 +166,14 @@ def _product(x: torch.Tensor, q: torch.Tensor, s: torch.Tensor, N: int, K: int, 
     with _lib.on_device(dev):
         st, err = _lib.stream_ptr(dev), ptr(_error_flag(dev))
         if M <= FEW and L.ltq_fp8_few_supported(M, N, K):
-            _check(L.ltq_fp8_few(ptr(x2), DTYPES[x2.dtype], ld, ptr(q), q.stride(0), ptr(s), s.shape[1], ptr(y), DTYPES[dtype],
-                                 N, M, N, K, err, st), "ltq_fp8_few")
+            _check(L.ltq_fp8_few(x2.data_ptr(), xcode, ld, q.data_ptr(), q.stride(0), s.data_ptr(), s.shape[1], y.data_ptr(),
+                                 code, N, M, N, K, err, st), "ltq_fp8_few")
             return y
         xq, xs = _quantize_rows(x2, ld)
         nws = L.ltq_fp8_gemm_workspace_bytes(M, N, K)
         ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
         _check(L.ltq_fp8_gemm(ptr(xq), xq.shape[1], ptr(xs), xs.shape[1], ptr(q), q.stride(0), ptr(s), s.shape[1], ptr(y),
-                              DTYPES[dtype], N, M, N, K, ptr(ws), nws, err, st), "ltq_fp8_gemm")
+                              code, N, M, N, K, ptr(ws), nws, err, st), "ltq_fp8_gemm")
     return y
 
 
