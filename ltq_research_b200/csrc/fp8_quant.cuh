@@ -15,40 +15,29 @@ __device__ __forceinline__ float block_scale(uint32_t amax_bits)  // the largest
     const float s = __fdiv_rn(__uint_as_float(amax_bits), E4M3_MAX);
     return s < S_MIN ? S_MIN : s;
 }
-// x / s rounded correctly without a division each: with r = 1 / s correctly rounded, q = x r and then q + (x - q s) r is the
-// correctly rounded quotient (Markstein's correction, IBM J. Res. Dev. 34, 1990) while the remainder stays above the smallest
-// normal number, which 2^-80 <= s guarantees for every quotient that e4m3 does not round to 0
-__device__ __forceinline__ float quotient(float x, float s, float r)
+// eight values under one scale s (r: its reciprocal, rounded correctly), as eight bytes.  The quotients x / s are rounded correctly
+// without a division each: q = x r and then q + (x - q s) r is the correctly rounded quotient (Markstein's correction, IBM J.
+// Res. Dev. 34, 1990) while the remainder stays above the smallest normal number, which 2^-80 <= s guarantees for every quotient
+// that e4m3 does not round to 0
+__device__ __forceinline__ uint2 quant8(float (&v)[8], float s, float r)
 {
-    const float q = __fmul_rn(x, r);
-    return __fmaf_rn(__fmaf_rn(-q, s, x), r, q);
-}
-// eight values under one scale, as eight bytes
-__device__ __forceinline__ uint2 quant8(float (&v)[8], float scale)
-{
-    if (!(scale >= 0x1p-80f)) {  // a tiny scale, or NaN
+    if (!(s >= 0x1p-80f)) {  // a tiny scale, or NaN
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = __fdiv_rn(v[i], scale);
+        for (int i = 0; i < 8; i++) v[i] = __fdiv_rn(v[i], s);
     } else {
-        const float r = __frcp_rn(scale);
+        const uint64_t rr = pair(r, r), ns = pair(-s, -s);
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = quotient(v[i], scale, r);
+        for (int i = 0; i < 8; i += 2) {
+            const uint64_t x = pair(v[i], v[i + 1]), q = mul2(x, rr);
+            const float2 y = unpair(fma2(fma2(q, ns, x), rr, q));
+            v[i] = y.x, v[i + 1] = y.y;
+        }
     }
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; i++)
         w[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
     return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
-}
-// the largest |v| of a block whose eight-value pieces lie on half a warp
-__device__ __forceinline__ uint32_t half_warp_amax(const float (&v)[8])
-{
-    uint32_t a = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) a = max(a, abs_bits(v[i]));
-#pragma unroll
-    for (int o = 8; o; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-    return a;
 }
 
 // eight elements of a row from column c on (zeros beyond K), as they are
@@ -76,5 +65,46 @@ __device__ __forceinline__ void unpack8(const Raw8<float>& x, float (&f)[8])
 }
 __device__ __forceinline__ void unpack8(const Raw8<__nv_bfloat16>& x, float (&f)[8]) { unpack16(x.u[0], f, __nv_bfloat16()); }
 __device__ __forceinline__ void unpack8(const Raw8<__half>& x, float (&f)[8]) { unpack16(x.u[0], f, __half()); }
+
+// the largest |x| of eight elements, by its fp32 bits (16-bit types: two at a time, as unsigned integers, NaN above infinity)
+__device__ __forceinline__ uint32_t amax8(const Raw8<float>& x)
+{
+    float f[8];
+    unpack8(x, f);
+    uint32_t a = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) a = max(a, abs_bits(f[i]));
+    return a;
+}
+__device__ __forceinline__ uint32_t amax16_bits(const uint4& u)
+{
+    const uint32_t m = 0x7fff7fffu;
+    const uint32_t a = __vmaxu2(__vmaxu2(u.x & m, u.y & m), __vmaxu2(u.z & m, u.w & m));
+    return max(a >> 16, a & 0xffffu);
+}
+__device__ __forceinline__ uint32_t amax8(const Raw8<__nv_bfloat16>& x) { return amax16_bits(x.u[0]) << 16; }
+__device__ __forceinline__ uint32_t amax8(const Raw8<__half>& x)
+{
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)amax16_bits(x.u[0]))));
+}
+// over the half warp that holds a block
+__device__ __forceinline__ uint32_t half_warp_max(uint32_t a)
+{
+#pragma unroll
+    for (int o = 8; o; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+    return a;
+}
+// The scales and reciprocals of four pairs of blocks (a half warp each), given their largest magnitudes: each lane divides for one
+// of the four, the others take it from there.
+__device__ __forceinline__ void scales4(const uint32_t (&a)[4], int lane, float (&s)[4], float (&r)[4])
+{
+    const uint32_t mine = lane & 2 ? (lane & 1 ? a[3] : a[2]) : (lane & 1 ? a[1] : a[0]);
+    const float sc = block_scale(mine), rc = __frcp_rn(sc);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        s[j] = __shfl_sync(0xffffffffu, sc, (lane & 16) | j);
+        r[j] = __shfl_sync(0xffffffffu, rc, (lane & 16) | j);
+    }
+}
 
 }  // namespace

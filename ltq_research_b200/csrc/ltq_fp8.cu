@@ -57,18 +57,22 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) quant_rows_kernel
         if (m + 1 < m1)  // the next row's loads are on their way while this one is worked on
 #pragma unroll
             for (int j = 0; j < 4; j++) load8(x + (m + 1) * ld, c0 + 256 * j + 8 * lane, K, aligned, next[j]);
+        uint32_t a[4];
+        float scale[4], rec[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) a[j] = half_warp_max(amax8(cur[j]));
+        scales4(a, lane, scale, rec);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             float v[8];
             unpack8(cur[j], v);
-            const float scale = block_scale(half_warp_amax(v));
-            const uint2 w = quant8(v, scale);
+            const uint2 w = quant8(v, scale[j], rec[j]);
             const int c = c0 + 256 * j + 8 * lane;
             uint8_t* o = q + m * ld_q + c;
             if (c + 8 <= K) *reinterpret_cast<uint2*>(o) = w;
             else
                 for (int i = 0; c + i < K; i++) o[i] = (uint8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
-            if ((lane & 15) == 0) sc[2 * j + (lane >> 4)][m - mb] = scale;
+            if ((lane & 15) == 0) sc[2 * j + (lane >> 4)][m - mb] = scale[j];
         }
     }
     __syncthreads();

@@ -132,8 +132,8 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
                 if (u >= pairs * g.M) break;
                 float v[8];
                 unpack8(raw[q], v);
-                const float scale = block_scale(half_warp_amax(v));
-                const uint2 w = quant8(v, scale);
+                const float scale = block_scale(half_warp_max(amax8(raw[q])));
+                const uint2 w = quant8(v, scale, __frcp_rn(scale));
                 if (b < nb) {  // eight bytes; 16-byte chunks are swizzled by the row
                     *reinterpret_cast<uint2*>(xq + b * BN * QB + m * QB + (((piece >> 1) ^ (m & 7)) << 4) + (piece & 1) * 8) = w;
                     if (piece == 0) xs[b * BN + m] = scale;
