@@ -314,19 +314,21 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
         // the bits of this thread's vectors: at a fixed step (and, of four-element vectors, a fixed half of a byte)
         const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bits) + (VEC == 8 ? tid + 1 : (tid + 1) >> 1);
         constexpr int step = VEC == 8 ? D_THREADS : D_THREADS / 2;
-        auto add = [&](uint4 raw, int t) {
+        auto masked = [&](uint4 raw, int t) {  // the slots' tokens as -infinity
             if (REST) {
                 const uint32_t by = bytes[t * step], mb = VEC == 8 ? by : by >> (((tid + 1) & 1) * 4) & 15u;
                 if (mb) raw = mask16(raw, mb, T());
             }
-            const float vm = __fmul_rn(max16(raw, T()), c);
+            return raw;
+        };
+        auto raise = [&](float vm) {  // the running maximum
             if (vm > m) {
                 const float f = ex2(m - vm);
                 s2 = mul2(s2, pair(f, f));
                 m = vm;
             }
-            const float b = m == -INFINITY ? 0.f : -m;
-            const uint64_t bb = pair(b, b);
+        };
+        auto sum = [&](const uint4& raw, uint64_t bb) {
             float x[VEC];
             unpack16(raw, x, T());
 #pragma unroll
@@ -335,15 +337,30 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
                 s2 = add2(s2, pair(ex2(e.x), ex2(e.y)));
             }
         };
+        auto add = [&](uint4 raw, int t) {
+            raw = masked(raw, t);
+            raise(__fmul_rn(max16(raw, T()), c));
+            const float b = m == -INFINITY ? 0.f : -m;
+            sum(raw, pair(b, b));
+        };
+        auto add_both = [&](uint4 r0, uint4 r1, int t) {  // vectors t and t + 1, one look at the maximum
+            r0 = masked(r0, t), r1 = masked(r1, t + 1);
+            raise(__fmul_rn(fmaxf(max16(r0, T()), max16(r1, T())), c));
+            const float b = m == -INFINITY ? 0.f : -m;
+            const uint64_t bb = pair(b, b);
+            sum(r0, bb);
+            sum(r1, bb);
+        };
         int t = 0;
         if (GRAD) {
             cp_wait<3>();
-            for (const int e = min(nth, bt); t < e; t++) add(held_vec(t), t);
+            for (const int e = min(nth, bt); t + 1 < e; t += 2) add_both(held_vec(t), held_vec(t + 1), t);
             cp_wait<2>();
-            for (const int e = min(nth, 2 * bt); t < e; t++) add(held_vec(t), t);
+            for (const int e = min(nth, 2 * bt); t + 1 < e; t += 2) add_both(held_vec(t), held_vec(t + 1), t);
             cp_wait<1>();
-            for (const int e = min(nth, 3 * bt); t < e; t++) add(held_vec(t), t);
+            for (const int e = min(nth, 3 * bt); t + 1 < e; t += 2) add_both(held_vec(t), held_vec(t + 1), t);
             cp_wait<0>();
+            for (; t + 1 < nth; t += 2) add_both(held_vec(t), held_vec(t + 1), t);
             for (; t < nth; t++) add(held_vec(t), t);
         }
         for (; t + 4 <= nt; t += 4) {
@@ -351,7 +368,7 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
 #pragma unroll
             for (int q = 0; q < 4; q++) u[q] = __ldg(zt + (t + q) * D_THREADS);
 #pragma unroll
-            for (int q = 0; q < 4; q++) add(u[q], t + q);
+            for (int q = 0; q < 4; q += 2) add_both(u[q], u[q + 1], t + q);
         }
         for (; t < nt; t++) add(__ldg(zt + t * D_THREADS), t);
         const float2 e = unpair(s2);
