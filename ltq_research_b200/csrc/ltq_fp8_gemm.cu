@@ -9,11 +9,18 @@
 // of the sums): per block 32 KB of operands a CTA for 2 * 128^2 * 256 operations, 64 bytes a clock of L2 reads an SM at full rate,
 // where one CTA with a 128 x 256 tile would need 96.
 //
-//   warp 8        lane 0: TMA producer, A and B blocks into a ring of W_STAGES buffers (128-byte swizzle) on both CTAs; the
-//                 bytes of both are counted on the first CTA's "full" mbarrier
-//   warp 9        lane 0 of the first CTA: four tcgen05.mma (K 32 each) a block; tcgen05.commit frees the buffers of both CTAs
-//                 and hands the sum to both CTAs' epilogue warps
+//   warp 8        TMA producer, A and B blocks into a ring of W_STAGES buffers (128-byte swizzle) on both CTAs; the bytes of both
+//                 are counted on the first CTA's "full" mbarrier
+//   warp 9        of the first CTA: four tcgen05.mma (K 32 each) a block; tcgen05.commit frees the buffers of both CTAs and hands
+//                 the sum to both CTAs' epilogue warps
 //   warps 0 .. 7  epilogue: lanes' quarter w % 4 of the rows, half w / 4 of the columns, 128 sums a thread
+// Warps 8 and 9 run whole and one elected lane issues: from a single-lane branch the operands of the MMAs leave the uniform
+// registers, which cost 800 cycles a block.
+//
+// What bounds it: a block's MMAs take 512 cycles a pair, and the chain sum complete -> read (two rounds of 64 columns, for which
+// the registers beside the sums suffice) -> buffer handed back -> next MMAs about twice that, over two buffers.  8192 x 8192 x
+// 4096: 235 us, 2340 TFLOP/s (the MMAs alone, without epilogue, 160 us; a 256 x 128 tile with four buffers 290 us, for each hand-over
+// costs the issuing warp the same).
 //
 // Pairs walk the tiles (rows first, so that neighbours share B in L2).  What is left after the last full round of tiles is cut
 // along K into equal shares (a share may end inside a tile); the parts go to a workspace and join_parts_kernel adds them in the
@@ -32,11 +39,12 @@ __device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
     return a;
 }
-// Arrival on an mbarrier of either CTA.  What it guards is tensor memory, ordered by the tcgen05 fences, so it carries no
-// cluster-wide release: that waits for the warp's outstanding loads and cost 2000 cycles a block of K.
+// Arrival on an mbarrier of either CTA.  What it guards is tensor memory, whose reads have completed (tcgen05.wait::ld) and are
+// ordered by the tcgen05 fences; so it is relaxed: a cluster-wide release waits for the warp's outstanding loads and cost 2000
+// cycles a block of K.
 __device__ __forceinline__ void arrive_cluster(uint32_t addr)
 {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(addr) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(addr) : "memory");
 }
 // the copy lands in this CTA's shared memory, its bytes are counted on the mbarrier at `bar` (of either CTA of the pair)
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar)
@@ -94,6 +102,7 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
 constexpr int WT = 256;                                  // tile of a pair, both ways
 constexpr int W_STAGES = 6;
 constexpr int W_OP = 128 * QB, W_STAGE = 2 * W_OP;       // one operand's block of a CTA: 16 KB
+constexpr int W_AHEAD = 8;                               // blocks whose scales are fetched together, one group ahead
 constexpr int W_THREADS = 384;
 // registers a thread: 168 at launch (384 x 168 = 64512 of the SM's 65536); the epilogue's eight warps take 232, the others keep 40
 constexpr int W_REGS_EPILOGUE = 232, W_REGS_ROLES = 40;
@@ -267,27 +276,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
             float acc[128];
 #pragma unroll
             for (int j = 0; j < 128; j++) acc[j] = 0.f;
-            float sc[4], na[4], nb[4];  // scales of four blocks, and of the next four on their way: L2 answers later than a block
+            // sa of W_AHEAD blocks, and of as many more on their way: L2 answers later than several blocks take while the
+            // operands stream.  sb comes for 32 blocks at a time, a lane each.  The loads go past L1, whose fills would take
+            // shared-memory cycles from the MMAs' operands (8192 x 8192 x 4096: 265 us with them, 242 without).
+            float sa[W_AHEAD], na[W_AHEAD], sb32 = 0.f, nb32;
             auto fetch = [&](int k) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const bool in = live && k + j < s.k1;
-                    na[j] = in ? pa[(k + j) * g.ld_sa] : 0.f;
-                    nb[j] = in ? pb[k + j] : 0.f;
-                }
+                for (int j = 0; j < W_AHEAD; j++) na[j] = live && k + j < s.k1 ? __ldcg(pa + (k + j) * g.ld_sa) : 0.f;
             };
+            auto fetch_b = [&](int k) { return n0 < g.N && k + lane < s.k1 ? __ldcg(pb + k + lane) : 0.f; };
             fetch(s.k0);
-            for (int kq = s.k0; kq < s.k1 && ok; kq += 4) {
+            nb32 = fetch_b(s.k0);
+            for (int kq = s.k0; kq < s.k1 && ok; kq += W_AHEAD) {
+                const int at = (kq - s.k0) & 31;
+                if (at == 0) sb32 = nb32, nb32 = fetch_b(kq + 32);
 #pragma unroll
-                for (int j = 0; j < 4; j++) sc[j] = na[j] * nb[j];
-                fetch(kq + 4);
+                for (int j = 0; j < W_AHEAD; j++) sa[j] = na[j];
+                fetch(kq + W_AHEAD);
 #pragma unroll
-                for (int kj = 0; kj < 4; kj++) {
+                for (int kj = 0; kj < W_AHEAD; kj++) {
                     if (kq + kj >= s.k1) break;
+                    const float sc = sa[kj] * __shfl_sync(0xffffffffu, sb32, at + kj);
                     const int buf = i & 1;
                     ok = mbar_wait(&accfull[buf], (i / 2) & 1, g.err, WAIT_LIMIT);
                     i++;
-                    __syncwarp();
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t t = lane_base + buf * WT;
@@ -297,10 +309,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
                     tmem_ld_wait(r[0]);
                     tmem_ld_pin(r[1]);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) acc[j] = fmaf(__uint_as_float(r[0][j]), sc[kj], acc[j]);
+                    for (int j = 0; j < 32; j++) acc[j] = fmaf(__uint_as_float(r[0][j]), sc, acc[j]);
                     tmem_ld32_issue(t + 64, r[0]);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) acc[32 + j] = fmaf(__uint_as_float(r[1][j]), sc[kj], acc[32 + j]);
+                    for (int j = 0; j < 32; j++) acc[32 + j] = fmaf(__uint_as_float(r[1][j]), sc, acc[32 + j]);
                     tmem_ld32_issue(t + 96, r[1]);
                     tmem_ld_wait(r[0]);
                     tmem_ld_pin(r[1]);
@@ -308,9 +320,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
                     __syncwarp();
                     if (lane == 0) arrive_cluster(free_bar[buf]);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) acc[64 + j] = fmaf(__uint_as_float(r[0][j]), sc[kj], acc[64 + j]);
+                    for (int j = 0; j < 32; j++) acc[64 + j] = fmaf(__uint_as_float(r[0][j]), sc, acc[64 + j]);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) acc[96 + j] = fmaf(__uint_as_float(r[1][j]), sc[kj], acc[96 + j]);
+                    for (int j = 0; j < 32; j++) acc[96 + j] = fmaf(__uint_as_float(r[1][j]), sc, acc[96 + j]);
                 }
             }
             if (!ok) break;
@@ -419,7 +431,7 @@ struct WidePlan {
     size_t workspace;
 };
 // Whole tiles in rounds of one per pair; the tiles of a last round that would leave pairs idle are shared along K when that
-// saves more than the parts cost (their traffic and a launch, about 10 us; a block of K takes 0.27 us).
+// saves more than the parts cost (their traffic and a launch, about 10 us; a block of K takes 0.5 us).
 WidePlan plan_wide(int M, int N, int K, int sms)
 {
     WidePlan p{};
@@ -428,7 +440,7 @@ WidePlan plan_wide(int M, int N, int K, int sms)
     p.nkb = (K + QB - 1) / QB;
     p.pairs = sms / 2 > 0 ? sms / 2 : 1;
     const int rest = p.tiles % p.pairs;
-    const bool share = rest && (double)(p.pairs - rest) / p.pairs * p.nkb * 0.27 > 10.0;
+    const bool share = rest && (double)(p.pairs - rest) / p.pairs * p.nkb * 0.5 > 10.0;
     p.whole = share ? p.tiles - rest : p.tiles;
     p.shared_units = (long long)(p.tiles - p.whole) * p.nkb;
     p.sharers = (int)(p.shared_units / 4 < p.pairs ? (p.shared_units + 3) / 4 : p.pairs);  // at least about four blocks each
