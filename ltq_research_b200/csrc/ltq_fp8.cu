@@ -34,17 +34,19 @@ __device__ __forceinline__ void store4(uint8_t* row, int c, int K, uint32_t q)
         for (int i = 0; c + i < K; i++) row[c + i] = (uint8_t)(q >> (8 * i));
 }
 
-// Activations.  A warp takes 1024 columns of ROWS rows, eight columns a lane and load (16 bytes of a 16-bit type), so a block
-// of 128 is half a warp's load and the maximum four exchanges; a row's loads are in flight while the row before it is worked on.  The scales of a
-// CTA's rows are gathered in shared memory and leave as one run of rows per block, the layout the products read.
+// Activations.  A warp takes 1024 columns of ROWS rows, eight columns a lane and load (16 bytes of a 16-bit type), so a block of
+// 128 is half a warp's load and its maximum four exchanges; a row's loads are in flight while the row before it is worked on.  The
+// scales of a CTA's rows are gathered in shared memory and leave as one run of rows per block, the layout the products read.
+// Bound by memory: 8192 x 4096 bf16 (67 MB in, 35 MB out) 18.5 us, 5.2 TB/s; 1003 x 128256 75 us, 5.1 TB/s.  With a division a
+// value and a warp a block it took 51 and 180 us.
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) quant_rows_kernel(const T* __restrict__ x, long long ld, int M, int K,
                                                          uint8_t* __restrict__ q, long long ld_q, float* __restrict__ s,
                                                          long long ld_s, int aligned)
 {
     __shared__ float sc[8][8 * ROWS];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c0 = blockIdx.x * 1024;
-    const int mb = blockIdx.y * (8 * ROWS);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, groups = (K + 1023) / 1024;
+    const int group = blockIdx.x % groups, c0 = group * 1024, mb = blockIdx.x / groups * (8 * ROWS);
     const int m0 = mb + warp * ROWS, m1 = min(M, m0 + ROWS);
     Raw8<T> next[4];
     if (m0 < m1)
@@ -77,7 +79,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) quant_rows_kernel
     }
     __syncthreads();
     for (int i = threadIdx.x; i < 8 * 8 * ROWS; i += 256) {
-        const int b = blockIdx.x * 8 + i / (8 * ROWS), m = mb + i % (8 * ROWS);
+        const int b = group * 8 + i / (8 * ROWS), m = mb + i % (8 * ROWS);
         if (b * QB < K && m < M) s[b * ld_s + m] = sc[i / (8 * ROWS)][i % (8 * ROWS)];
     }
 }
@@ -139,8 +141,9 @@ template <typename T, int ROWS>
 int quant_rows(const void* x, long long ld, int M, int K, uint8_t* q, long long ld_q, float* s, long long ld_s, cudaStream_t st)
 {
     const int aligned = (uintptr_t)x % 16 == 0 && ld * sizeof(T) % 16 == 0;
-    const dim3 grid((K + 1023) / 1024, (M + 8 * ROWS - 1) / (8 * ROWS));
-    quant_rows_kernel<T, ROWS><<<grid, 256, 0, st>>>((const T*)x, ld, M, K, q, ld_q, s, ld_s, aligned);
+    const long long grid = (K + 1023LL) / 1024 * ((M + 8LL * ROWS - 1) / (8 * ROWS));
+    if (grid > 0x7fffffff) return -1;
+    quant_rows_kernel<T, ROWS><<<(unsigned)grid, 256, 0, st>>>((const T*)x, ld, M, K, q, ld_q, s, ld_s, aligned);
     return (int)cudaGetLastError();
 }
 template <typename T>
@@ -161,7 +164,7 @@ extern "C" int ltq_fp8_quant_rows(const void* x, int dtype, long long ld, int M,
     if (!es || M < 0 || K < 1 || ld < K || ld_s < M || ld_q % 16 || ld_q < K) return -1;
     if (M == 0) return 0;
     if (!x || (uintptr_t)x % es || !q || (uintptr_t)q % 16 || !s || (uintptr_t)s % 4) return -1;
-    if (M > 65535 * 8) return -1;
+    if (M > 0x7fffffff - 32 || K > 0x7fffffff - 2048) return -1;
     const cudaStream_t st = (cudaStream_t)stream;
     // one row a warp while that fills the GPU no more than a few times over, else four
     const bool few = (long long)M * ((K + 1023) / 1024) < 8192;
