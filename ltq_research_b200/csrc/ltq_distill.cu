@@ -24,7 +24,7 @@ constexpr int D_THREADS = 256;
 constexpr int D_MAXCL = 8;
 constexpr long long D_ROW = 72 * 1024, D_SLICE = 52 * 1024;  // shared memory for a whole row of one CTA, for a cluster CTA's slice
 constexpr int D_SMEM = 200 * 1024;   // dynamic shared memory of a CTA at most
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr double LOG2E_D = 1.4426950408889634, LN2_D = 0.6931471805599453;
 enum { M_LOSS = 0, M_BOTH = 1, M_GRAD = 2 };
 
 struct DistillParams {
@@ -44,6 +44,7 @@ struct DistillParams {
     long long ld_d;
     int T, V, K, idx64, u_dt;
     float inv_tau;
+    double inv_tau_d;
     int cl;         // CTAs of a row (cluster size)
     int hold;       // vectors of a slice that are held in shared memory (twice: this row's and the next one's)
     int bit_words;  // words of the bitmap, before the held vectors in shared memory
@@ -135,46 +136,54 @@ __device__ __forceinline__ void load_slot(const DistillParams& p, long long row,
     u = id >= 0 ? t : -INFINITY;
 }
 
-// p_k into pr (from u) on one warp; returns P's two parts and sum p log p.  log p is formed from differences, small where p is
-// large: u / tau and the log-sum-exp alone would each be rounded to their own size.
+template <typename F>
+__device__ __forceinline__ F warp_sum(F v)
+{
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// p_k into pr (from u) on one warp; returns P's two parts and sum p log p.  In 64 bits: p_r is what the others leave of 1, and the
+// loss is small beside its terms; K exponentials on one warp while the others read the row cost no time.
 template <bool REST>
 __device__ __forceinline__ void teacher_probabilities(const DistillParams& p, float lse, float* pr, const int* id, int lane,
-                                                      float& psum, float& prest, float& plogp)
+                                                      double& psum, double& prest, double& plogp)
 {
     const int K = p.K;
-    float um = 0.f, lt = 0.f, inv = 0.f;  // without rest: the largest u, log and reciprocal of the sum relative to it
+    double um = 0.0, lt = lse;  // without rest: the largest u / tau, and the log of the sum relative to it
     if (!REST) {
-        um = -INFINITY;
-        for (int k = lane; k < K; k += 32) um = fmaxf(um, pr[k]);
-        um = warp_reduce<0>(um);
-        if (um == -INFINITY) um = 0.f;
-        float t = 0.f;
-        for (int k = lane; k < K; k += 32) t += expf(__fmul_rn(pr[k] - um, p.inv_tau));
-        t = warp_reduce<1>(t);
-        if (t != 0.f) lt = logf(t), inv = 1.f / t;  // else no live slot, or all of them -inf: p = 0
+        float m = -INFINITY;
+        for (int k = lane; k < K; k += 32) m = fmaxf(m, pr[k]);
+        m = warp_reduce<0>(m);
+        um = m == -INFINITY ? 0.0 : __dmul_rn(m, p.inv_tau_d);
+        double t = 0.0;
+        for (int k = lane; k < K; k += 32) t += exp(__fma_rn(pr[k], p.inv_tau_d, -um));
+        t = warp_sum(t);
+        lt = t == 0.0 ? 0.0 : log(t);  // 0: no live slot, or all of them -inf: p = 0
     }
-    float distinct = 0.f;
-    psum = plogp = 0.f;
+    int distinct = 0;
+    psum = plogp = 0.0;
     for (int k = lane; k < K; k += 32) {
-        float pk = 0.f;
+        double pk = 0.0;
         if (id[k] >= 0) {
-            const float d = REST ? __fmaf_rn(pr[k], p.inv_tau, -lse) : __fmul_rn(pr[k] - um, p.inv_tau);
-            const float lp = REST ? d : d - lt;
-            pk = REST ? expf(d) : __fmul_rn(expf(d), inv);
+            const double lp = __fma_rn(pr[k], p.inv_tau_d, -um) - lt;
+            pk = exp(lp);
             psum += pk;
-            if (!(pk == 0.f)) plogp = __fmaf_rn(pk, lp, plogp);
+            if (!(pk == 0.0)) plogp = __fma_rn(pk, lp, plogp);
             if (REST && K >= p.V) {
                 bool first = true;
                 for (int q = 0; q < k && first; q++) first = id[q] != id[k];
-                distinct += first ? 1.f : 0.f;
+                distinct += first;
             }
         }
-        pr[k] = pk;
+        pr[k] = (float)pk;
     }
-    psum = warp_reduce<1>(psum);
-    plogp = warp_reduce<1>(plogp);
-    prest = REST ? fmaxf(1.f - psum, 0.f) : 0.f;
-    if (REST && K >= p.V && warp_reduce<1>(distinct) == (float)p.V) prest = 0.f;  // slots that hold every token leave no rest
+    psum = warp_sum(psum);
+    plogp = warp_sum(plogp);
+    prest = REST ? fmax(1.0 - psum, 0.0) : 0.0;
+    if (REST && psum != psum) prest = psum;  // NaN
+    if (REST && K >= p.V && warp_sum(distinct) == p.V) prest = 0.0;  // slots that hold every token leave no rest
 }
 
 // slot k is the first with its id: of slots with one id the lowest stands for the token
@@ -236,7 +245,8 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
     constexpr int VEC = 16 / sizeof(T), WARPS = D_THREADS / 32, ALL = D_THREADS + 32;
     extern __shared__ __align__(16) uint32_t dsm[];  // bitmap, held slice, slots
     __shared__ float red[2][WARPS];
-    __shared__ float slot_sums[5];  // sum p, p_r, sum p log p, the pair of the slots' tokens in the slice
+    __shared__ float slot_sums[4];    // sum p, p_r, the pair of the slots' tokens in the slice
+    __shared__ double slot_logs[2];   // sum p log p, p_r
     __shared__ float xch[4][D_MAXCL];
     __shared__ int dup;
     uint32_t* bits = dsm;
@@ -281,7 +291,7 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
     for (int i = tid; i < ((nvec + 2) * VEC + 31) / 32; i += ALL) bits[i] = 0;
     if (tid == 0) dup = 0;
     __syncthreads();
-    const float c = p.inv_tau * LOG2E;
+    const float c = (float)(p.inv_tau_d * LOG2E_D);
     for (int k = tid; k < K; k += ALL) {
         if (k != tid) load_slot(p, row, k, id0, u0);
         const bool own = id0 >= 0 && id0 >= sl.j0 && id0 < sl.j1;
@@ -308,18 +318,16 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
     const int nth = tid < D_THREADS ? max(0, (nh - tid + D_THREADS - 1) / D_THREADS) : 0;
 
     if (warp < WARPS) {
-        // one pass: (m, s) with the running maximum, over the tokens outside the slots (REST) or all
+        // One pass: (m, s) with the running maximum, over the tokens outside the slots.  The slots' tokens, which hold most of
+        // the mass, are summed apart and in 64 bits.
         float m = -INFINITY, s;
         uint64_t s2 = 0;  // two sums, by the elements' parity
         // the bits of this thread's vectors: at a fixed step (and, of four-element vectors, a fixed half of a byte)
         const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bits) + (VEC == 8 ? tid + 1 : (tid + 1) >> 1);
         constexpr int step = VEC == 8 ? D_THREADS : D_THREADS / 2;
         auto masked = [&](uint4 raw, int t) {  // the slots' tokens as -infinity
-            if (REST) {
-                const uint32_t by = bytes[t * step], mb = VEC == 8 ? by : by >> (((tid + 1) & 1) * 4) & 15u;
-                if (mb) raw = mask16(raw, mb, T());
-            }
-            return raw;
+            const uint32_t by = bytes[t * step], mb = VEC == 8 ? by : by >> (((tid + 1) & 1) * 4) & 15u;
+            return mb ? mask16(raw, mb, T()) : raw;
         };
         auto raise = [&](float vm) {  // the running maximum
             if (vm > m) {
@@ -370,11 +378,12 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
 #pragma unroll
             for (int q = 0; q < 4; q += 2) add_both(u[q], u[q + 1], t + q);
         }
+        for (; t + 2 <= nt; t += 2) add_both(__ldg(zt + t * D_THREADS), __ldg(zt + (t + 1) * D_THREADS), t);  // the same pairs as above
         for (; t < nt; t++) add(__ldg(zt + t * D_THREADS), t);
         const float2 e = unpair(s2);
         s = e.x + e.y;
         auto scalar = [&](int j) {
-            if (REST && (bits[(j - jb) >> 5] >> ((j - jb) & 31) & 1u)) return;
+            if (bits[(j - jb) >> 5] >> ((j - jb) & 31) & 1u) return;
             const float z = to_f(sl.z[j]), M = fmaxf(m, __fmul_rn(z, c)), b = M == -INFINITY ? 0.f : M;
             s = __fmaf_rn(s, ex2(m - b), ex2(__fmaf_rn(z, c, -b)));
             m = M;
@@ -384,22 +393,24 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
         warp_join<32>(m, s);
         if (lane == 0) red[0][warp] = m, red[1][warp] = s;
     } else {  // the slots' sums
-        float psum, prest, plogp, mt = -INFINITY, st = 0.f;
+        double psum, prest, plogp, t = 0.0;
         teacher_probabilities<REST>(p, REST ? p.lse[row] : 0.f, pr, id, lane, psum, prest, plogp);
-        if (REST) {
-            auto counts = [&](int k) { return id[k] >= 0 && id[k] >= sl.j0 && id[k] < sl.j1 && (!any_dup || leads(id, k)); };
-            for (int k = lane; k < K; k += 32)
-                if (counts(k)) mt = fmaxf(mt, __fmul_rn(zk[k], c));
-            mt = warp_reduce<0>(mt);
-            for (int k = lane; k < K; k += 32)
-                if (counts(k)) st += ex2(__fmaf_rn(zk[k], c, mt == -INFINITY ? 0.f : -mt));
-            st = warp_reduce<1>(st);
+        float mt = -INFINITY;
+        auto counts = [&](int k) { return id[k] >= 0 && id[k] >= sl.j0 && id[k] < sl.j1 && (!any_dup || leads(id, k)); };
+        for (int k = lane; k < K; k += 32)
+            if (counts(k)) mt = fmaxf(mt, __fmul_rn(zk[k], c));
+        mt = warp_reduce<0>(mt);
+        for (int k = lane; k < K; k += 32)
+            if (counts(k)) t += exp2(__fma_rn(zk[k], c, mt == -INFINITY ? 0.0 : -(double)mt));
+        t = warp_sum(t);
+        if (lane == 0) {
+            slot_sums[0] = (float)psum, slot_sums[1] = (float)prest, slot_sums[2] = mt, slot_sums[3] = (float)t;
+            slot_logs[0] = plogp, slot_logs[1] = prest;
         }
-        if (lane == 0) slot_sums[0] = psum, slot_sums[1] = prest, slot_sums[2] = plogp, slot_sums[3] = mt, slot_sums[4] = st;
     }
     __syncthreads();
     const float psum = slot_sums[0], prest = slot_sums[1];
-    float m = red[0][lane & (WARPS - 1)], s = red[1][lane & (WARPS - 1)], mt = slot_sums[3], st = slot_sums[4];
+    float m = red[0][lane & (WARPS - 1)], s = red[1][lane & (WARPS - 1)], mt = slot_sums[2], st = slot_sums[3];
     warp_join<WARPS>(m, s);
     if (cl > 1) {
         cluster_wait();
@@ -415,24 +426,23 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
         const int q = lane & (D_MAXCL - 1);
         m = q < cl ? xch[0][q] : -INFINITY, s = q < cl ? xch[1][q] : 0.f;
         warp_join<D_MAXCL>(m, s);
-        if (REST) {
-            mt = q < cl ? xch[2][q] : -INFINITY, st = q < cl ? xch[3][q] : 0.f;
-            warp_join<D_MAXCL>(mt, st);
-        }
+        mt = q < cl ? xch[2][q] : -INFINITY, st = q < cl ? xch[3][q] : 0.f;
+        warp_join<D_MAXCL>(mt, st);
     }
     float ma = m, sa = s;
-    if (REST) join(ma, sa, mt, st);
+    join(ma, sa, mt, st);
     // S = sa 2^ma: the two stay apart, for log2 S itself would be rounded to the size of the logits
     const float ls = log2f(sa), base = ma == -INFINITY ? 0.f : ma;
     const float log2qr = !REST || s == 0.f ? -INFINITY : (m - base) + (log2f(s) - ls);
     if (rank == 0 && warp == WARPS) {
-        float l = 0.f;
+        double l = 0.0;
+        const double shift = ma == -INFINITY ? 0.0 : (double)base + log2((double)sa);
         for (int k = lane; k < K; k += 32)
-            if (!(pr[k] == 0.f)) l = __fmaf_rn(-pr[k], __fmul_rn(__fmaf_rn(zk[k], c, -base) - (ma == -INFINITY ? 0.f : ls), LN2), l);
-        l = warp_reduce<1>(l) + slot_sums[2];
+            if (!(pr[k] == 0.f)) l = __fma_rn(-(double)pr[k], __dmul_rn(__fma_rn(zk[k], c, -shift), LN2_D), l);
+        l = warp_sum(l) + slot_logs[0];
         if (lane == 0) {
-            if (prest > 0.f) l = __fmaf_rn(prest, __fmaf_rn(-log2qr, LN2, logf(prest)), l);
-            p.loss[row] = __fmul_rn(w, l);
+            if (slot_logs[1] > 0.0) l = __fma_rn(slot_logs[1], __fma_rn(-(double)log2qr, LN2_D, log(slot_logs[1])), l);
+            p.loss[row] = (float)__dmul_rn(w, l);
             if (p.stats) p.stats[3 * row] = ma, p.stats[3 * row + 1] = sa, p.stats[3 * row + 2] = log2qr;
         }
     }
@@ -481,7 +491,7 @@ __global__ void __launch_bounds__(D_THREADS) distill_grad_kernel(const DistillPa
         zero_slice(p, sl, dz, 0, tid, D_THREADS);
         return;
     }
-    const float c = p.inv_tau * LOG2E;
+    const float c = (float)(p.inv_tau_d * LOG2E_D);
     float* zk = reinterpret_cast<float*>(id + K);
     for (int k = tid; k < K; k += D_THREADS) {
         load_slot(p, row, k, id[k], pr[k]);
@@ -489,9 +499,9 @@ __global__ void __launch_bounds__(D_THREADS) distill_grad_kernel(const DistillPa
     }
     __syncthreads();
     if (tid < 32) {
-        float psum, prest, plogp;
+        double psum, prest, plogp;
         teacher_probabilities<REST>(p, REST ? p.lse[row] : 0.f, pr, id, lane, psum, prest, plogp);
-        if (lane == 0) sums[0] = psum, sums[1] = prest;
+        if (lane == 0) sums[0] = (float)psum, sums[1] = (float)prest;
     }
     __syncthreads();
     const float up = p.grad ? p.grad[row * p.s_grad] : 1.f;
@@ -608,7 +618,7 @@ extern "C" int ltq_distill_topk(const void* logits, int dtype, long long ld, con
     DistillParams p{};
     p.z = logits, p.ld = ld, p.idx = idx, p.ld_idx = ld_idx, p.u = teacher, p.ld_u = ld_t, p.lse = teacher_lse;
     p.weight = weight, p.grad = grad, p.s_grad = grad_stride, p.loss = loss, p.stats = stats, p.dz = dlogits, p.ld_d = ld_d;
-    p.T = T, p.V = V, p.K = K, p.idx64 = idx64 != 0, p.u_dt = teacher_dtype, p.inv_tau = 1.f / temperature;
+    p.T = T, p.V = V, p.K = K, p.idx64 = idx64 != 0, p.u_dt = teacher_dtype, p.inv_tau = 1.f / temperature, p.inv_tau_d = 1.0 / temperature;
     p.vec_out = mode != M_LOSS && ((uintptr_t)logits & 15) == ((uintptr_t)dlogits & 15) && ((ld - ld_d) * es) % 16 == 0;
     const cudaStream_t st = (cudaStream_t)stream;
     if (dtype == DT_F32) return dispatch<float>(p, mode, st);
