@@ -11,6 +11,10 @@
 // list is cut into chunks of equal length; a warp sums one chunk's rows over 32 vectors of the width and writes the rows
 // whose positions all lie in the chunk, and the sums of the rows that reach over its ends to a workspace.  (3) Those
 // sums are joined from the row's first chunk to its last.  Nothing depends on the order in which CTAs run.
+//
+// Both directions are bound by memory.  Lookup of 16384 rows of 2560 bf16: 27 us, 6.2 TB/s.  Gradient of 16384 positions (bf16)
+// into 128256 x 2048 fp32, 1.1 GB of it written: 173 us sort and zeros (6.1 TB/s; the sort alone takes 25 and hides), 31 us sums
+// (67 MB read, 65 MB written, rows in random order), 10 us joins.
 #include "ltq_b200.h"
 #include "stride_grid.cuh"
 #include "vec_types.cuh"
@@ -239,8 +243,7 @@ __device__ void fill_rows(const SortParams& p, uint32_t* bits, int f, const uint
 }
 
 // Few positions: a position's place in the sorted list is the number of smaller keys and of equal keys before it, counted by a
-// warp over all keys in shared memory.  At 4099 positions and 50003 rows this takes 2 us of a launch where the digit passes'
-// barriers would take 17.
+// warp over all keys in shared memory.  4099 positions: 9 us, where the digit passes of one cluster take 21.
 constexpr int RANK_MAX = 8192;
 __global__ void __launch_bounds__(S_THREADS, 2) rank_fill_kernel(const SortParams p)
 {
