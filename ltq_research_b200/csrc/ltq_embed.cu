@@ -5,16 +5,18 @@
 //
 // A token outside [0, V) reads as a row of zeros and takes no gradient; neither does the padding token.
 //
-// The gradient runs in three launches.  (1) The positions are sorted by token (stable) and zeros written to the table rows
-// that no token names.  Up to 8192 positions every CTA counts the ranks of a few positions and then writes its zeros; beyond,
-// one cluster of 8 CTAs sorts (least digit first, 10 bits a pass) while the other CTAs write the zeros.  (2) The sorted
-// list is cut into chunks of equal length; a warp sums one chunk's rows over 32 vectors of the width and writes the rows
-// whose positions all lie in the chunk, and the sums of the rows that reach over its ends to a workspace.  (3) Those
-// sums are joined from the row's first chunk to its last.  Nothing depends on the order in which CTAs run.
+// The gradient runs in three launches.  (1) The positions are sorted by token (stable) and zeros written to some of the table
+// rows that no token names.  Up to 8192 positions every CTA counts the ranks of a few positions; beyond, one cluster of 8 CTAs
+// sorts (least digit first, 10 bits a pass) while the other CTAs write the zeros.  (2) The sorted list is cut into chunks of
+// equal length; a warp sums one chunk's rows over 32 vectors of the width and writes the rows whose positions all lie in the
+// chunk, and the sums of the rows that reach over its ends to a workspace; the last CTAs write the zeros that are left.
+// (3) The sums are joined from the row's first chunk to its last.  Nothing depends on the order in which CTAs run.
 //
 // Both directions are bound by memory.  Lookup of 16384 rows of 2560 bf16: 27 us, 6.2 TB/s.  Gradient of 16384 positions (bf16)
-// into 128256 x 2048 fp32, 1.1 GB of it written: 173 us sort and zeros (6.1 TB/s; the sort alone takes 25 and hides), 31 us sums
-// (67 MB read, 65 MB written, rows in random order), 10 us joins.
+// into 128256 x 2048 fp32, 1.1 GB of it written: 193 us, 5.8 TB/s; 33 us sort and the zeros beside it, 143 us sums and the other
+// zeros, 10 us joins.
+#include <algorithm>
+
 #include "ltq_b200.h"
 #include "stride_grid.cuh"
 #include "vec_types.cuh"
@@ -80,6 +82,23 @@ constexpr int KEPT = 4;  // groups of 32 positions that a warp keeps in register
 static_assert(BINS == 2 * S_THREADS, "two bins a thread");
 static_assert(FILL_ROWS / 32 <= S_WARPS * BINS, "the fill's bitmap fits the histograms' memory");
 
+// Zeros to the rows that no token names, in equal shares: the first `early` rows of each share beside the sort, the others beside
+// the sums, so that neither leaves the memory idle.
+struct Fill {
+    uint8_t* out;
+    long long ld_bytes, row_bytes;
+    int V, shares, parts;  // CTAs of a share's later rows
+    long long early;
+    int* start;  // [shares]: sorted keys below the share's later rows; NULL without positions, when no row is late
+    __device__ void share(int f, long long& b0, long long& b1, long long& e) const
+    {
+        const long long per = (V + shares - 1) / shares;
+        b0 = f * per < V ? f * per : V;
+        b1 = b0 + per < V ? b0 + per : V;
+        e = b0 + early < b1 ? b0 + early : b1;
+    }
+};
+
 struct SortParams {
     const void* tok;
     int t64;
@@ -87,10 +106,7 @@ struct SortParams {
     long long pad;  // padding token, or -1
     uint32_t* key[2];
     uint32_t* pos[2];  // pass p reads buffer 1 - (p & 1) (the first: the tokens) and writes buffer p & 1
-    // fill
-    uint8_t* out;
-    long long ld_bytes, row_bytes;
-    int fill_ctas;
+    Fill fill;
 };
 
 // buffer of the sorted list
@@ -213,31 +229,77 @@ __device__ void zero_row(uint8_t* row, long long bytes, int lane)
     }
 }
 
-// zeros to this CTA's share of the rows that no token names; keys: all sort keys in shared memory, or NULL to read the tokens
-__device__ void fill_rows(const SortParams& p, uint32_t* bits, int f, const uint32_t* keys)
+// zeros to rows r0 .. r0 + nr - 1 whose bit is not set, a warp a row
+__device__ void zero_rows(const Fill& p, const uint32_t* bits, long long r0, int nr, int warp, int warps, int lane)
 {
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const long long per = (p.V + p.fill_ctas - 1) / p.fill_ctas;
-    const long long b0 = f * per, b1 = b0 + per < p.V ? b0 + per : p.V;
     const int width = !((uintptr_t)p.out % 16 || p.ld_bytes % 16 || p.row_bytes % 16)  ? 16
                       : !((uintptr_t)p.out % 4 || p.ld_bytes % 4 || p.row_bytes % 4) ? 4
                                                                                      : 2;
-    for (long long r0 = b0; r0 < b1; r0 += FILL_ROWS) {
-        const int nr = (int)(b1 - r0 < FILL_ROWS ? b1 - r0 : FILL_ROWS);
+    for (int r = warp; r < nr; r += warps) {
+        if (bits[r >> 5] >> (r & 31) & 1u) continue;
+        uint8_t* row = p.out + (r0 + r) * p.ld_bytes;
+        if (width == 16) zero_row<16>(row, p.row_bytes, lane);
+        else if (width == 4) zero_row<4>(row, p.row_bytes, lane);
+        else zero_row<2>(row, p.row_bytes, lane);
+    }
+}
+
+// The early rows of share f, and where its later rows' keys will begin; keys: all sort keys in shared memory, or NULL to read the
+// tokens.
+__device__ void fill_early(const SortParams& p, uint32_t* bits, int f, const uint32_t* keys)
+{
+    __shared__ int below;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    long long b0, b1, e;
+    p.fill.share(f, b0, b1, e);
+    if (tid == 0) below = 0;
+    long long r0 = b0;
+    do {  // once at least, for the count
+        const int nr = (int)(e - r0 < FILL_ROWS ? e - r0 : FILL_ROWS);
         for (int i = tid; i < (nr + 31) / 32; i += S_THREADS) bits[i] = 0;
         __syncthreads();
+        int c = 0;
         for (int i = tid; i < p.n; i += S_THREADS) {
             const long long t = keys ? (long long)keys[i] : (long long)sort_key(p, i);
+            c += t < e;
             if (t >= r0 && t < r0 + nr) atomicOr(&bits[(t - r0) >> 5], 1u << ((t - r0) & 31));
         }
-        __syncthreads();
-        for (int r = warp; r < nr; r += S_WARPS) {
-            if (bits[r >> 5] >> (r & 31) & 1u) continue;
-            uint8_t* row = p.out + (r0 + r) * p.ld_bytes;
-            if (width == 16) zero_row<16>(row, p.row_bytes, lane);
-            else if (width == 4) zero_row<4>(row, p.row_bytes, lane);
-            else zero_row<2>(row, p.row_bytes, lane);
+        if (r0 == b0) {
+            c = __reduce_add_sync(0xffffffffu, c);
+            if (lane == 0) atomicAdd(&below, c);
         }
+        __syncthreads();
+        zero_rows(p.fill, bits, r0, nr, warp, S_WARPS, lane);
+        __syncthreads();
+        r0 += FILL_ROWS;
+    } while (r0 < e);
+    if (tid == 0 && p.fill.start) p.fill.start[f] = below;
+}
+
+// A part of share f's later rows, by a CTA of 128 threads; the sorted keys are there now.
+constexpr int LATE_BYTES = 49152, LATE_ROWS = 4096;
+__device__ void fill_late(const Fill& p, const uint32_t* key, int n, int f, int part)
+{
+    __shared__ uint32_t bits[LATE_ROWS / 32];
+    const int tid = threadIdx.y * 32 + threadIdx.x;
+    long long b0, b1, e;
+    p.share(f, b0, b1, e);
+    const long long step = (b1 - e + p.parts - 1) / p.parts, p0 = e + part * step, p1 = p0 + step < b1 ? p0 + step : b1;
+    for (long long r0 = p0; r0 < p1; r0 += LATE_ROWS) {
+        const int nr = (int)(p1 - r0 < LATE_ROWS ? p1 - r0 : LATE_ROWS);
+        for (int i = tid; i < LATE_ROWS / 32; i += 128) bits[i] = 0;
+        __syncthreads();
+        for (int i = p.start[f] + tid; i < n; i += 128 * 8) {
+            uint32_t k[8];
+#pragma unroll
+            for (int q = 0; q < 8; q++) k[q] = i + 128 * q < n ? key[i + 128 * q] : 0xffffffffu;
+#pragma unroll
+            for (int q = 0; q < 8; q++)
+                if (k[q] >= r0 && k[q] < r0 + nr) atomicOr(&bits[(k[q] - r0) >> 5], 1u << ((k[q] - r0) & 31));
+            if (k[7] >= r0 + nr) break;
+        }
+        __syncthreads();
+        zero_rows(p, bits, r0, nr, tid >> 5, 4, tid & 31);
         __syncthreads();
     }
 }
@@ -264,9 +326,9 @@ __global__ void __launch_bounds__(S_THREADS, 2) rank_fill_kernel(const SortParam
         below = __reduce_add_sync(0xffffffffu, below);
         if (lane == 0) p.key[0][below] = k, p.pos[0][below] = i;
     }
-    if (p.fill_ctas) {
+    if (p.fill.shares) {
         __syncthreads();
-        fill_rows(p, bits, blockIdx.x, key);
+        fill_early(p, bits, blockIdx.x, key);
     }
 }
 
@@ -275,7 +337,7 @@ __global__ void __cluster_dims__(S_CL, 1, 1) __launch_bounds__(S_THREADS, 2) sor
     extern __shared__ uint32_t sm[];
     const int cluster = blockIdx.x / S_CL;
     if (cluster == 0) sort_cluster(p, sm);
-    else fill_rows(p, sm, blockIdx.x - S_CL, nullptr);
+    else fill_early(p, sm, blockIdx.x - S_CL, nullptr);
 }
 
 struct SumParams {
@@ -288,6 +350,8 @@ struct SumParams {
     float* part;  // [chunk][2][D]: the sum of a row begun in an earlier chunk; of one that a later chunk goes on with
     int n, V, D, chunk, nchunks, accumulate;
     float scale;
+    int sum_ctas, slices;
+    Fill fill;
 };
 
 template <typename TO, int VEC>
@@ -321,7 +385,12 @@ __device__ __forceinline__ void store_part(float* part, const float (&a)[VEC])
 template <typename TI, typename TO, int VEC, bool ACC>
 __global__ void __launch_bounds__(128) sum_chunks_kernel(const SumParams p)
 {
-    const int lane = threadIdx.x, ch = blockIdx.x * 4 + threadIdx.y, v = blockIdx.y * 32 + lane, nv = p.D / VEC;
+    if (!ACC && blockIdx.x >= p.sum_ctas) {
+        const int f = blockIdx.x - p.sum_ctas;
+        fill_late(p.fill, p.key, p.n, f / p.fill.parts, f % p.fill.parts);
+        return;
+    }
+    const int lane = threadIdx.x, ch = blockIdx.x / p.slices * 4 + threadIdx.y, v = blockIdx.x % p.slices * 32 + lane, nv = p.D / VEC;
     if (ch >= p.nchunks) return;
     const int c0 = ch * p.chunk, c1 = min(p.n, c0 + p.chunk);
     // keys and positions of up to 32 places, a lane each, and the keys beside the chunk: one round of loads
@@ -485,12 +554,20 @@ int chunk_of(long long n, int D)
     return n <= 8LL * target ? 8 : (int)(((n + target - 1) / target + 3) / 4 * 4);
 }
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
+size_t part_bytes(long long n, int D)
+{
+    const int c = chunk_of(n, D);
+    return align256(8 * (size_t)((n + c - 1) / c) * D);
+}
+constexpr int MAX_SHARES = 512;
 
 template <typename TI, typename TO, int VEC, bool ACC>
-int sum_launch(const SumParams& p, cudaStream_t st)
+int sum_launch(SumParams p, cudaStream_t st)
 {
     const unsigned slices = (p.D / VEC + 31) / 32;
-    sum_chunks_kernel<TI, TO, VEC, ACC><<<dim3((p.nchunks + 3) / 4, slices), dim3(32, 4), 0, st>>>(p);
+    p.slices = (int)slices;
+    p.sum_ctas = (p.nchunks + 3) / 4 * p.slices;
+    sum_chunks_kernel<TI, TO, VEC, ACC><<<p.sum_ctas + p.fill.shares * p.fill.parts, dim3(32, 4), 0, st>>>(p);
     if (p.nchunks > 1) join_chunks_kernel<TO, VEC, ACC><<<dim3((p.nchunks + 30) / 32, slices), dim3(32, 8), 0, st>>>(p);
     return (int)cudaGetLastError();
 }
@@ -541,8 +618,7 @@ extern "C" int ltq_embed_lookup(const void* table, int dtype, long long ld, cons
 extern "C" size_t ltq_embed_grad_workspace_bytes(long long n, int D)
 {
     if (n <= 0 || n > N_MAX || D < 1 || D > D_MAX) return 0;
-    const int c = chunk_of(n, D);
-    return 4 * align256(4 * (size_t)n) + align256(8 * (size_t)((n + c - 1) / c) * D);
+    return 4 * align256(4 * (size_t)n) + part_bytes(n, D) + 4 * MAX_SHARES;
 }
 
 extern "C" int ltq_embed_grad(const void* tokens, int tok64, long long n, int V, long long padding, const void* dout,
@@ -562,9 +638,8 @@ extern "C" int ltq_embed_grad(const void* tokens, int tok64, long long n, int V,
     s.passes = 1;
     while (s.passes * DIGIT < 31 && ((unsigned)V >> (s.passes * DIGIT))) s.passes++;
     uint8_t* ws = (uint8_t*)workspace;
-    const size_t a = align256(4 * (size_t)n);
+    const size_t a = align256(4 * (size_t)n), parts = n > 0 ? part_bytes(n, D) : 0;
     for (int i = 0; i < 2; i++) s.key[i] = (uint32_t*)(ws + 2 * i * a), s.pos[i] = (uint32_t*)(ws + (2 * i + 1) * a);
-    s.out = (uint8_t*)out, s.ld_bytes = ld_out * eo, s.row_bytes = (long long)D * eo;
     static std::atomic<int> clusters[64], sms[64];  // clusters of the sort kernel that a device holds at once
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
@@ -582,22 +657,33 @@ extern "C" int ltq_embed_grad(const void* tokens, int tok64, long long n, int V,
         if (nc < 2) nc = 2;
         clusters[dev].store(nc, std::memory_order_release);
     }
-    if (n <= RANK_MAX) {
+    const bool rank = n <= RANK_MAX;
+    const int m = sms[dev].load(std::memory_order_relaxed);
+    Fill& fl = s.fill;
+    fl.out = (uint8_t*)out, fl.ld_bytes = ld_out * eo, fl.row_bytes = (long long)D * eo, fl.V = V;
+    fl.shares = accumulate ? 0 : rank ? 2 * m : (nc - 1) * S_CL;
+    if (fl.shares > MAX_SHARES) fl.shares = MAX_SHARES;
+    fl.start = n > 0 ? (int*)(ws + 4 * a + parts) : nullptr;
+    // Early: what can be written while the digits are sorted, 15 us and 0.5 us a thousand positions, at 6 TB/s.  Beside ranks nothing,
+    // those are counted by all CTAs first; without positions everything, there are no sums to hide the rest behind.  Late: about 48 KB
+    // a CTA.  To 128256 x 4096 bf16: 220 us from 16384 positions, 253 with all rows early; 177 and 204 from 4096.
+    const double early = (15.0 + n / 2000.0) * 6e6 / (double)fl.row_bytes;
+    fl.early = n == 0 ? V : rank || !fl.shares ? 0 : (long long)(early / fl.shares) + 1;
+    const long long late = fl.shares ? (V + (long long)fl.shares - 1) / fl.shares - fl.early : 0;
+    fl.parts = late > 0 ? (int)std::min(((double)late * fl.row_bytes + LATE_BYTES - 1) / LATE_BYTES, 1024.0) : 0;
+    if (rank) {
         s.passes = 1;
-        const int all = 2 * sms[dev].load(std::memory_order_relaxed), need = (int)((n + S_WARPS - 1) / S_WARPS);
-        s.fill_ctas = accumulate ? 0 : all;
-        rank_fill_kernel<<<accumulate && need < all ? need : all, S_THREADS, 0, st>>>(s);
-    } else {
-        s.fill_ctas = accumulate ? 0 : (nc - 1) * S_CL;
-        sort_fill_kernel<<<S_CL + s.fill_ctas, S_THREADS, SORT_SMEM, st>>>(s);
-    }
+        const int need = (int)((n + S_WARPS - 1) / S_WARPS);
+        rank_fill_kernel<<<accumulate ? (need < 2 * m ? need : 2 * m) : fl.shares, S_THREADS, 0, st>>>(s);
+    } else
+        sort_fill_kernel<<<S_CL + fl.shares, S_THREADS, SORT_SMEM, st>>>(s);
     e = cudaGetLastError();
     if (e != cudaSuccess || n == 0) return (int)e;
     SumParams p{};
     const int b = sorted_buffer(s.passes);
     p.key = s.key[b], p.pos = s.pos[b], p.d = dout, p.ld_d = ld_d, p.out = out, p.ld_out = ld_out;
     p.part = (float*)(ws + 4 * a);
-    p.n = (int)n, p.V = V, p.D = D, p.chunk = chunk_of(n, D), p.accumulate = accumulate != 0, p.scale = scale;
+    p.n = (int)n, p.V = V, p.D = D, p.chunk = chunk_of(n, D), p.accumulate = accumulate != 0, p.scale = scale, p.fill = s.fill;
     p.nchunks = (int)((n + p.chunk - 1) / p.chunk);
     if (dtype == DT_F32) return sum_type<float>(p, out_dtype, st);
     if (dtype == DT_BF16) return sum_type<__nv_bfloat16>(p, out_dtype, st);

@@ -123,6 +123,29 @@ def test_grad_million_rows_of_tokens():
     check_grad(tok, torch.randn(300001, 16, device="cuda", generator=g), 1 << 21)
 
 
+@pytest.mark.parametrize("n", [1, 300, 9001])
+@pytest.mark.parametrize("D", [1032, 1031])
+def test_grad_zeros_of_a_large_table(n, D):
+    """Rows that no token names, more than are written beside the sort; some tokens in runs of neighbours, some at the ends."""
+    g = gen(n + D)
+    V = 70001
+    tok = (torch.rand(n, device="cuda", generator=g) ** 4 * V).long()
+    tok[n // 2:] = V - 1 - tok[n // 2:] // 64
+    dout = torch.randn(n, D, device="cuda", generator=g)
+    out = torch.full((V, D + 9), float("nan"), device="cuda")
+    got = embedding.lookup_grad(tok, dout, V, out=out[:, :D])
+    check_grad(tok, dout, V, got=got)
+    assert not got[torch.bincount(tok, minlength=V) == 0].any()
+    assert out[:, D:].isnan().all()
+
+
+def test_grad_without_positions():
+    for V, D in ((1, 1), (70001, 40)):
+        out = torch.ones(V, D, device="cuda")
+        embedding.lookup_grad(torch.empty(0, dtype=torch.int64, device="cuda"), torch.empty(0, D, device="cuda"), V, out=out)
+        assert not out.any()
+
+
 def test_grad_order_is_that_of_the_positions():
     """Equal tokens are summed in the order of their positions: a sum whose value depends on it."""
     tok = torch.zeros(8, dtype=torch.int64, device="cuda")
