@@ -18,20 +18,20 @@ __device__ __forceinline__ float block_scale(uint32_t amax_bits)  // the largest
 // eight values under one scale s (r: its reciprocal, rounded correctly), as eight bytes.  The quotients x / s are rounded correctly
 // without a division each: q = x r and then q + (x - q s) r is the correctly rounded quotient (Markstein's correction, IBM J.
 // Res. Dev. 34, 1990) while the remainder stays above the smallest normal number, which 2^-80 <= s guarantees for every quotient
-// that e4m3 does not round to 0
+// that e4m3 does not round to 0; below, x and s are taken 2^64 times as large, which is exact
 __device__ __forceinline__ uint2 quant8(float (&v)[8], float s, float r)
 {
     if (!(s >= 0x1p-80f)) {  // a tiny scale, or NaN
+        s *= 0x1p64f, r *= 0x1p-64f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = __fdiv_rn(v[i], s);
-    } else {
-        const uint64_t rr = pair(r, r), ns = pair(-s, -s);
+        for (int i = 0; i < 8; i++) v[i] *= 0x1p64f;
+    }
+    const uint64_t rr = pair(r, r), ns = pair(-s, -s);
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            const uint64_t x = pair(v[i], v[i + 1]), q = mul2(x, rr);
-            const float2 y = unpair(fma2(fma2(q, ns, x), rr, q));
-            v[i] = y.x, v[i + 1] = y.y;
-        }
+    for (int i = 0; i < 8; i += 2) {
+        const uint64_t x = pair(v[i], v[i + 1]), q = mul2(x, rr);
+        const float2 y = unpair(fma2(fma2(q, ns, x), rr, q));
+        v[i] = y.x, v[i + 1] = y.y;
     }
     uint32_t w[4];
 #pragma unroll
@@ -94,11 +94,20 @@ __device__ __forceinline__ uint32_t half_warp_max(uint32_t a)
     for (int o = 8; o; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
     return a;
 }
-// The scales and reciprocals of four pairs of blocks (a half warp each), given their largest magnitudes: each lane divides for one
-// of the four, the others take it from there.
-__device__ __forceinline__ void scales4(const uint32_t (&a)[4], int lane, float (&s)[4], float (&r)[4])
+// The scales and reciprocals of four pairs of blocks, a half warp's load each.  The maxima are exchanged so that a lane ends with that
+// of one of the four and divides for it alone; the others take the results from there.
+template <typename T>
+__device__ __forceinline__ void scales4(const Raw8<T> (&x)[4], int lane, float (&s)[4], float (&r)[4])
 {
-    const uint32_t mine = lane & 2 ? (lane & 1 ? a[3] : a[2]) : (lane & 1 ? a[1] : a[0]);
+    uint32_t a[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) a[j] = amax8(x[j]);
+    const bool b0 = lane & 1, b1 = lane & 2;
+    const uint32_t k0 = max(b0 ? a[1] : a[0], __shfl_xor_sync(0xffffffffu, b0 ? a[0] : a[1], 1));
+    const uint32_t k1 = max(b0 ? a[3] : a[2], __shfl_xor_sync(0xffffffffu, b0 ? a[2] : a[3], 1));
+    uint32_t mine = max(b1 ? k1 : k0, __shfl_xor_sync(0xffffffffu, b1 ? k0 : k1, 2));
+    mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 4));
+    mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 8));
     const float sc = block_scale(mine), rc = __frcp_rn(sc);
 #pragma unroll
     for (int j = 0; j < 4; j++) {

@@ -46,7 +46,7 @@ struct DistillParams {
     float inv_tau;
     double inv_tau_d;
     int cl;         // CTAs of a row (cluster size)
-    int hold;       // vectors of a slice that are held in shared memory (twice: this row's and the next one's)
+    int hold;       // vectors of a slice that are held in shared memory
     int bit_words;  // words of the bitmap, before the held vectors in shared memory
     int vec_out;    // dz rows have the alignment of z rows
 };
@@ -237,8 +237,9 @@ __device__ __forceinline__ void zero_slice(const DistillParams& p, const Slice<T
 // between the two passes, so that the row is read from memory once.  Several small CTAs an SM, not one large one: a row has
 // latencies in a chain (its weight, its slots, the sums, the cluster's barrier) and only other rows can fill them.  The last warp
 // works on the slots alone, while the others are in their first pass.
-// Bound: the logits read once and the gradient written once; two exponentials an element (16 a clock and SM) take about half
-// of that time.
+// Bound: the logits read once and the gradient written once; an exponential an element and pass (16 a clock and SM) and the
+// instructions around it take 60 to 70 % of that time.  4096 x 128256 bf16 with the gradient: 384 us, 5.5 TB/s; 2048 rows, the loss
+// alone: 96 us, 5.5 TB/s.
 template <typename T, bool GRAD, bool REST>
 __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const DistillParams p)
 {

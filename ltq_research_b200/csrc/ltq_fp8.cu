@@ -35,10 +35,10 @@ __device__ __forceinline__ void store4(uint8_t* row, int c, int K, uint32_t q)
 }
 
 // Activations.  A warp takes 1024 columns of ROWS rows, eight columns a lane and load (16 bytes of a 16-bit type), so a block of
-// 128 is half a warp's load and its maximum four exchanges; a row's loads are in flight while the row before it is worked on.  The
-// scales of a CTA's rows are gathered in shared memory and leave as one run of rows per block, the layout the products read.
-// Bound by memory: 8192 x 4096 bf16 (67 MB in, 35 MB out) 18.5 us, 5.2 TB/s; 1003 x 128256 75 us, 5.1 TB/s.  With a division a
-// value and a warp a block it took 51 and 180 us.
+// 128 is half a warp's load; four blocks' maxima are exchanged together; a row's loads are in flight while the row before it is
+// worked on.  The scales of a CTA's rows are gathered in shared memory and leave as one run of rows per block, the layout the products
+// read.  Bound by memory: 8192 x 4096 bf16 (67 MB in, 35 MB out) 18 us, 5.6 TB/s; 1003 x 128256 61 us, 6.4 TB/s (75 with the maxima
+// exchanged one by one and a slow path that divides; 180 with a division a value and a warp a block).
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) quant_rows_kernel(const T* __restrict__ x, long long ld, int M, int K,
                                                          uint8_t* __restrict__ q, long long ld_q, float* __restrict__ s,
@@ -59,11 +59,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) quant_rows_kernel
         if (m + 1 < m1)  // the next row's loads are on their way while this one is worked on
 #pragma unroll
             for (int j = 0; j < 4; j++) load8(x + (m + 1) * ld, c0 + 256 * j + 8 * lane, K, aligned, next[j]);
-        uint32_t a[4];
         float scale[4], rec[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) a[j] = half_warp_max(amax8(cur[j]));
-        scales4(a, lane, scale, rec);
+        scales4(cur, lane, scale, rec);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             float v[8];

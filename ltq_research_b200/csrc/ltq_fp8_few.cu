@@ -10,6 +10,10 @@
 //   warps 2 .. 5  epilogue: lane = weight row; each block's sums times sw sx added to fp32 registers
 //   warps 1 ..    first quantize x
 //
+// Bound by the weight's bytes where it is large: 1 x 128256 x 2048 48 us, 5.5 TB/s; 24 rows 53 us, 5.0 TB/s: all CTAs read x
+// from L2 at the start, and the first MMAs wait for it longer than the ring of weight blocks lasts.  A small
+// weight is bound by the chain launch, first loads, MMAs, epilogue: 1 x 8192 x 2048 12 us, where the bytes alone would take 3.
+//
 // Narrow weights are cut along K over a cluster of 2, 4 or 8 CTAs; each hands the others their columns of its sums through
 // distributed shared memory and adds its own in the order of K.  Wide ones: one CTA an SM walks the row tiles.
 // Every mbarrier wait is bounded, as in ltq_fp8_gemm.cu.
@@ -73,6 +77,18 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
     const int kb0 = (int)((long long)g.nkb * split / g.splits), kb1 = (int)((long long)g.nkb * (split + 1) / g.splits);
     const int nb = kb1 - kb0;
 
+    // Four rows of x in two blocks of K, for one warp: eight columns a lane and row
+    constexpr int STEP = F_WARPS - 1;
+    const int quads = (g.M + 3) / 4;
+    Raw8<T> next[4] = {};
+    auto load_quad = [&](int u) {
+        const int pair = u / quads, m0 = 4 * (u - pair * quads), c = (kb0 + 2 * pair) * QB + 8 * lane;
+        const T* row = (const T*)g.x + m0 * g.ldx;
+#pragma unroll
+        for (int q = 0; q < 4; q++, row += g.ldx)
+            if (m0 + q < g.M) load8(row, c, g.K, g.aligned, next[q]);
+    };
+    if (BN > 16 && warp >= 1 && warp - 1 < (nb + 1) / 2 * quads) load_quad(warp - 1);
     if (tid == 0) {
         for (int i = 0; i < F_STAGES; i++) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
         for (int i = 0; i < F_BUFS; i++) mbar_init(&accfull[i], 1), mbar_init(&accempty[i], 4);
@@ -111,32 +127,58 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
         for (int j = issued > g.stages ? issued - g.stages : 0; j < issued; j++)
             mbar_wait(&empty[j % g.stages], (j / g.stages) & 1, g.err, F_WAIT);
     } else {
-        // x, a warp per row and two blocks, four of those in flight; rows M .. BN - 1 are zeros
         const int pairs = (nb + 1) / 2, piece = lane & 15;
-        const T* x = (const T*)g.x;
+        // rows M .. BN - 1 are zeros
         for (int i = tid - 32; i < nb * BN * (QB / 16); i += F_THREADS - 32)
             if (i / (QB / 16) % BN >= g.M) reinterpret_cast<uint4*>(xq)[i] = make_uint4(0, 0, 0, 0);
         for (int i = tid - 32; i < nb * BN; i += F_THREADS - 32)
             if (i % BN >= g.M) xs[i] = 0.f;
-        constexpr int AHEAD = 4, STEP = F_WARPS - 1;
-        for (int u0 = warp - 1; u0 < pairs * g.M; u0 += AHEAD * STEP) {
-            Raw8<T> raw[AHEAD];
+        if constexpr (BN == 16) {
+            // a row at a time, four in flight: little else fits the registers of two CTAs an SM
+            constexpr int AHEAD = 4;
+            const T* x = (const T*)g.x;
+            for (int u0 = warp - 1; u0 < pairs * g.M; u0 += AHEAD * STEP) {
+                Raw8<T> raw[AHEAD];
 #pragma unroll
-            for (int q = 0; q < AHEAD; q++) {
-                const int u = u0 + q * STEP, m = u % g.M, c = (kb0 + 2 * (u / g.M)) * QB + 8 * lane;
-                if (u < pairs * g.M) load8(x + m * g.ldx, c, g.K, g.aligned, raw[q]);
+                for (int q = 0; q < AHEAD; q++) {
+                    const int u = u0 + q * STEP, m = u % g.M, c = (kb0 + 2 * (u / g.M)) * QB + 8 * lane;
+                    if (u < pairs * g.M) load8(x + m * g.ldx, c, g.K, g.aligned, raw[q]);
+                }
+#pragma unroll
+                for (int q = 0; q < AHEAD; q++) {
+                    const int u = u0 + q * STEP, m = u % g.M, b = 2 * (u / g.M) + (lane >> 4);
+                    if (u >= pairs * g.M) break;
+                    float v[8];
+                    unpack8(raw[q], v);
+                    const float scale = block_scale(half_warp_max(amax8(raw[q])));
+                    const uint2 w = quant8(v, scale, __frcp_rn(scale));
+                    if (b < nb) {  // eight bytes; 16-byte chunks are swizzled by the row
+                        *reinterpret_cast<uint2*>(xq + b * BN * QB + m * QB + (((piece >> 1) ^ (m & 7)) << 4) + (piece & 1) * 8) = w;
+                        if (piece == 0) xs[b * BN + m] = scale;
+                    }
+                }
             }
+        } else {
+            // four rows at a time, the next four in flight: 32 x 128256 x 4096 108 us, 117 with the form above; two or
+            // three groups in flight are no faster
+            for (int u = warp - 1; u < pairs * quads; u += STEP) {
+                const int pair = u / quads, m0 = 4 * (u - pair * quads), b = 2 * pair + (lane >> 4);
+                Raw8<T> raw[4];
+                float scale[4], rec[4];
 #pragma unroll
-            for (int q = 0; q < AHEAD; q++) {
-                const int u = u0 + q * STEP, m = u % g.M, b = 2 * (u / g.M) + (lane >> 4);
-                if (u >= pairs * g.M) break;
-                float v[8];
-                unpack8(raw[q], v);
-                const float scale = block_scale(half_warp_max(amax8(raw[q])));
-                const uint2 w = quant8(v, scale, __frcp_rn(scale));
-                if (b < nb) {  // eight bytes; 16-byte chunks are swizzled by the row
-                    *reinterpret_cast<uint2*>(xq + b * BN * QB + m * QB + (((piece >> 1) ^ (m & 7)) << 4) + (piece & 1) * 8) = w;
-                    if (piece == 0) xs[b * BN + m] = scale;
+                for (int q = 0; q < 4; q++) raw[q] = next[q];
+                if (u + STEP < pairs * quads) load_quad(u + STEP);
+                scales4(raw, lane, scale, rec);
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int m = m0 + q;
+                    float v[8];
+                    unpack8(raw[q], v);
+                    const uint2 w = quant8(v, scale[q], rec[q]);
+                    if (m < g.M && b < nb) {
+                        *reinterpret_cast<uint2*>(xq + b * BN * QB + m * QB + (((piece >> 1) ^ (m & 7)) << 4) + (piece & 1) * 8) = w;
+                        if (piece == 0) xs[b * BN + m] = scale[q];
+                    }
                 }
             }
         }
