@@ -238,8 +238,8 @@ __device__ __forceinline__ void zero_slice(const DistillParams& p, const Slice<T
 // latencies in a chain (its weight, its slots, the sums, the cluster's barrier) and only other rows can fill them.  The last warp
 // works on the slots alone, while the others are in their first pass.
 // Bound: the logits read once and the gradient written once; an exponential an element and pass (16 a clock and SM) and the
-// instructions around it take 60 to 70 % of that time.  4096 x 128256 bf16 with the gradient: 384 us, 5.5 TB/s; 2048 rows, the loss
-// alone: 96 us, 5.5 TB/s.
+// instructions around it take 60 to 70 % of that time.  4096 x 128256 bf16 with the gradient, a quarter
+// of the rows of weight 0: 384 us, 4.8 TB/s; 2048 rows, the loss alone: 96 us, 5.5 TB/s.
 template <typename T, bool GRAD, bool REST>
 __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const DistillParams p)
 {

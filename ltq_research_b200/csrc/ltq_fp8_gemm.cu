@@ -19,7 +19,7 @@
 //
 // What bounds it: a block's MMAs take 512 cycles a pair, and the chain sum complete -> read (two rounds of 64 columns, for which
 // the registers beside the sums suffice) -> buffer handed back -> next MMAs about twice that, over two buffers.  8192 x 8192 x
-// 4096: 235 us, 2340 TFLOP/s (the MMAs alone, without epilogue, 160 us; a 256 x 128 tile with four buffers 290 us, for each hand-over
+// 4096: 240 us, 2290 TFLOP/s (the MMAs alone, without epilogue, 160 us; a 256 x 128 tile with four buffers 290 us, for each hand-over
 // costs the issuing warp the same).
 //
 // Pairs walk the tiles (rows first, so that neighbours share B in L2).  What is left after the last full round of tiles is cut

@@ -66,6 +66,17 @@ def test_quantize_ties_and_extremes():
     assert torch.equal(q.double(), plain_quant(x, 1)[0])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantize_tiny_scales(dtype):
+    """Rows of every magnitude down to the subnormal numbers: around the scales below which values and scale are taken larger."""
+    g = gen(9)
+    e = torch.arange(-149, -40, device="cuda", dtype=torch.float64)[:, None]
+    x = (torch.randn(109, 300, device="cuda", generator=g).double() * torch.exp2(e)).float().to(dtype)
+    q, s = fp8.quantize_rows(x)
+    wq, ws = plain_quant(x, 1)
+    assert torch.equal(s, ws) and torch.equal(q.double(), wq)
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_non_finite_values_make_their_rows_nan(bad):
     g = gen(3)
