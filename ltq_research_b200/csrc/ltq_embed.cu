@@ -17,6 +17,7 @@
 // zeros, 10 us joins.
 #include <algorithm>
 
+#include "launch_next.cuh"
 #include "ltq_b200.h"
 #include "stride_grid.cuh"
 #include "vec_types.cuh"
@@ -312,6 +313,7 @@ __global__ void __launch_bounds__(S_THREADS, 2) rank_fill_kernel(const SortParam
     __shared__ __align__(16) uint32_t key[RANK_MAX];
     __shared__ uint32_t bits[RANK_BITS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n4 = (p.n + 3) / 4;
+    next_may_start();
     for (int i = tid; i < 4 * n4; i += S_THREADS) key[i] = i < p.n ? sort_key(p, i) : 0xffffffffu;
     __syncthreads();
     for (int i = blockIdx.x * S_WARPS + warp; i < p.n; i += gridDim.x * S_WARPS) {
@@ -336,6 +338,7 @@ __global__ void __cluster_dims__(S_CL, 1, 1) __launch_bounds__(S_THREADS, 2) sor
 {
     extern __shared__ uint32_t sm[];
     const int cluster = blockIdx.x / S_CL;
+    next_may_start();
     if (cluster == 0) sort_cluster(p, sm);
     else fill_early(p, sm, blockIdx.x - S_CL, nullptr);
 }
@@ -385,6 +388,8 @@ __device__ __forceinline__ void store_part(float* part, const float (&a)[VEC])
 template <typename TI, typename TO, int VEC, bool ACC>
 __global__ void __launch_bounds__(128) sum_chunks_kernel(const SumParams p)
 {
+    wait_for_previous();
+    next_may_start();
     if (!ACC && blockIdx.x >= p.sum_ctas) {
         const int f = blockIdx.x - p.sum_ctas;
         fill_late(p.fill, p.key, p.n, f / p.fill.parts, f % p.fill.parts);
@@ -478,6 +483,7 @@ __global__ void __launch_bounds__(256) join_chunks_kernel(const SumParams p)
     __shared__ float stretch[8][32][VEC + 1];
     __shared__ int ends[32];  // the last chunk of a long row that begins in chunk i, or -1
     const int lane = threadIdx.x, warp = threadIdx.y, v = blockIdx.y * 32 + lane, nv = p.D / VEC, base = blockIdx.x * 32;
+    wait_for_previous();
     // those whose last row goes on into the next chunk and was not begun in an earlier one
     const int mine = base + lane, c0 = mine * p.chunk, c1 = c0 + p.chunk;
     uint32_t k1 = (uint32_t)p.V;
@@ -567,9 +573,9 @@ int sum_launch(SumParams p, cudaStream_t st)
     const unsigned slices = (p.D / VEC + 31) / 32;
     p.slices = (int)slices;
     p.sum_ctas = (p.nchunks + 3) / 4 * p.slices;
-    sum_chunks_kernel<TI, TO, VEC, ACC><<<p.sum_ctas + p.fill.shares * p.fill.parts, dim3(32, 4), 0, st>>>(p);
-    if (p.nchunks > 1) join_chunks_kernel<TO, VEC, ACC><<<dim3((p.nchunks + 30) / 32, slices), dim3(32, 8), 0, st>>>(p);
-    return (int)cudaGetLastError();
+    const cudaError_t e = launch_next(sum_chunks_kernel<TI, TO, VEC, ACC>, p.sum_ctas + p.fill.shares * p.fill.parts, dim3(32, 4), 0, st, p);
+    if (e != cudaSuccess || p.nchunks == 1) return (int)e;
+    return (int)launch_next(join_chunks_kernel<TO, VEC, ACC>, dim3((p.nchunks + 30) / 32, slices), dim3(32, 8), 0, st, p);
 }
 template <typename TI, typename TO>
 int sum_dispatch(const SumParams& p, cudaStream_t st)

@@ -3,6 +3,7 @@
 //
 // 128 values: s = max |x| / 448 (at least 2^-126), q = e4m3(x / s), an fp32 quotient rounded to nearest even; a block with a
 // NaN or an infinity becomes NaN.  Activations: one scale per row and 128 columns; weights: one per 128 x 128 block.
+#include "launch_next.cuh"
 #include "ltq_b200.h"
 #include "fp8_quant.cuh"
 
@@ -45,6 +46,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) quant_rows_kernel
                                                          long long ld_s, int aligned)
 {
     __shared__ float sc[8][8 * ROWS];
+    next_may_start();  // the product
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, groups = (K + 1023) / 1024;
     const int group = blockIdx.x % groups, c0 = group * 1024, mb = blockIdx.x / groups * (8 * ROWS);
     const int m0 = mb + warp * ROWS, m1 = min(M, m0 + ROWS);

@@ -27,6 +27,7 @@
 // order of K.  Every wait is bounded: when one runs out *err is set, the role stops and the CTAs still meet at their last barrier.
 #include "ltq_b200.h"
 #include "fp8_tc.cuh"
+#include "launch_next.cuh"
 #include "vec_types.cuh"
 
 namespace {
@@ -197,6 +198,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
     cluster_wait();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    wait_for_previous();  // A and its scales are written
+    next_may_start();     // the parts' join
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(W_REGS_ROLES));
@@ -379,6 +382,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) join_parts_kernel(const WideArgs g)
 {
     __shared__ float rows[32][J_COLS + 1];
+    wait_for_previous();
     const int tile = g.whole + blockIdx.x, rank = blockIdx.y >> 2, r0 = (blockIdx.y & 3) * 32, col0 = blockIdx.z * J_COLS;
     const int m0 = (tile % g.mt) * WT + rank * 128 + r0, n0 = (tile / g.mt) * WT + col0;
     if (m0 >= g.M || n0 >= g.N) return;
@@ -461,11 +465,9 @@ int run_wide(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc
         if (e != cudaSuccess) return (int)e;
         ready[dev].store(1, std::memory_order_release);
     }
-    gemm_wide_kernel<T><<<2 * p.pairs, W_THREADS, W_SMEM, st>>>(ta, tb, tc, g);
-    cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_next(gemm_wide_kernel<T>, 2 * p.pairs, W_THREADS, W_SMEM, st, ta, tb, tc, g);
     if (e != cudaSuccess || p.whole == p.tiles) return (int)e;
-    join_parts_kernel<T><<<dim3(p.tiles - p.whole, 8, WT / J_COLS), 256, 0, st>>>(g);
-    return (int)cudaGetLastError();
+    return (int)launch_next(join_parts_kernel<T>, dim3(p.tiles - p.whole, 8, WT / J_COLS), 256, 0, st, g);
 }
 
 }  // namespace
