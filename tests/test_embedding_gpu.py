@@ -223,6 +223,30 @@ def test_autograd_and_streams():
     check_grad(tok, dout, 90, 2.0, 1, got=table.grad)
 
 
+@pytest.mark.parametrize("n,V,D", [(700, 5000, 264), (9000, 40000, 1040)])
+def test_grad_calls_one_after_another(n, V, D):
+    """Calls without a pause between them, into one output, alone and from a graph: each has the result that it has by itself."""
+    g = gen(n)
+    toks = [(torch.rand(n, device="cuda", generator=g) ** 3 * V).long() for _ in range(4)]
+    d = torch.randn(n, D, device="cuda", generator=g).bfloat16()
+    want = []
+    for t in toks:
+        want.append(embedding.lookup_grad(t, d, V))
+        torch.cuda.synchronize()
+    out = torch.empty(V, D, device="cuda")
+    tok = toks[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        embedding.lookup_grad(tok, d, V, out=out)
+    for k in range(12):
+        embedding.lookup_grad(toks[(k + 1) % 4], d, V, out=out)
+        embedding.lookup_grad(toks[k % 4], d, V, out=out)
+        assert torch.equal(out, want[k % 4])
+        tok.copy_(toks[(k + 2) % 4])
+        graph.replay()
+        assert torch.equal(out, want[(k + 2) % 4])
+
+
 def test_refusals():
     table = torch.zeros(10, 8, device="cuda")
     tok = torch.zeros(3, dtype=torch.int64, device="cuda")

@@ -212,6 +212,32 @@ def test_cuda_graph():
     assert torch.equal(y, fp8.linear(x, W))
 
 
+@pytest.mark.parametrize("M,N,K", [(60, 512, 640), (300, 256, 4000), (700, 1100, 256)])
+def test_calls_one_after_another(M, N, K):
+    """Calls without a pause between them, in buffers that pass from one to the next, alone and from a graph: each has the
+    result that it has by itself."""
+    g = gen(M)
+    W = fp8.BlockWeight.quantize(torch.randn(N, K, device="cuda", generator=g))
+    xs = [torch.randn(M, K, device="cuda", generator=g).bfloat16() for _ in range(6)]
+    want = []
+    for x in xs:
+        want.append(fp8.linear(x, W))
+        torch.cuda.synchronize()
+    for _ in range(10):
+        got = [fp8.linear(x, W) for x in xs]
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    x = xs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = fp8.linear(x, W)
+        z = fp8.linear(x * 2, W)
+    for k in range(6):
+        x.copy_(xs[k])
+        graph.replay()
+        assert torch.equal(y, want[k]) and torch.equal(z, want[k] * 2)
+    fp8.check_errors(x.device)
+
+
 def test_gradient_against_differences():
     """linear is linear in its quantized input, and inputs that are e4m3 values under a power of two quantize to themselves
     when their block holds 448 of it: so the difference quotient is exact but for the sums' rounding."""
