@@ -22,9 +22,13 @@
 // 4096: 240 us, 2290 TFLOP/s (the MMAs alone, without epilogue, 160 us; a 256 x 128 tile with four buffers 290 us, for each hand-over
 // costs the issuing warp the same).
 //
-// Pairs walk the tiles (rows first, so that neighbours share B in L2).  What is left after the last full round of tiles is cut
-// along K into equal shares (a share may end inside a tile); the parts go to a workspace and join_parts_kernel adds them in the
-// order of K.  Every wait is bounded: when one runs out *err is set, the role stops and the CTAs still meet at their last barrier.
+// Pairs walk the tiles (rows first, so that neighbours share B in L2).  The tiles that are left after the last full round are cut
+// along K into one equal share for each pair: as many slices of each tile as there are pairs for, and the rest of K of all tiles, cut
+// across tiles, for the pairs that remain.  So all tiles' slices run through the same K at the same time and a block of A or B is
+// read from memory once and by the other tiles from L2: 1003 x 2048 x 128256 249 us and 0.5 GB of reads, where shares that follow one
+// another through the tiles took 266 us and 1.5 GB.  The parts go to a workspace and join_parts_kernel adds them in the order of K.  Every wait is bounded: when one runs out *err is set, the role stops and the CTAs still meet at their last barrier.
+#include <algorithm>
+
 #include "ltq_b200.h"
 #include "fp8_tc.cuh"
 #include "launch_next.cuh"
@@ -120,36 +124,53 @@ struct WideArgs {
     long long ld_sb;
     void* C;
     long long ldc;
-    float* parts;  // [pair][2][CTA][column / 4][row][4]
+    float* parts;  // [part][CTA][column / 4][row][4]
     int* err;
     int M, N, nkb, mt, whole, tma_c;  // whole: tiles done in one piece
-    long long shared_units;           // blocks of K of the tiles after them,
-    int sharers;                      // shared equally by the first `sharers` pairs (at least one block each)
+    int cut;                          // tiles after them, of which pair g cut + r < slices cut takes blocks g slice .. of tile r;
+    int slices, slice;                // the `tail` blocks behind a tile's slices, all tiles' in a row, are shared equally by the
+    int tail, tailers;                // next `tailers` pairs (at least one block each)
 };
+// a pair's slice is part g cut + r; of the tails that of the q-th of its pairs in tile r is part slices cut + q + r (from share to share
+// and tile to tile one of q and r grows, so no two are the same)
+__host__ __device__ inline int part_count(int cut, int slices, int tail, int tailers)
+{
+    return cut * slices + (tail ? cut + tailers - 1 : 0);
+}
+__device__ __forceinline__ long long tail_share(const WideArgs& g, int q) { return (long long)g.cut * g.tail * q / g.tailers; }
 
 struct Segment {
-    int tile, k0, k1;
+    int tile, k0, k1, part;
 };
 // the pieces of work of pair c of G, in order
 struct Walk {
-    int c, G, nkb, whole, t;
-    long long u, u1;
-    __device__ Walk(const WideArgs& g, int c_, int G_)
-        : c(c_), G(G_), nkb(g.nkb), whole(g.whole), t(c_), u(0), u1(0)
+    const WideArgs& g;
+    int c, pairs, t;
+    bool slice;       // still to be done
+    long long u, u1;  // blocks of the tails
+    __device__ Walk(const WideArgs& g_, int c_, int pairs_)
+        : g(g_), c(c_), pairs(pairs_), t(c_), slice(c_ < g_.slices * g_.cut), u(0), u1(0)
     {
-        if (c < g.sharers) u = g.shared_units * c / g.sharers, u1 = g.shared_units * (c + 1) / g.sharers;
+        const int q = c - g.slices * g.cut;
+        if (q >= 0 && q < g.tailers) u = tail_share(g, q), u1 = tail_share(g, q + 1);
     }
     __device__ bool next(Segment& s)
     {
-        if (t < whole) {
-            s = {t, 0, nkb};
-            t += G;
+        if (t < g.whole) {
+            s = {t, 0, g.nkb, 0};
+            t += pairs;
+            return true;
+        }
+        if (slice) {
+            const int k0 = c / g.cut * g.slice;
+            s = {g.whole + c % g.cut, k0, k0 + g.slice, c};
+            slice = false;
             return true;
         }
         if (u >= u1) return false;
-        const int k0 = (int)(u % nkb);
+        const int r = (int)(u / g.tail), k = (int)(u % g.tail), k0 = g.slices * g.slice + k;
         const long long left = u1 - u;
-        s = {whole + (int)(u / nkb), k0, left < nkb - k0 ? k0 + (int)left : nkb};
+        s = {g.whole + r, k0, left < g.tail - k ? k0 + (int)left : g.nkb, c + r};
         u += s.k1 - s.k0;
         return true;
     }
@@ -330,7 +351,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
             }
             if (!ok) break;
             if (s.k0 != 0 || s.k1 != g.nkb) {  // a part of the tile's sum
-                float* part = g.parts + (((long long)pair * 2 + (s.k0 ? 0 : 1)) * 2 + rank) * PART_FLOATS;
+                float* part = g.parts + ((long long)s.part * 2 + rank) * PART_FLOATS;
 #pragma unroll
                 for (int c = 0; c < 32; c++)
                     *reinterpret_cast<float4*>(part + ((half * 32 + c) * 128 + 32 * quarter + lane) * 4) =
@@ -386,22 +407,23 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const WideArgs g)
     const int tile = g.whole + blockIdx.x, rank = blockIdx.y >> 2, r0 = (blockIdx.y & 3) * 32, col0 = blockIdx.z * J_COLS;
     const int m0 = (tile % g.mt) * WT + rank * 128 + r0, n0 = (tile / g.mt) * WT + col0;
     if (m0 >= g.M || n0 >= g.N) return;
-    const long long a = (long long)blockIdx.x * g.nkb, b = a + g.nkb, U = g.shared_units;
-    const int npairs = g.sharers;
-    int c0 = (int)(a * npairs / U);  // the pair whose share holds block a, or the one before it
-    while (U * (c0 + 1) / npairs <= a) c0++;
-    if (U * c0 / npairs <= a && U * (c0 + 1) / npairs >= b) return;  // one pair did all of the tile
     const int r = threadIdx.x & 31, q = threadIdx.x >> 5;
     float4 v[2] = {};
-    for (int c = c0; c < npairs && U * c / npairs < b; c++) {
-        // a share that begins inside the tile left part 0, one that begins at its first block or before it part 1
-        const int slot = U * c / npairs > a ? 0 : 1;
-        const float* part = g.parts + (((long long)c * 2 + slot) * 2 + rank) * PART_FLOATS + (col0 / 4 * 128LL + r0 + r) * 4;
+    auto add = [&](int index) {
+        const float* part = g.parts + ((long long)index * 2 + rank) * PART_FLOATS + (col0 / 4 * 128LL + r0 + r) * 4;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const float4 x = *reinterpret_cast<const float4*>(part + (q + 8 * h) * 512);
             v[h].x += x.x, v[h].y += x.y, v[h].z += x.z, v[h].w += x.w;
         }
+    };
+    const int cut_tile = blockIdx.x;
+    for (int i = 0; i < g.slices; i++) add(i * g.cut + cut_tile);
+    if (g.tail) {
+        const long long a = (long long)cut_tile * g.tail, b = a + g.tail;
+        int c = (int)(a * g.tailers / ((long long)g.cut * g.tail));  // the share that holds block a, or the one before it
+        while (tail_share(g, c + 1) <= a) c++;
+        for (; c < g.tailers && tail_share(g, c) < b; c++) add(g.slices * g.cut + c + cut_tile);
     }
 #pragma unroll
     for (int h = 0; h < 2; h++) {
@@ -430,8 +452,7 @@ bool make_map_out(CUtensorMap* m, void* base, int es, long long rows, long long 
 }
 
 struct WidePlan {
-    int mt, tiles, nkb, pairs, whole, sharers;
-    long long shared_units;
+    int mt, tiles, nkb, pairs, whole, cut, slices, slice, tail, tailers;
     size_t workspace;
 };
 // Whole tiles in rounds of one per pair; the tiles of a last round that would leave pairs idle are shared along K when that
@@ -445,12 +466,23 @@ WidePlan plan_wide(int M, int N, int K, int sms)
     p.pairs = sms / 2 > 0 ? sms / 2 : 1;
     const int rest = p.tiles % p.pairs;
     const bool share = rest && (double)(p.pairs - rest) / p.pairs * p.nkb * 0.5 > 10.0;
-    p.whole = share ? p.tiles - rest : p.tiles;
-    p.shared_units = (long long)(p.tiles - p.whole) * p.nkb;
-    p.sharers = (int)(p.shared_units / 4 < p.pairs ? (p.shared_units + 3) / 4 : p.pairs);  // at least about four blocks each
-    const int busy = p.whole < p.sharers ? p.sharers : p.whole;
+    p.whole = p.tiles;
+    if (share) {
+        const long long blocks = (long long)rest * p.nkb;
+        p.slice = (int)std::max((blocks + p.pairs - 1) / p.pairs, 4LL);  // of at least 20 blocks, or it would not save so much
+        p.slices = p.nkb / p.slice;  // rest < pairs: at least one, and at most pairs / rest
+        p.tail = p.nkb - p.slices * p.slice;
+        if (p.slices > 1 || p.tail) {
+            p.cut = rest, p.whole -= rest;
+            // not 0 where there is a tail: with a pair for each slice the slices would have taken all of K
+            const long long tails = (long long)rest * p.tail, left = p.pairs - p.slices * rest;
+            p.tailers = (int)std::min((tails + 3) / 4, left);
+        }
+    }
+    if (!p.cut) p.slice = p.slices = p.tail = p.tailers = 0;
+    const int sharers = p.slices * p.cut + p.tailers, busy = p.whole < sharers ? sharers : p.whole;
     if (busy < p.pairs) p.pairs = busy;
-    p.workspace = (size_t)p.sharers * 4 * PART_FLOATS * 4;
+    p.workspace = (size_t)(p.cut ? part_count(p.cut, p.slices, p.tail, p.tailers) : 0) * 2 * PART_FLOATS * 4;
     return p;
 }
 
@@ -466,8 +498,8 @@ int run_wide(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc
         ready[dev].store(1, std::memory_order_release);
     }
     const cudaError_t e = launch_next(gemm_wide_kernel<T>, 2 * p.pairs, W_THREADS, W_SMEM, st, ta, tb, tc, g);
-    if (e != cudaSuccess || p.whole == p.tiles) return (int)e;
-    return (int)launch_next(join_parts_kernel<T>, dim3(p.tiles - p.whole, 8, WT / J_COLS), 256, 0, st, g);
+    if (e != cudaSuccess || !p.cut) return (int)e;
+    return (int)launch_next(join_parts_kernel<T>, dim3(p.cut, 8, WT / J_COLS), 256, 0, st, g);
 }
 
 }  // namespace
@@ -494,7 +526,8 @@ extern "C" int ltq_fp8_gemm(const uint8_t* A, long long lda, const float* sa, lo
     if (!make_map_8(&ta, A, M, K, lda, 128) || !make_map_8(&tb, B, N, K, ldb, 128)) return -1;
     const int tma_c = (uintptr_t)C % 16 == 0 && ldc * es % 16 == 0;
     if (tma_c && !make_map_out(&tc, C, es, M, N, ldc)) return -1;
-    const WideArgs g{sa, ld_sa, sb, ld_sb, C, ldc, (float*)workspace, err, M, N, p.nkb, p.mt, p.whole, tma_c, p.shared_units, p.sharers};
+    const WideArgs g{sa, ld_sa, sb, ld_sb, C, ldc, (float*)workspace, err, M, N, p.nkb, p.mt, p.whole, tma_c,
+                     p.cut, p.slices, p.slice, p.tail, p.tailers};
     const cudaStream_t st = (cudaStream_t)stream;
     if (dtype == DT_F32) return run_wide<float>(ta, tb, tc, g, p, st);
     if (dtype == DT_BF16) return run_wide<__nv_bfloat16>(ta, tb, tc, g, p, st);

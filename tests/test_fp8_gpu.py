@@ -212,6 +212,19 @@ def test_cuda_graph():
     assert torch.equal(y, fp8.linear(x, W))
 
 
+@pytest.mark.parametrize("M,N,K", [(40, 100, 2900), (257, 257, 5300), (600, 1100, 9000), (1030, 2048, 11000), (2048, 2040, 20000),
+                                   (1800, 2560, 17000)])
+def test_long_sums(M, N, K):
+    """Few tiles and a long K, cut among the GPU's SMs: slices that fill them, slices and a rest, one slice and a rest."""
+    g = gen(K)
+    W = fp8.BlockWeight.quantize(torch.randn(N, K, device="cuda", generator=g))
+    x = torch.randn(M, K, device="cuda", generator=g).bfloat16()
+    y = fp8.linear(x, W, dtype=torch.float32)
+    check(x, W, y)
+    assert torch.equal(y, fp8.linear(x, W, dtype=torch.float32))
+    fp8.check_errors(x.device)
+
+
 @pytest.mark.parametrize("M,N,K", [(60, 512, 640), (300, 256, 4000), (700, 1100, 256)])
 def test_calls_one_after_another(M, N, K):
     """Calls without a pause between them, in buffers that pass from one to the next, alone and from a graph: each has the
