@@ -10,7 +10,7 @@
 //   warps 2 .. 5  epilogue: lane = weight row; each block's sums times sw sx added to fp32 registers
 //   warps 1 ..    first quantize x
 //
-// Bound by the weight's bytes where it is large: 1 x 128256 x 2048 48 us, 5.5 TB/s; 24 rows 53 us, 5.0 TB/s: all CTAs read x
+// Bound by the weight's bytes where it is large: 1 x 128256 x 2048 48 us, 5.5 TB/s; 24 rows 52 us, 5.1 TB/s: all CTAs read x
 // from L2 at the start, and the first MMAs wait for it longer than the ring of weight blocks lasts.  A small
 // weight is bound by the chain launch, first loads, MMAs, epilogue: 1 x 8192 x 2048 12 us, where the bytes alone would take 3.
 //
@@ -53,9 +53,18 @@ __device__ __forceinline__ void arrive(uint64_t* b)
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(b)) : "memory");
 }
 
+// where `p` of this CTA's shared memory lies in CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t map_other(const void* p, uint32_t rank)
+{
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+
 template <typename T, int BN>
 __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(const __grid_constant__ CUtensorMap tmW, const FewArgs g)
 {
+    constexpr bool DUO = BN > 16;             // pairs of CTAs, each of which quantizes half of x for both (K is never cut then)
     constexpr int PER = 2;                    // blocks whose sums are handed over together
     constexpr int F_BUFS = BN == 16 ? 8 : 4;  // tensor-memory buffers
     extern __shared__ uint8_t smem_raw[];
@@ -88,7 +97,8 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
         for (int q = 0; q < 4; q++, row += g.ldx)
             if (m0 + q < g.M) load8(row, c, g.K, g.aligned, next[q]);
     };
-    if (BN > 16 && warp >= 1 && warp - 1 < (nb + 1) / 2 * quads) load_quad(warp - 1);
+    const int duo_rank = DUO ? (int)cluster_rank() : 0, first = 2 * (warp - 1) + duo_rank;
+    if (DUO && warp >= 1 && first < (nb + 1) / 2 * quads) load_quad(first);
     if (tid == 0) {
         for (int i = 0; i < F_STAGES; i++) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
         for (int i = 0; i < F_BUFS; i++) mbar_init(&accfull[i], 1), mbar_init(&accempty[i], 4);
@@ -102,11 +112,13 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
     tc_fence_before();
     __syncthreads();
     if (g.splits > 1) cluster_arrive_relaxed();  // paired with the wait before the columns are handed over
+    if (DUO) cluster_arrive_relaxed();           // paired with the wait before x is written to both CTAs
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     bool waited = false;  // for the cluster's start
 
     if (warp == 0) {
+        if (DUO) cluster_wait(), cluster_arrive_relaxed();  // for the barrier behind x, to which this warp adds nothing
         int st = 0;
         uint32_t parity = 1;  // the first wait for each buffer passes at once
         int issued = 0;
@@ -126,6 +138,8 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
         // none of this CTA's copies is in flight when it leaves: a buffer is free again once they have landed and been read
         for (int j = issued > g.stages ? issued - g.stages : 0; j < issued; j++)
             mbar_wait(&empty[j % g.stages], (j / g.stages) & 1, g.err, F_WAIT);
+        __syncwarp();
+        if (DUO) cluster_wait();
     } else {
         const int pairs = (nb + 1) / 2, piece = lane & 15;
         // rows M .. BN - 1 are zeros
@@ -133,7 +147,7 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
             if (i / (QB / 16) % BN >= g.M) reinterpret_cast<uint4*>(xq)[i] = make_uint4(0, 0, 0, 0);
         for (int i = tid - 32; i < nb * BN; i += F_THREADS - 32)
             if (i % BN >= g.M) xs[i] = 0.f;
-        if constexpr (BN == 16) {
+        if constexpr (!DUO) {
             // a row at a time, four in flight: little else fits the registers of two CTAs an SM
             constexpr int AHEAD = 4;
             const T* x = (const T*)g.x;
@@ -159,15 +173,17 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
                 }
             }
         } else {
-            // four rows at a time, the next four in flight: 32 x 128256 x 4096 108 us, 117 with the form above; two or
-            // three groups in flight are no faster
-            for (int u = warp - 1; u < pairs * quads; u += STEP) {
+            // four rows at a time, the next four in flight, half of them each CTA of a pair: 32 x 128256 x 4096 100 us, 106 if each does
+            // all, 117 also in the form above; two or three groups in flight are no faster
+            cluster_wait();
+            const uint32_t xq_other = map_other(xq, duo_rank ^ 1), xs_other = map_other(xs, duo_rank ^ 1);
+            for (int u = first; u < pairs * quads; u += 2 * STEP) {
                 const int pair = u / quads, m0 = 4 * (u - pair * quads), b = 2 * pair + (lane >> 4);
                 Raw8<T> raw[4];
                 float scale[4], rec[4];
 #pragma unroll
                 for (int q = 0; q < 4; q++) raw[q] = next[q];
-                if (u + STEP < pairs * quads) load_quad(u + STEP);
+                if (u + 2 * STEP < pairs * quads) load_quad(u + 2 * STEP);
                 scales4(raw, lane, scale, rec);
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
@@ -176,14 +192,25 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
                     unpack8(raw[q], v);
                     const uint2 w = quant8(v, scale[q], rec[q]);
                     if (m < g.M && b < nb) {
-                        *reinterpret_cast<uint2*>(xq + b * BN * QB + m * QB + (((piece >> 1) ^ (m & 7)) << 4) + (piece & 1) * 8) = w;
-                        if (piece == 0) xs[b * BN + m] = scale[q];
+                        const int at = b * BN * QB + m * QB + (((piece >> 1) ^ (m & 7)) << 4) + (piece & 1) * 8;
+                        *reinterpret_cast<uint2*>(xq + at) = w;
+                        asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};\n" ::"r"(xq_other + at), "r"(w.x), "r"(w.y) : "memory");
+                        if (piece == 0) {
+                            xs[b * BN + m] = scale[q];
+                            asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(xs_other + 4 * (b * BN + m)), "f"(scale[q]) : "memory");
+                        }
                     }
                 }
             }
         }
-        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // written here, read by the MMAs
-        asm volatile("bar.sync 1, %0;\n" ::"n"(F_THREADS - 32) : "memory");
+        asm volatile("fence.proxy.async;\n" ::: "memory");  // written here, read by the MMAs
+        __syncwarp();
+        if (DUO) {
+            cluster_arrive();
+            cluster_wait();
+            asm volatile("fence.proxy.async;\n" ::: "memory");
+        } else
+            asm volatile("bar.sync 1, %0;\n" ::"n"(F_THREADS - 32) : "memory");
 
         if (warp == 1) {
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
@@ -308,7 +335,7 @@ struct FewPlan {
 // at 64 (one block a buffer, 88 us for 128256 x 2048) the 256-row tiles behind a separate quantization are as fast (83 us).
 bool plan_few(int M, int N, int K, int sms, FewPlan& p)
 {
-    if (M < 1 || M > F_ROWS || N < 1 || K < 1 || sms < 1) return false;
+    if (M < 1 || M > F_ROWS || N < 1 || K < 1 || sms < 2) return false;
     p.bn = M <= 16 ? 16 : 32;
     p.nkb = (int)(((long long)K + QB - 1) / QB);
     p.tiles = (int)(((long long)N + 127) / 128);
@@ -330,6 +357,7 @@ bool plan_few(int M, int N, int K, int sms, FewPlan& p)
     while (p.stages < F_STAGES && p.stages < blocks && need(p.splits, p.stages + 1) <= budget) p.stages++;
     p.smem = need(p.splits, p.stages);
     p.grid = (p.splits > 1 || p.tiles < sms ? p.tiles : sms) * p.splits;
+    if (p.bn > 16) p.grid &= ~1;
     return true;
 }
 
@@ -352,9 +380,9 @@ int run_few(const CUtensorMap& tw, const FewArgs& g, const FewPlan& p, cudaStrea
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim = {(unsigned)p.splits, 1, 1};
+    at[0].val.clusterDim = {BN > 16 ? 2u : (unsigned)p.splits, 1, 1};
     cfg.attrs = at;
-    cfg.numAttrs = p.splits > 1 ? 1 : 0;
+    cfg.numAttrs = BN > 16 || p.splits > 1 ? 1 : 0;
     return (int)cudaLaunchKernelEx(&cfg, k, tw, g);
 }
 template <typename T>
