@@ -132,6 +132,7 @@ __device__ void sort_cluster(const SortParams& p, uint32_t* sm)
     const int i0 = (int)(a < p.n ? a : p.n), i1 = (int)(a + per < p.n ? a + per : p.n);
     const bool kept = per <= 32 * KEPT;
     uint32_t* mine = hist + warp * BINS;
+    cluster_arrive_relaxed();  // paired with the first pass's wait: the others' shared memory is written once they have started
     for (int pass = 0; pass < p.passes; pass++) {
         const int shift = pass * DIGIT;
         const uint32_t* ik = p.key[(pass & 1) ^ 1];
@@ -167,6 +168,7 @@ __device__ void sort_cluster(const SortParams& p, uint32_t* sm)
             reinterpret_cast<uint2*>(hist + w * BINS)[tid] = run;
             run.x += c[w].x, run.y += c[w].y;
         }
+        if (pass == 0) cluster_wait();  // the later passes have the barrier at the end of the one before
         for (int q = 0; q < S_CL; q++) {
             st_cluster_u32(&all[rank * BINS + 2 * tid], q, run.x);
             st_cluster_u32(&all[rank * BINS + 2 * tid + 1], q, run.y);

@@ -247,6 +247,17 @@ def test_grad_calls_one_after_another(n, V, D):
         assert torch.equal(out, want[(k + 2) % 4])
 
 
+@pytest.mark.parametrize("n,V", [(8193, 900), (20001, 70000), (100000, 1 << 21)])
+def test_grad_of_many_positions_again_and_again(n, V):
+    """One, two and three digit passes in a cluster, beside CTAs of the call before that still write: the same bits each time."""
+    g = gen(n)
+    tok = torch.randint(0, V, (n,), device="cuda", generator=g)
+    dout = torch.randn(n, 8, device="cuda", generator=g)
+    want = check_grad(tok, dout, V)
+    for _ in range(30):
+        assert torch.equal(embedding.lookup_grad(tok, dout, V), want)
+
+
 def test_refusals():
     table = torch.zeros(10, 8, device="cuda")
     tok = torch.zeros(3, dtype=torch.int64, device="cuda")
