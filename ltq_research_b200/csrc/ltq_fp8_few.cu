@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
         bool ok = true;
         for (int tile = worker; tile < g.tiles && ok; tile += workers)
             for (int k = kb0; k < kb1; k++) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], parity, g.err, F_WAIT));
+                ok = mbar_wait_warp(&empty[st], parity, g.err, F_WAIT);
                 if (!ok) break;
                 if (elect_one()) {
                     mbar_expect_tx(&full[st], F_STAGE);
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
             }
         // none of this CTA's copies is in flight when it leaves: a buffer is free again once they have landed and been read
         for (int j = issued > g.stages ? issued - g.stages : 0; j < issued; j++)
-            mbar_wait(&empty[j % g.stages], (j / g.stages) & 1, g.err, F_WAIT);
+            mbar_wait_warp(&empty[j % g.stages], (j / g.stages) & 1, g.err, F_WAIT);
         __syncwarp();
         if (DUO) cluster_wait();
     } else {
@@ -220,9 +220,8 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
             bool ok = true;
             for (int tile = worker; tile < g.tiles && ok; tile += workers)
                 for (int k = 0; k < nb; k++) {
-                    ok = mbar_wait(&full[st], full_parity, g.err, F_WAIT) &&
-                         (k % PER || mbar_wait(&accempty[buf], free_parity, g.err, F_WAIT));
-                    ok = __all_sync(0xffffffffu, ok);
+                    ok = mbar_wait_warp(&full[st], full_parity, g.err, F_WAIT) &&
+                         (k % PER || mbar_wait_warp(&accempty[buf], free_parity, g.err, F_WAIT));
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t a = wdesc + (uint32_t)(st * (F_STAGE >> 4)), b = xdesc + (uint32_t)(k * (BN * QB >> 4));
@@ -254,7 +253,7 @@ __global__ void __launch_bounds__(F_THREADS, BN == 16 ? 2 : 1) gemm_few_kernel(c
                     float sw[PER];
 #pragma unroll
                     for (int h = 0; h < PER; h++) sw[h] = __shfl_sync(0xffffffffu, sw32, (k + h) & 31);
-                    ok = __all_sync(0xffffffffu, mbar_wait(&accfull[buf], parity, g.err, F_WAIT));
+                    ok = mbar_wait_warp(&accfull[buf], parity, g.err, F_WAIT);
                     if (!ok) break;
                     tc_fence_after();
                     uint32_t part[PER * BN];  // behind a single last block the second half is not used

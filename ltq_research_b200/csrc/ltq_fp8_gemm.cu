@@ -26,7 +26,8 @@
 // along K into one equal share for each pair: as many slices of each tile as there are pairs for, and the rest of K of all tiles, cut
 // across tiles, for the pairs that remain.  So all tiles' slices run through the same K at the same time and a block of A or B is
 // read from memory once and by the other tiles from L2: 1003 x 2048 x 128256 249 us and 0.5 GB of reads, where shares that follow one
-// another through the tiles took 266 us and 1.5 GB.  The parts go to a workspace and join_parts_kernel adds them in the order of K.  Every wait is bounded: when one runs out *err is set, the role stops and the CTAs still meet at their last barrier.
+// another through the tiles took 266 us and 1.5 GB.  The parts go to a workspace and join_parts_kernel adds them in the order of K.  Every wait is bounded: when one runs out
+// *err is set, the role stops and the CTAs still meet at their last barrier.
 #include <algorithm>
 
 #include "ltq_b200.h"
@@ -233,7 +234,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
                 const int m0 = (s.tile % g.mt) * WT + rank * 128, n0 = (s.tile / g.mt) * WT + rank * 128;
                 for (int k = s.k0; k < s.k1; k++, i++) {
                     const int st = i % W_STAGES;
-                    if (i >= W_STAGES && !mbar_wait(&empty[st], (i / W_STAGES - 1) & 1, g.err, WAIT_LIMIT)) {
+                    if (i >= W_STAGES && !mbar_wait_warp(&empty[st], (i / W_STAGES - 1) & 1, g.err, WAIT_LIMIT)) {
                         ok = false;
                         break;
                     }
@@ -247,7 +248,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
                 }
             }
             // a buffer is free again once its copies have landed and been read: none is in flight when the CTA leaves
-            for (int j = i > W_STAGES ? i - W_STAGES : 0; j < i; j++) mbar_wait(&empty[j % W_STAGES], (j / W_STAGES) & 1, g.err, WAIT_LIMIT);
+            for (int j = i > W_STAGES ? i - W_STAGES : 0; j < i; j++)
+                mbar_wait_warp(&empty[j % W_STAGES], (j / W_STAGES) & 1, g.err, WAIT_LIMIT);
         }
         if (warp == 9 && rank == 0) {
             // the whole warp runs the loop and one elected lane issues: the operands then stay in uniform registers
@@ -261,9 +263,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
             bool ok = true;
             while (ok && walk.next(s))
                 for (int k = s.k0; k < s.k1; k++) {
-                    ok = mbar_wait(&full[st], full_parity, g.err, WAIT_LIMIT) &&
-                         mbar_wait(&accempty[buf], free_parity, g.err, WAIT_LIMIT);
-                    ok = __all_sync(0xffffffffu, ok);
+                    ok = mbar_wait_warp(&full[st], full_parity, g.err, WAIT_LIMIT) &&
+                         mbar_wait_warp(&accempty[buf], free_parity, g.err, WAIT_LIMIT);
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t a = base + (uint32_t)(st * (W_STAGE >> 4)), b = a + (W_OP >> 4);
@@ -322,7 +323,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
                     if (kq + kj >= s.k1) break;
                     const float sc = sa[kj] * __shfl_sync(0xffffffffu, sb32, at + kj);
                     const int buf = i & 1;
-                    ok = mbar_wait(&accfull[buf], (i / 2) & 1, g.err, WAIT_LIMIT);
+                    ok = mbar_wait_warp(&accfull[buf], (i / 2) & 1, g.err, WAIT_LIMIT);
                     i++;
                     if (!ok) break;
                     tc_fence_after();

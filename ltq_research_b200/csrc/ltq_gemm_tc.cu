@@ -105,7 +105,7 @@ __device__ __forceinline__ void tma_store_box(const CUtensorMap* map, const void
 __device__ __forceinline__ void epilogue_tma(const GemmParams& p, const CUtensorMap* tmC, bool reduce, uint64_t* accum,
                                              uint32_t tmem, uint8_t* smem, int m0, int n0, int warp, int lane)
 {
-    const bool ok = mbar_wait(accum, 0, p.err);
+    const bool ok = mbar_wait_warp(accum, 0, p.err);
     __syncwarp();
     tc_fence_after();
     if (!ok) return;
@@ -145,7 +145,7 @@ __device__ __forceinline__ void epilogue_tma(const GemmParams& p, const CUtensor
 __device__ __forceinline__ void epilogue(const GemmParams& p, uint64_t* accum, uint32_t tmem, uint8_t* smem, int m0,
                                          int n0, int warp, int lane)
 {
-    const bool ok = mbar_wait(accum, 0, p.err);
+    const bool ok = mbar_wait_warp(accum, 0, p.err);
     __syncwarp();
     tc_fence_after();
     if (!ok) return;
@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(192, 1) gemm_bf16x3p_tn_persist(const __grid_c
             int m0, n0, z;
             tile_of(t, m0, n0, z);
             const int acc = i & 1;
-            const bool ok = mbar_wait(&accfull[acc], (i >> 1) & 1, p.err);
+            const bool ok = mbar_wait_warp(&accfull[acc], (i >> 1) & 1, p.err);
             __syncwarp();
             tc_fence_after();
             if (!ok) break;
