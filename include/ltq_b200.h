@@ -305,7 +305,8 @@ int ltq_viterbi_tb_noalloc(const float* x, const float* w, int w_stride, const f
  *       loss = weight (sum p (log p - log q) + p_r (log p_r - log q_r))
  *   mode 0: loss [T], and stats [T, 3] = (m, s, r) when not NULL: sum exp(z / temperature) = s 2^m, q_r = 2^r; mode 1: the same and
  *   dlogits = d loss / d logits (dtype, row stride ld_d; may be `logits` itself with ld_d = ld); mode 2: dlogits alone, from
- *   stats, times grad[t * grad_stride] (or NULL: 1).  Terms with p = 0 are 0; a row without a live slot has loss and gradient
+ *   stats, times grad[t * grad_stride] (or NULL: 1).  Logits of any finite size, and any mass q_r > 0, have their loss and gradient (in
+ *   rows of logits beyond 2^29 temperature, m may round to an infinity; mode 2 takes it).  Terms with p = 0 are 0; a row without a live slot has loss and gradient
  *   0, as has a row of weight 0, whose logits are not read; slots that name one token add up.  V <= 2^20, K <= 1024.
  */
 int ltq_distill_topk(const void* logits, int dtype, long long ld, const void* idx, int idx64, long long ld_idx,

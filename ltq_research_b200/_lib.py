@@ -92,7 +92,8 @@ KERNELS_PER_CALL = {
     "ltq_ldlq_inter": 1, "ltq_ldlq_inter3": 1, "ltq_bf16x6_split": 1, "ltq_bf16x6_split_batched": 1,
     "ltq_trtri256_lower": 1, "ltq_chol256_diag": 1, "lut_subs_quant": 1, "ltq_int8_rings": 1, "ltq_matvec_slice": 1,
     "ltq_pack_slice": 1, "ltq_decode_slice": 1,
-    "ltq_distill_topk": lambda a: int(a[13] > 0), "ltq_embed_lookup": lambda a: int(a[5] > 0),
+    "ltq_distill_topk": lambda a: int(a[13] > 0) * (2 if a[17] == 1 else 1),  # loss and gradient: also the rows out of range
+    "ltq_embed_lookup": lambda a: int(a[5] > 0),
     "ltq_embed_grad": lambda a: 3 if a[2] > 8 else (2 if a[2] > 0 else int(not a[13])),
     "ltq_fp8_quant_rows": lambda a: int(a[3] > 0), "ltq_fp8_quant_blocks": lambda a: int(a[3] > 0),
     "ltq_fp8_transpose": 1,

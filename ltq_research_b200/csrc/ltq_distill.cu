@@ -10,10 +10,18 @@
 // so outside the slots the gradient is one factor times exp(z_j / tau), and the K slots are set afterwards.  S_r is summed
 // over the tokens outside the slots (a bitmap of the slots' ids), not taken as S minus the slots, which would cancel.
 //
+// The fast kernels take exponentials relative to a maximum in units of log2, z log2(e) / tau, rounded to fp32.  That holds while
+// the maximum is below BIG in magnitude (what lies below -BIG counts as 0 there).  Where the student has less than 2^-60 of its mass
+// outside the slots (a masked vocabulary), P - p_r / q_r and exponentials relative to the row's maximum would leave fp32's range, and
+// the rest has a maximum of its own.  Other rows (masked with -1e10 or the type's lowest value, very low temperatures) are
+// found by their statistics and done again by exact_row from differences of logits, which are exact where they count.
+//
 // A term with p_k = 0 is 0.  A row of weight 0, or without a live slot, has loss 0 and gradient 0 (weight 0: its logits
 // are not read).  Where q_{id_k} = 0 < p_k the loss is +inf and the gradient finite (q_j = 0).  NaN logits give NaN.
 #include <float.h>
+#include <algorithm>
 #include <atomic>
+#include "launch_next.cuh"
 #include "ltq_b200.h"
 #include "vec_types.cuh"
 
@@ -24,6 +32,9 @@ constexpr int D_THREADS = 256;
 constexpr int D_MAXCL = 8;
 constexpr long long D_ROW = 72 * 1024, D_SLICE = 52 * 1024;  // shared memory for a whole row of one CTA, for a cluster CTA's slice
 constexpr int D_SMEM = 200 * 1024;   // dynamic shared memory of a CTA at most
+constexpr float BIG = 0x1p30f;        // an exponent's rounding error, 2^-25 of it, stays far inside fp32's range
+constexpr uint32_t TO_DO = 0x7fd15711u;  // a NaN that no arithmetic makes: loss of a row that exact_rows_kernel will do
+constexpr float FAR_REST = -60.f;     // log2 q_r below which the rest's gradient is taken relative to the rest's own sum
 constexpr double LOG2E_D = 1.4426950408889634, LN2_D = 0.6931471805599453;
 enum { M_LOSS = 0, M_BOTH = 1, M_GRAD = 2 };
 
@@ -68,12 +79,11 @@ __device__ __forceinline__ void cp_wait()
     asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
 }
 
-// (m, s) <- s 2^m-scaled sums joined: the pair (m, s) stands for s * 2^m
+// (m, s) <- s 2^m-scaled sums joined: the pair (m, s) stands for s * 2^m; m is at least -BIG
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2)
 {
     const float M = fmaxf(m, m2);
-    const float b = M == -INFINITY ? 0.f : M;
-    s = __fmaf_rn(s, ex2(m - b), __fmul_rn(s2, ex2(m2 - b)));
+    s = __fmaf_rn(s, ex2(m - M), __fmul_rn(s2, ex2(m2 - M)));
     m = M;
 }
 
@@ -94,7 +104,7 @@ __device__ __forceinline__ void warp_join(float& m, float& s)
     float M = m;
 #pragma unroll
     for (int o = N / 2; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    s = __fmul_rn(s, ex2(m - (M == -INFINITY ? 0.f : M)));
+    s = __fmul_rn(s, ex2(m - M));
 #pragma unroll
     for (int o = N / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     m = M;
@@ -194,16 +204,19 @@ __device__ __forceinline__ bool leads(const int* id, int k)
     return true;
 }
 
-// what the gradient of a row needs, S = sa 2^ma: outside the slots cr 2^(z c - b), for a slot's token Pq 2^(z c - b) - scale sum p
+// what the gradient of a row needs, S = sa 2^ma: outside the slots cr 2^(z c - br), for a slot's token Pq 2^(z c - b) - scale sum p
 struct GradScale {
-    float scale, Pq, cr, b;
-    __device__ GradScale(float scale_, float psum, float prest, float ma, float sa, float log2qr) : scale(scale_)
+    float scale, Pq, cr, b, br;
+    __device__ GradScale(float scale_, float psum, float prest, float ma, float sa, float log2qr) : scale(scale_), b(ma), br(ma)
     {
-        const float P = psum + prest, inv = sa == 0.f ? 0.f : 1.f / sa;
+        const float P = psum + prest, inv = 1.f / sa;
         Pq = scale * P * inv;
-        // a rest that the student gives nothing has q_j = 0 throughout
-        cr = scale * (prest > 0.f ? (log2qr == -INFINITY ? 0.f : P - prest * ex2(-log2qr)) : P) * inv;
-        b = ma == -INFINITY ? 0.f : ma;
+        cr = scale * (prest > 0.f ? P - prest * ex2(-log2qr) : P) * inv;
+    }
+    // a rest of which the student has so little that p_r / q_r overflows and 2^(z c - b) ends at 0: relative to its own pair (m, s)
+    __device__ void far_rest(float psum, float prest, float log2qr, float m, float s)
+    {
+        br = m, cr = scale * ((psum + prest) * ex2(log2qr) - prest) / s;
     }
 };
 template <typename T>
@@ -233,6 +246,140 @@ __device__ __forceinline__ void zero_slice(const DistillParams& p, const Slice<T
         for (int j = w.j0 + tid; j < w.j1; j += threads) dz[j] = from_f<T>(0.f);
 }
 
+// ------------------------------------------------------------------------------------- rows outside the fast kernels' range
+
+// f(j, z_j) for the tokens of a slice outside the slots, in stretches of a bitmap of `words` words
+template <typename T, typename F>
+__device__ __forceinline__ void over_rest(const Slice<T>& sl, const int* id, int K, uint32_t* bits, int words, F f)
+{
+    constexpr int AHEAD = 8;  // loads in flight
+    for (int a = sl.j0; a < sl.j1; a += 32 * words) {
+        const int n = min(32 * words, sl.j1 - a), step = blockDim.x;
+        for (int i = threadIdx.x; i < (n + 31) / 32; i += step) bits[i] = 0;
+        __syncthreads();
+        for (int k = threadIdx.x; k < K; k += step)
+            if (id[k] >= a && id[k] < a + n) atomicOr(&bits[(id[k] - a) >> 5], 1u << ((id[k] - a) & 31));
+        __syncthreads();
+        for (int j = threadIdx.x; j < n; j += AHEAD * step) {
+            T z[AHEAD];
+#pragma unroll
+            for (int q = 0; q < AHEAD; q++)
+                if (j + q * step < n) z[q] = sl.z[a + j + q * step];
+#pragma unroll
+            for (int q = 0; q < AHEAD; q++) {
+                const int t = j + q * step;
+                if (t < n && !(bits[t >> 5] >> (t & 31) & 1u)) f(a + t, to_f(z[q]));
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// what the kernels find out about the slots of a row
+struct SlotSums {
+    float psum, prest, mt, st;  // sum p, p_r, the pair of the slots' tokens in the slice
+    double plogp, prest64;
+    int dup;  // slots may name one token more than once
+};
+__shared__ SlotSums sums;
+__shared__ float xch[4][D_MAXCL];  // of the row's CTAs
+extern __shared__ __align__(128) uint32_t dsm[];  // bitmap, held slice, then p_k, z and id of the slots
+
+constexpr int PART_WARPS = 16, MIN_BIT_WORDS = 2 * PART_WARPS * 2;
+
+// One row (a CTA's slice of it) whatever its logits' range: sums and gradient from exponentials of differences to the largest logit
+// of the rest, of the slots and of the row, statistics in 64 bits.  Three passes over the row, element by element.  All threads of the row's CTAs come here together, with the slots in shared memory.
+template <typename T, bool REST, int MODE>
+__device__ __forceinline__ void exact_row(const DistillParams& p, long long row)
+{
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5, K = p.K, cl = p.cl;
+    const int rank = cl > 1 ? (int)cluster_rank() : 0;
+    uint32_t* bits = dsm;
+    // the warps' sums, where the bitmap is between two passes
+    double(*dpart)[PART_WARPS] = reinterpret_cast<double(*)[PART_WARPS]>(dsm);
+    float(*part)[PART_WARPS] = reinterpret_cast<float(*)[PART_WARPS]>(dsm);
+    const float* pr = reinterpret_cast<const float*>(dsm + p.bit_words + 4 * p.hold);
+    const float* zk = pr + K;
+    const int* id = reinterpret_cast<const int*>(zk + K);
+    const Slice<T> sl(p, row, rank);
+    const float c = (float)(p.inv_tau_d * LOG2E_D), w = p.weight ? p.weight[row] : 1.f;
+    const double prest = REST ? sums.prest64 : 0.0;
+    auto counts = [&](int k) { return id[k] >= 0 && id[k] >= sl.j0 && id[k] < sl.j1 && (!sums.dup || leads(id, k)); };
+    // four values of each of the row's CTAs to all of them
+    auto exchange = [&](float v0, float v1, float v2, float v3) {
+        const float v[4] = {v0, v1, v2, v3};
+        if (cl > 1) {
+            cluster_arrive(), cluster_wait();  // all CTAs have read what was there
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (tid < cl) st_cluster_u32(&xch[i][rank], tid, __float_as_uint(v[i]));
+            cluster_arrive(), cluster_wait();
+        } else {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (tid == 0) xch[i][0] = v[i];
+            __syncthreads();
+        }
+    };
+    float mr = -INFINITY, mt = -INFINITY;  // the largest logit outside the slots, and in them
+    over_rest(sl, id, K, bits, p.bit_words, [&](int, float z) { mr = fmaxf(mr, z); });
+    for (int k = tid; k < K; k += blockDim.x)
+        if (counts(k)) mt = fmaxf(mt, zk[k]);
+    mr = warp_reduce<0>(mr), mt = warp_reduce<0>(mt);
+    if (lane == 0) part[0][warp] = mr, part[1][warp] = mt;
+    __syncthreads();
+    for (int w = 0; w < warps; w++) mr = fmaxf(mr, part[0][w]), mt = fmaxf(mt, part[1][w]);
+    exchange(mr, mt, 0.f, 0.f);
+    for (int q = 0; q < cl; q++) mr = fmaxf(mr, xch[0][q]), mt = fmaxf(mt, xch[1][q]);
+    const float rr = mr == -INFINITY ? 0.f : mr, rt = mt == -INFINITY ? 0.f : mt;
+    double sr = 0.0, st = 0.0;
+    over_rest(sl, id, K, bits, p.bit_words, [&](int, float z) { sr += ex2(__fmul_rn(z - rr, c)); });
+    for (int k = tid; k < K; k += blockDim.x)
+        if (counts(k)) st += exp2(((double)zk[k] - rt) * c);
+    sr = warp_sum(sr), st = warp_sum(st);
+    if (lane == 0) dpart[0][warp] = sr, dpart[1][warp] = st;
+    __syncthreads();
+    sr = st = 0.0;
+    for (int w = 0; w < warps; w++) sr += dpart[0][w], st += dpart[1][w];
+    exchange((float)sr, (float)(sr - (float)sr), (float)st, (float)(st - (float)st));
+    sr = st = 0.0;
+    for (int q = 0; q < cl; q++) sr += (double)xch[0][q] + xch[1][q], st += (double)xch[2][q] + xch[3][q];
+    // S = s 2^(zm c)
+    const float zm = fmaxf(mr, mt);
+    const double base = zm == -INFINITY ? 0.0 : zm;
+    const double s = sr * exp2(((double)mr - base) * c) + st * exp2(((double)mt - base) * c);
+    const double log2s = zm == -INFINITY ? 0.0 : log2(s);
+    const double log2qr = sr == 0.0 ? -INFINITY : ((double)mr - base) * c + log2(sr) - log2s;
+    if (MODE != M_GRAD && rank == 0 && warp == 0) {
+        double l = 0.0;
+        for (int k = lane; k < K; k += 32)
+            if (!(pr[k] == 0.f)) l = __fma_rn(-(double)pr[k], (((double)zk[k] - base) * c - log2s) * LN2_D, l);
+        l = warp_sum(l) + sums.plogp;
+        if (lane == 0) {
+            if (prest > 0.0) l = __fma_rn(prest, __fma_rn(-log2qr, LN2_D, log(prest)), l);
+            p.loss[row] = (float)__dmul_rn(w, l);
+            // out of range again for the gradient's kernel
+            if (p.stats) p.stats[3 * row] = __fmul_rn(zm, c), p.stats[3 * row + 1] = (float)s, p.stats[3 * row + 2] = (float)log2qr;
+        }
+    }
+    if (MODE == M_LOSS) return;
+    T* dz = (T*)p.dz + row * p.ld_d;
+    const float scale = MODE == M_GRAD ? (p.grad ? p.grad[row * p.s_grad] : 1.f) * w * p.inv_tau : __fmul_rn(w, p.inv_tau);
+    const double P = sums.psum + prest, inv = s == 0.0 ? 0.0 : 1.0 / s;
+    // outside the slots q_j P - p_r q_j / q_r = (q_r P - p_r) q_j / q_r; a rest that the student gives nothing has q_j = 0 throughout
+    const float fr = sr == 0.0 ? 0.f : (float)(scale * (exp2(log2qr) * P - prest) / sr);
+    over_rest(sl, id, K, bits, p.bit_words, [&](int j, float z) { dz[j] = from_f<T>(fr * ex2(__fmul_rn(z - rr, c))); });
+    for (int k = tid; k < K; k += blockDim.x) {
+        if (!counts(k)) continue;
+        double pk = pr[k];
+        if (sums.dup)
+            for (int q = k + 1; q < K; q++)
+                if (id[q] == id[k]) pk += pr[q];
+        dz[id[k]] = from_f<T>((float)(scale * (P * exp2(((double)zk[k] - base) * c) * inv - pk)));
+    }
+}
+
 // Losses, and with GRAD their gradients.  A cluster per row, each CTA a slice of it; with GRAD the slice stays in shared memory
 // between the two passes, so that the row is read from memory once.  Several small CTAs an SM, not one large one: a row has
 // latencies in a chain (its weight, its slots, the sums, the cluster's barrier) and only other rows can fill them.  The last warp
@@ -241,20 +388,16 @@ __device__ __forceinline__ void zero_slice(const DistillParams& p, const Slice<T
 // instructions around it take 60 to 70 % of that time.  4096 x 128256 bf16 with the gradient, a quarter
 // of the rows of weight 0: 384 us, 4.8 TB/s; 2048 rows, the loss alone: 96 us, 5.5 TB/s.
 template <typename T, bool GRAD, bool REST>
-__global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const DistillParams p)
+__global__ void __launch_bounds__(D_THREADS + 32, REST && !GRAD ? 5 : 0) distill_rows_kernel(const __grid_constant__ DistillParams p)
 {
     constexpr int VEC = 16 / sizeof(T), WARPS = D_THREADS / 32, ALL = D_THREADS + 32;
-    extern __shared__ __align__(16) uint32_t dsm[];  // bitmap, held slice, slots
     __shared__ float red[2][WARPS];
-    __shared__ float slot_sums[4];    // sum p, p_r, the pair of the slots' tokens in the slice
-    __shared__ double slot_logs[2];   // sum p log p, p_r
-    __shared__ float xch[4][D_MAXCL];
-    __shared__ int dup;
     uint32_t* bits = dsm;
     float* pr = reinterpret_cast<float*>(dsm + p.bit_words + 4 * p.hold);  // u, then p_k
     float* zk = pr + p.K;  // z of the slot's token (slots of the slice; all of them on the first CTA)
     int* id = reinterpret_cast<int*>(zk + p.K);  // token or -1
     const uint32_t held = (uint32_t)__cvta_generic_to_shared(dsm + p.bit_words);
+    if (GRAD) next_may_start();
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, K = p.K, V = p.V, cl = p.cl;
     const int rank = cl > 1 ? (int)cluster_rank() : 0;
@@ -290,7 +433,7 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
     }
     const int jb = sl.head + (sl.v0 - 1) * VEC;  // element of bit 0: vector v's bits start at (v - v0 + 1) VEC
     for (int i = tid; i < ((nvec + 2) * VEC + 31) / 32; i += ALL) bits[i] = 0;
-    if (tid == 0) dup = 0;
+    if (tid == 0) sums.dup = 0;
     __syncthreads();
     const float c = (float)(p.inv_tau_d * LOG2E_D);
     for (int k = tid; k < K; k += ALL) {
@@ -300,11 +443,11 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
         if (own || (rank == 0 && id0 >= 0)) zk[k] = to_f(sl.z[id0]);
         if (own) {
             const int b = id0 - jb;
-            if (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31) & 1u) dup = 1;
+            if (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31) & 1u) sums.dup = 1;
         }
     }
     __syncthreads();
-    const bool any_dup = dup != 0;
+    const bool any_dup = sums.dup != 0;
 
     const uint64_t cc = pair(c, c);
     auto held_vec = [&](int t) {
@@ -321,7 +464,7 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
     if (warp < WARPS) {
         // One pass: (m, s) with the running maximum, over the tokens outside the slots.  The slots' tokens, which hold most of
         // the mass, are summed apart and in 64 bits.
-        float m = -INFINITY, s;
+        float m = -BIG, s;
         uint64_t s2 = 0;  // two sums, by the elements' parity
         // the bits of this thread's vectors: at a fixed step (and, of four-element vectors, a fixed half of a byte)
         const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bits) + (VEC == 8 ? tid + 1 : (tid + 1) >> 1);
@@ -349,14 +492,12 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
         auto add = [&](uint4 raw, int t) {
             raw = masked(raw, t);
             raise(__fmul_rn(max16(raw, T()), c));
-            const float b = m == -INFINITY ? 0.f : -m;
-            sum(raw, pair(b, b));
+            sum(raw, pair(-m, -m));
         };
         auto add_both = [&](uint4 r0, uint4 r1, int t) {  // vectors t and t + 1, one look at the maximum
             r0 = masked(r0, t), r1 = masked(r1, t + 1);
             raise(__fmul_rn(fmaxf(max16(r0, T()), max16(r1, T())), c));
-            const float b = m == -INFINITY ? 0.f : -m;
-            const uint64_t bb = pair(b, b);
+            const uint64_t bb = pair(-m, -m);
             sum(r0, bb);
             sum(r1, bb);
         };
@@ -385,8 +526,8 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
         s = e.x + e.y;
         auto scalar = [&](int j) {
             if (bits[(j - jb) >> 5] >> ((j - jb) & 31) & 1u) return;
-            const float z = to_f(sl.z[j]), M = fmaxf(m, __fmul_rn(z, c)), b = M == -INFINITY ? 0.f : M;
-            s = __fmaf_rn(s, ex2(m - b), ex2(__fmaf_rn(z, c, -b)));
+            const float z = to_f(sl.z[j]), M = fmaxf(m, __fmul_rn(z, c));
+            s = __fmaf_rn(s, ex2(m - M), ex2(__fmaf_rn(z, c, -M)));
             m = M;
         };
         if (rank == 0 && tid < sl.head) scalar(tid);
@@ -396,22 +537,22 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
     } else {  // the slots' sums
         double psum, prest, plogp, t = 0.0;
         teacher_probabilities<REST>(p, REST ? p.lse[row] : 0.f, pr, id, lane, psum, prest, plogp);
-        float mt = -INFINITY;
+        float mt = -BIG;
         auto counts = [&](int k) { return id[k] >= 0 && id[k] >= sl.j0 && id[k] < sl.j1 && (!any_dup || leads(id, k)); };
         for (int k = lane; k < K; k += 32)
             if (counts(k)) mt = fmaxf(mt, __fmul_rn(zk[k], c));
         mt = warp_reduce<0>(mt);
         for (int k = lane; k < K; k += 32)
-            if (counts(k)) t += exp2(__fma_rn(zk[k], c, mt == -INFINITY ? 0.0 : -(double)mt));
+            if (counts(k)) t += exp2(__fma_rn(zk[k], c, -(double)mt));
         t = warp_sum(t);
         if (lane == 0) {
-            slot_sums[0] = (float)psum, slot_sums[1] = (float)prest, slot_sums[2] = mt, slot_sums[3] = (float)t;
-            slot_logs[0] = plogp, slot_logs[1] = prest;
+            sums.psum = (float)psum, sums.prest = (float)prest, sums.mt = mt, sums.st = (float)t;
+            sums.plogp = plogp, sums.prest64 = prest;
         }
     }
     __syncthreads();
-    const float psum = slot_sums[0], prest = slot_sums[1];
-    float m = red[0][lane & (WARPS - 1)], s = red[1][lane & (WARPS - 1)], mt = slot_sums[2], st = slot_sums[3];
+    const float psum = sums.psum, prest = sums.prest;
+    float m = red[0][lane & (WARPS - 1)], s = red[1][lane & (WARPS - 1)], mt = sums.mt, st = sums.st;
     warp_join<WARPS>(m, s);
     if (cl > 1) {
         cluster_wait();
@@ -433,24 +574,30 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
     float ma = m, sa = s;
     join(ma, sa, mt, st);
     // S = sa 2^ma: the two stay apart, for log2 S itself would be rounded to the size of the logits
-    const float ls = log2f(sa), base = ma == -INFINITY ? 0.f : ma;
-    const float log2qr = !REST || s == 0.f ? -INFINITY : (m - base) + (log2f(s) - ls);
+    const float log2qr = !REST || s == 0.f ? -INFINITY : (m - ma) + (log2f(s) - log2f(sa));
+    // the same for all CTAs of the row: a largest logit, or a rest with some of the teacher's mass, outside the exponents' range
+    if (!(fabsf(ma) < BIG) || (REST && prest > 0.f && s == 0.f)) {
+        if (!GRAD) exact_row<T, REST, M_LOSS>(p, row);
+        else if (rank == 0 && tid == 0) p.loss[row] = __uint_as_float(TO_DO);  // by exact_rows_kernel
+        return;
+    }
     if (rank == 0 && warp == WARPS) {
         double l = 0.0;
-        const double shift = ma == -INFINITY ? 0.0 : (double)base + log2((double)sa);
+        const double shift = (double)ma + log2((double)sa);
         for (int k = lane; k < K; k += 32)
             if (!(pr[k] == 0.f)) l = __fma_rn(-(double)pr[k], __dmul_rn(__fma_rn(zk[k], c, -shift), LN2_D), l);
-        l = warp_sum(l) + slot_logs[0];
+        l = warp_sum(l) + sums.plogp;
         if (lane == 0) {
-            if (slot_logs[1] > 0.0) l = __fma_rn(slot_logs[1], __fma_rn(-(double)log2qr, LN2_D, log(slot_logs[1])), l);
+            if (sums.prest64 > 0.0) l = __fma_rn(sums.prest64, __fma_rn(-(double)log2qr, LN2_D, log(sums.prest64)), l);
             p.loss[row] = (float)__dmul_rn(w, l);
             if (p.stats) p.stats[3 * row] = ma, p.stats[3 * row + 1] = sa, p.stats[3 * row + 2] = log2qr;
         }
     }
     if (GRAD) {
-        const GradScale g(__fmul_rn(w, p.inv_tau), psum, prest, ma, sa, log2qr);
+        GradScale g(__fmul_rn(w, p.inv_tau), psum, prest, ma, sa, log2qr);
+        if (REST && prest > 0.f && log2qr < FAR_REST) g.far_rest(psum, prest, log2qr, m, s);
         if (p.vec_out) {
-            const uint64_t bb = pair(-g.b, -g.b), rr = pair(g.cr, g.cr);
+            const uint64_t bb = pair(-g.br, -g.br), rr = pair(g.cr, g.cr);
             uint4* dt = reinterpret_cast<uint4*>(dz + sl.head) + sl.v0 + tid;
             int t = 0;
 #pragma unroll 2
@@ -458,11 +605,11 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
             // plain loads: the rows may be overwritten (dz = z), each vector by the thread that has read it
 #pragma unroll 4
             for (; t < nt; t++) __stcs(dt + t * D_THREADS, grad16<T>(zt[t * D_THREADS], cc, bb, rr));
-            auto scalar = [&](int j) { dz[j] = from_f<T>(g.cr * ex2(fmaf(to_f(sl.z[j]), c, -g.b))); };
+            auto scalar = [&](int j) { dz[j] = from_f<T>(g.cr * ex2(fmaf(to_f(sl.z[j]), c, -g.br))); };
             if (rank == 0 && tid < sl.head) scalar(tid);
             if (rank == cl - 1 && sl.tail() + tid < V) scalar(sl.tail() + tid);
         } else
-            for (int j = sl.j0 + tid; j < sl.j1; j += ALL) dz[j] = from_f<T>(g.cr * ex2(fmaf(to_f(sl.z[j]), c, -g.b)));
+            for (int j = sl.j0 + tid; j < sl.j1; j += ALL) dz[j] = from_f<T>(g.cr * ex2(fmaf(to_f(sl.z[j]), c, -g.br)));
         __syncthreads();
         for (int k = tid; k < K; k += ALL) {
             if (id[k] < 0 || id[k] < sl.j0 || id[k] >= sl.j1 || (any_dup && !leads(id, k))) continue;
@@ -475,15 +622,62 @@ __global__ void __launch_bounds__(D_THREADS + 32) distill_rows_kernel(const Dist
     }
 }
 
-// the gradient alone, from the statistics: one pass, a CTA per row
+// The slots of a row into shared memory, and p_k, by a CTA that has the whole row.
 template <typename T, bool REST>
-__global__ void __launch_bounds__(D_THREADS) distill_grad_kernel(const DistillParams p)
+__device__ __forceinline__ void load_slots(const DistillParams& p, long long row, const T* z)
 {
-    extern __shared__ __align__(16) uint32_t dsm[];
-    __shared__ float sums[2];
-    float* pr = reinterpret_cast<float*>(dsm);
-    int* id = reinterpret_cast<int*>(pr + p.K);
-    const int tid = threadIdx.x, lane = tid & 31, K = p.K, V = p.V;
+    const int tid = threadIdx.x, K = p.K;
+    float* pr = reinterpret_cast<float*>(dsm + p.bit_words);
+    float* zk = pr + K;
+    int* id = reinterpret_cast<int*>(zk + K);
+    for (int k = tid; k < K; k += blockDim.x) {
+        load_slot(p, row, k, id[k], pr[k]);
+        if (id[k] >= 0) zk[k] = to_f(z[id[k]]);
+    }
+    __syncthreads();
+    if (tid < 32) {
+        double psum, prest, plogp;
+        teacher_probabilities<REST>(p, REST ? p.lse[row] : 0.f, pr, id, tid, psum, prest, plogp);
+        if (tid == 0) sums.psum = (float)psum, sums.prest = (float)prest, sums.plogp = plogp, sums.prest64 = prest, sums.dup = 1;
+    }
+    __syncthreads();
+}
+
+// 4096 x 128256 bf16 with all rows masked by -1e10 outside the slots: 4.2 ms, 0.46 in range; the gradient alone 2.1 ms against 0.40.
+// The rows that the kernel of losses and gradients left to do (their losses hold TO_DO), a CTA each.  A launch of its own, for
+// exact_row inside that kernel makes its fast path slower (4096 x 128256 bf16 386 us: 412 as part of it, 400 as a call; the launch
+// costs 2); the others carry it at no cost.
+template <typename T, bool REST>
+__global__ void __launch_bounds__(D_THREADS) exact_rows_kernel(const __grid_constant__ DistillParams p)
+{
+    __shared__ int found;
+    wait_for_previous();
+    for (long long r0 = blockIdx.x; r0 < p.T; r0 += (long long)D_THREADS * gridDim.x) {
+        const long long mine = r0 + (long long)threadIdx.x * gridDim.x;
+        bool todo = mine < p.T && __float_as_uint(p.loss[mine]) == TO_DO;
+        while (__syncthreads_or(todo)) {
+            if (threadIdx.x == 0) found = D_THREADS;
+            __syncthreads();
+            if (todo) atomicMin(&found, (int)threadIdx.x);
+            __syncthreads();
+            const int f = found;
+            todo = todo && f != (int)threadIdx.x;
+            const long long row = r0 + (long long)f * gridDim.x;
+            load_slots<T, REST>(p, row, (const T*)p.z + row * p.ld);
+            exact_row<T, REST, M_BOTH>(p, row);
+        }
+    }
+}
+
+// the gradient alone, from the statistics: one pass, a CTA per row.  CTAs an SM as many as before exact_row was part of it: 2048 x
+// 128256 bf16 215 us, 226 with the registers that it would take
+template <typename T, bool REST>
+__global__ void __launch_bounds__(D_THREADS, sizeof(T) == 4 ? 6 : 5) distill_grad_kernel(const __grid_constant__ DistillParams p)
+{
+    float* pr = reinterpret_cast<float*>(dsm + p.bit_words);
+    float* zk = pr + p.K;
+    int* id = reinterpret_cast<int*>(zk + p.K);
+    const int tid = threadIdx.x, K = p.K, V = p.V;
     const long long row = blockIdx.x;
     const Slice<T> sl(p, row, 0);
     T* dz = (T*)p.dz + row * p.ld_d;
@@ -493,22 +687,16 @@ __global__ void __launch_bounds__(D_THREADS) distill_grad_kernel(const DistillPa
         return;
     }
     const float c = (float)(p.inv_tau_d * LOG2E_D);
-    float* zk = reinterpret_cast<float*>(id + K);
-    for (int k = tid; k < K; k += D_THREADS) {
-        load_slot(p, row, k, id[k], pr[k]);
-        if (id[k] >= 0) zk[k] = to_f(sl.z[id[k]]);
-    }
-    __syncthreads();
-    if (tid < 32) {
-        double psum, prest, plogp;
-        teacher_probabilities<REST>(p, REST ? p.lse[row] : 0.f, pr, id, lane, psum, prest, plogp);
-        if (lane == 0) sums[0] = (float)psum, sums[1] = (float)prest;
-    }
-    __syncthreads();
+    load_slots<T, REST>(p, row, sl.z);
     const float up = p.grad ? p.grad[row * p.s_grad] : 1.f;
-    const GradScale g(up * w * p.inv_tau, sums[0], sums[1], p.stats[3 * row], p.stats[3 * row + 1], p.stats[3 * row + 2]);
+    const float scale = up * w * p.inv_tau, ma = p.stats[3 * row], log2qr = p.stats[3 * row + 2];
+    if (!(fabsf(ma) < BIG) || (REST && sums.prest > 0.f && log2qr < FAR_REST)) {  // the statistics do not hold the rest's own pair
+        exact_row<T, REST, M_GRAD>(p, row);
+        return;
+    }
+    const GradScale g(scale, sums.psum, sums.prest, ma, p.stats[3 * row + 1], log2qr);
     if (p.vec_out) {
-        const uint64_t cc = pair(c, c), bb = pair(-g.b, -g.b), rr = pair(g.cr, g.cr);
+        const uint64_t cc = pair(c, c), bb = pair(-g.br, -g.br), rr = pair(g.cr, g.cr);
         // plain loads: the rows may be overwritten (dz = z), each vector by the thread that has read it
         const uint4* zt = reinterpret_cast<const uint4*>(sl.z + sl.head);
         uint4* dt = reinterpret_cast<uint4*>(dz + sl.head);
@@ -521,11 +709,11 @@ __global__ void __launch_bounds__(D_THREADS) distill_grad_kernel(const DistillPa
             for (int q = 0; q < 4; q++) __stcs(dt + v + q * D_THREADS, grad16<T>(u[q], cc, bb, rr));
         }
         for (; v < sl.nb; v += D_THREADS) __stcs(dt + v, grad16<T>(zt[v], cc, bb, rr));
-        auto scalar = [&](int j) { dz[j] = from_f<T>(g.cr * ex2(fmaf(to_f(sl.z[j]), c, -g.b))); };
+        auto scalar = [&](int j) { dz[j] = from_f<T>(g.cr * ex2(fmaf(to_f(sl.z[j]), c, -g.br))); };
         if (tid < sl.head) scalar(tid);
         if (sl.tail() + tid < V) scalar(sl.tail() + tid);
     } else
-        for (int j = tid; j < V; j += D_THREADS) dz[j] = from_f<T>(g.cr * ex2(fmaf(to_f(sl.z[j]), c, -g.b)));
+        for (int j = tid; j < V; j += D_THREADS) dz[j] = from_f<T>(g.cr * ex2(fmaf(to_f(sl.z[j]), c, -g.br)));
     __syncthreads();
     for (int k = tid; k < K; k += D_THREADS) {
         if (id[k] < 0 || !leads(id, k)) continue;
@@ -547,6 +735,11 @@ int row_ctas(long long T, int V, int es, bool grad)
     return cl < D_MAXCL ? cl : D_MAXCL;
 }
 
+// for kernels whose CTAs have whole rows and hold nothing of them but the slots
+constexpr int WHOLE_BITS = 1024;  // words of exact_row's bitmap
+void whole_row(DistillParams& p) { p.cl = 1, p.bit_words = WHOLE_BITS, p.hold = 0; }
+int slots_smem(int K) { return WHOLE_BITS * 4 + K * 12; }
+
 template <typename T, bool GRAD, bool REST>
 int launch_rows(DistillParams p, cudaStream_t st)
 {
@@ -554,7 +747,8 @@ int launch_rows(DistillParams p, cudaStream_t st)
     auto k = distill_rows_kernel<T, GRAD, REST>;
     p.cl = row_ctas(p.T, p.V, sizeof(T), GRAD);
     const int per = (p.V / VEC + p.cl - 1) / p.cl;
-    p.bit_words = (((per + 2) * VEC + 31) / 32 + 3) / 4 * 4;
+    // whole 256 bytes: 1024 x 128256 fp32 226 us, up to 250 when the held slice behind them begins elsewhere
+    p.bit_words = (((per + 2) * VEC + 31) / 32 + MIN_BIT_WORDS - 1) / MIN_BIT_WORDS * MIN_BIT_WORDS;
     const int fixed = p.bit_words * 4 + p.K * 12;
     p.hold = GRAD ? per : 0;
     if (fixed + p.hold * 16 > D_SMEM) p.hold = (D_SMEM - fixed) / 16;
@@ -579,14 +773,17 @@ int launch_rows(DistillParams p, cudaStream_t st)
     at[0].val.clusterDim = {(unsigned)p.cl, 1, 1};
     cfg.attrs = at;
     cfg.numAttrs = p.cl > 1 ? 1 : 0;
-    return (int)cudaLaunchKernelEx(&cfg, k, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k, p);
+    if (!GRAD || e != cudaSuccess) return (int)e;
+    whole_row(p);
+    return (int)launch_next(exact_rows_kernel<T, REST>, std::min(p.T, 296), D_THREADS, slots_smem(p.K), st, p);
 }
 
 template <typename T, bool REST>
 int launch_grad(DistillParams p, cudaStream_t st)
 {
-    p.cl = 1;
-    distill_grad_kernel<T, REST><<<p.T, D_THREADS, p.K * 12, st>>>(p);
+    whole_row(p);
+    distill_grad_kernel<T, REST><<<p.T, D_THREADS, slots_smem(p.K), st>>>(p);
     return (int)cudaGetLastError();
 }
 

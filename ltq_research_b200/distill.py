@@ -11,9 +11,10 @@ For a row of student logits z [V] and a teacher's K kept logits u_k of tokens id
 
 A slot whose id is negative (or not below V) is empty.  Rows of weight 0 (prompt positions, padding) have loss and
 gradient 0 and their logits are not read; a row without a live slot has loss and gradient 0; a kept token that the student
-excludes (logit -inf) gives loss +inf and a finite gradient; NaN logits give NaN.  Sums and statistics are fp32.
+excludes (logit -inf) gives loss +inf and a finite gradient; NaN logits give NaN.  Finite logits of any size are taken as they
+are: a vocabulary masked with -1e4, -1e30 or the type's lowest value has its share of the loss and of the gradient.
 
-One kernel (ltq_distill_topk): the loss reads the logits once, loss and gradient together read them once more from cache
+One entry (ltq_distill_topk): the loss reads the logits once, loss and gradient together read them once more from cache
 or shared memory and write the gradient.  There is no CPU path.
 """
 from __future__ import annotations
@@ -130,7 +131,8 @@ def topk_loss(logits: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor, *,
               teacher_lse: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
               temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
     """(loss [T], stats [T, 3]) of logits [T, V] against teacher [T, K] at the tokens idx [T, K].  stats = (m, s, r), which
-    topk_grad takes: the student's sum of exponentials is s 2^m, its mass outside the slots 2^r."""
+    topk_grad takes: the student's sum of exponentials is s 2^m, its mass outside the slots 2^r (m may round to an infinity in
+    rows of logits beyond 2^29 temperature)."""
     loss, stats, _ = _call(logits, idx, teacher, teacher_lse, weight, temperature, LOSS, want_stats=True)
     return loss, stats
 
@@ -138,7 +140,7 @@ def topk_loss(logits: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor, *,
 def topk_loss_grad(logits: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor, *,
                    teacher_lse: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
                    temperature: float = 1.0, out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(loss [T], d sum(loss) / d logits [T, V] in the logits' type), in one kernel.  A mean or any other weighting goes
+    """(loss [T], d sum(loss) / d logits [T, V] in the logits' type), in one call.  A mean or any other weighting goes
     into `weight`.  out may be `logits` itself, which the gradient then replaces."""
     loss, _, d = _call(logits, idx, teacher, teacher_lse, weight, temperature, LOSS_AND_GRAD, out=out)
     return loss, d

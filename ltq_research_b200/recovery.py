@@ -59,7 +59,7 @@ def step(table: torch.Tensor, tokens: torch.Tensor, body: Callable, head: fp8.Bl
          scale: float = 1.0, temperature: float = 1.0, weight: Optional[torch.Tensor] = None,
          padding_idx: Optional[int] = None) -> torch.Tensor:
     """Mean divergence over the weighted positions; leaves its gradient in table.grad (added to what is there) and in
-    whatever of `body` asks for one.  The loss and the logits' gradient come from one kernel that writes the gradient over
+    whatever of `body` asks for one.  The loss and the logits' gradient come from one call that writes the gradient over
     the logits."""
     if not table.requires_grad:
         raise ValueError("recovery.step: the table must require a gradient")

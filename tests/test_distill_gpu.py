@@ -174,6 +174,124 @@ def test_student_gives_the_rest_nothing():
     loss, d = distill.topk_loss_grad(logits, idx, u, teacher_lse=lse)
     assert loss[0] == math.inf and torch.isfinite(d).all() and not d[0, rest].any()
 
+def in_logs(logits, idx, teacher, lse=None, weight=None, tau=1.0):
+    """Loss and gradient from the definition in 64 bits and in logarithms of probabilities, so that no mass of the student is too
+    small; and the gradient's parts (q_j P, p_j and the rest's spread), of which each is rounded by itself."""
+    T, V = logits.shape
+    z = logits.double().cpu() / tau
+    idx, u = idx.cpu().long(), teacher.double().cpu() / tau
+    live = (idx >= 0) & (idx < V)
+    at = torch.where(live, idx, torch.zeros_like(idx))
+    p = torch.exp(u - lse.double().cpu()[:, None]) if lse is not None else torch.softmax(u.masked_fill(~live, -math.inf), 1)
+    p = torch.where(live, p, torch.zeros_like(p))
+    rest = (1 - p.sum(1)).clamp(min=0) if lse is not None else torch.zeros(T, dtype=torch.float64)
+    top = torch.zeros(T, V, dtype=torch.float64).scatter_add_(1, at, live.double()) > 0
+    first = z.amax(1, keepdim=True)  # differences before anything else: z may be 1e30
+    log_s = torch.log(torch.exp(z - first).sum(1, keepdim=True))
+    log_q = z - first - log_s
+    z_r = z.masked_fill(top, -math.inf)
+    first_r = z_r.amax(1, keepdim=True)
+    e_r = torch.exp(z_r - torch.where(first_r > -math.inf, first_r, torch.zeros_like(first_r)))
+    s_r = e_r.sum(1, keepdim=True)
+    log_r = (first_r - first + torch.log(s_r) - log_s)[:, 0]
+    w = torch.ones(T, dtype=torch.float64) if weight is None else weight.double().cpu()
+    row = torch.where(p > 0, p * (torch.log(p) - log_q.gather(1, at)), torch.zeros_like(p)).sum(1)
+    row += torch.where(rest > 0, rest * (torch.log(rest) - log_r), torch.zeros_like(rest))
+    target = torch.zeros(T, V, dtype=torch.float64).scatter_add_(1, at, p)
+    spread = torch.where((s_r == 0) | (rest == 0)[:, None], torch.zeros_like(z), e_r / s_r * rest[:, None])
+    own = log_q.exp() * (p.sum(1) + rest)[:, None]
+    return w * row, (own - target - spread) * (w / tau)[:, None], (own + target + spread) * (w / tau)[:, None].abs(), top
+
+
+def check_logs(logits, idx, teacher, lse=None, tau=1.0):
+    """The fused form, the loss alone and the gradient alone against in_logs.  An exponent of at most 126 in fp32 is good to 126
+    2^-24 = 7.5e-6, so an exponential, a sum of them and a part of the gradient to 2e-5 of itself (what is below 2^-100 counts as
+    0: exponentials end at 2^-126); a loss to 4e-7 of itself besides the 1e-4 above."""
+    want_l, want_d, parts, _ = in_logs(logits, idx, teacher, lse, None, tau)
+    kw = dict(teacher_lse=lse, temperature=tau)
+    loss, d = distill.topk_loss_grad(logits, idx, teacher, **kw)
+    loss0, stats = distill.topk_loss(logits, idx, teacher, **kw)
+    assert torch.equal(loss, loss0)
+    limit = torch.finfo(torch.float32).max
+    inf = want_l.abs() > limit
+    assert torch.equal(torch.isinf(loss.cpu()), inf) and not torch.isnan(loss).any()
+    assert bool(((loss.double().cpu() - want_l).abs() <= 1e-4 + 4e-7 * want_l.abs())[~inf].all())
+    out = torch.empty_like(logits)
+    for g in (d, distill.topk_grad(logits, idx, teacher, stats, **kw),
+              distill.topk_loss_grad(logits, idx, teacher, out=out.copy_(logits), **kw)[1],
+              distill.topk_grad(out.copy_(logits), idx, teacher, stats, out=out, **kw)):
+        g = g.double().cpu()
+        assert torch.isfinite(g).all()
+        tol = 2e-5 * parts + HALF_ULP[logits.dtype] * 1.01 * want_d.abs() + 2.0 ** -100 / tau
+        tol += 2.0 ** -25 if logits.dtype == torch.float16 else 0
+        assert bool(((g - want_d).abs() <= tol).all()), float(((g - want_d).abs() / tol).max())
+
+
+def far(T, V, K, dtype, at, seed, share=0.3, spread=1.0):
+    """Rows whose tokens outside the slots all lie near `at`, while the teacher leaves them `share` of its mass."""
+    g = torch.Generator().manual_seed(seed)
+    idx = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(T)])
+    z = at + spread * torch.randn(T, V, generator=g)
+    z = z.clamp(min=torch.finfo(dtype).min).scatter_(1, idx, torch.randn(T, K, generator=g) * 3)
+    u = torch.randn(T, K, generator=g) * 2
+    lse = torch.logsumexp(u, 1) - math.log(1 - share)
+    return z.to(dtype).cuda(), idx.cuda(), u.cuda(), lse.cuda()
+
+
+FAR = [-40.0, -60.0, -85.0, -100.0, -1e4, -1e9, -1e10, -1e30, -3e38]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("at", FAR)
+def test_rest_far_below_the_slots(at, dtype):
+    """A vocabulary masked with a finite value, the slots' tokens alone allowed: the teacher's remaining mass is spread over the
+    rest, however small the student's own mass there is."""
+    if dtype == torch.float16 and at < -65000.0:
+        at = -65504.0
+    for share in (0.3, 2e-7):
+        check_logs(*far(3, 301, 5, dtype, at, seed=21, share=share))
+    check_logs(*far(2, 40003, 40, dtype, at, seed=22))
+
+
+@pytest.mark.parametrize("at", [-85.0, -1e4, -1e30])
+def test_rest_far_below_the_slots_in_long_rows(at):
+    check_logs(*far(40, 128256, 20, torch.bfloat16, at, seed=23))
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("mask", [-1e4, -1e10, -1e30, -3.3e38])
+def test_vocabulary_masked_with_a_large_number(mask, dtype, rest):
+    """Most tokens masked, so that whole threads' and CTAs' shares of a row are; a few left, in the slots and beside them."""
+    mask = max(mask, torch.finfo(dtype).min)
+    for V, keep in ((3001, 12), (60000, 40)):
+        logits, idx, u, lse = make(4, V, 6, dtype, seed=24, rest=rest)
+        allowed = torch.zeros(4, V, dtype=torch.bool, device="cuda").scatter_(1, idx, True)
+        allowed[:, torch.randperm(V, generator=torch.Generator().manual_seed(25))[:keep].cuda()] = True
+        logits.copy_(torch.where(allowed, logits, torch.full_like(logits, mask)))
+        check_logs(logits, idx, u, lse)
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("at", [-3e38, -1e30, -4e9, 3e9, 1e30])
+def test_rows_of_large_numbers(at, rest):
+    """All logits far from 0, equal ones and ones that differ by units of their type."""
+    logits, idx, u, lse = make(3, 2100, 9, torch.float32, seed=26, rest=rest)
+    z = torch.full_like(logits, at)
+    z[1] *= 1 + 2.0 ** -23 * torch.randint(0, 2, (2100,), device="cuda", generator=torch.Generator("cuda").manual_seed(27))
+    z[2, idx[2, :3]] = 0.9 * at
+    check_logs(z, idx, u, lse)
+
+
+@pytest.mark.parametrize("rest", [False, True])
+def test_low_temperature(rest):
+    logits, idx, u, lse = make(4, 1500, 8, torch.float32, seed=28, rest=False)
+    tau = 2.0 ** -30  # a value of fp32, in which the temperature is held
+    if rest:
+        lse = (torch.logsumexp(u.double() / tau, 1) + 0.4).float()
+        lse = torch.where(lse.double() < u.double().amax(1) / tau, torch.nextafter(lse, torch.full_like(lse, math.inf)), lse)
+    check_logs(logits, idx, u, lse, tau=tau)
+
 
 def test_nan_reaches_its_row_only():
     logits, idx, u, lse = make(3, 700, 4, torch.bfloat16, seed=11)
