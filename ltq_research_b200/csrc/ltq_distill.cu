@@ -154,8 +154,9 @@ __device__ __forceinline__ F warp_sum(F v)
     return v;
 }
 
-// p_k into pr (from u) on one warp; returns P's two parts and sum p log p.  In 64 bits: p_r is what the others leave of 1, and the
-// loss is small beside its terms; K exponentials on one warp while the others read the row cost no time.
+// p_k into pr (from u) on one warp, rounded to fp32; returns P's two parts and sum p log p.  In 64 bits: p_r is what the others leave
+// of 1, and the loss is small beside its terms, so both of its sums take the same rounded p (a student that equals its teacher had
+// losses of 3e-7 otherwise); K exponentials on one warp while the others read the row cost no time.
 template <bool REST>
 __device__ __forceinline__ void teacher_probabilities(const DistillParams& p, float lse, float* pr, const int* id, int lane,
                                                       double& psum, double& prest, double& plogp)
@@ -180,7 +181,7 @@ __device__ __forceinline__ void teacher_probabilities(const DistillParams& p, fl
             const double lp = __fma_rn(pr[k], p.inv_tau_d, -um) - lt;
             pk = exp(lp);
             psum += pk;
-            if (!(pk == 0.0)) plogp = __fma_rn(pk, lp, plogp);
+            if (!((float)pk == 0.f)) plogp = __fma_rn((double)(float)pk, lp, plogp);  // p as it is held and meets log q
             if (REST && K >= p.V) {
                 bool first = true;
                 for (int q = 0; q < k && first; q++) first = id[q] != id[k];

@@ -13,6 +13,8 @@ A slot whose id is negative (or not below V) is empty.  Rows of weight 0 (prompt
 gradient 0 and their logits are not read; a row without a live slot has loss and gradient 0; a kept token that the student
 excludes (logit -inf) gives loss +inf and a finite gradient; NaN logits give NaN.  Finite logits of any size are taken as they
 are: a vocabulary masked with -1e4, -1e30 or the type's lowest value has its share of the loss and of the gradient.
+Exponentials and sums over the vocabulary are fp32; the teacher's probabilities, the slots' sums and the loss are formed in 64
+bits from p rounded to fp32.
 
 One entry (ltq_distill_topk): the loss reads the logits once, loss and gradient together read them once more from cache
 or shared memory and write the gradient.  There is no CPU path.

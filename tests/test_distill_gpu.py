@@ -293,6 +293,24 @@ def test_low_temperature(rest):
     check_logs(logits, idx, u, lse, tau=tau)
 
 
+@pytest.mark.parametrize("K", [2, 10, 100, 777, 1000])
+@pytest.mark.parametrize("spread", [0.0, 3.0])
+def test_student_that_equals_its_teacher(K, spread):
+    """The loss is 0 but for the rounding of the student's sum to fp32 (twice half a unit, 2^-24) and that of p's sum."""
+    z = spread * torch.randn(3, K, generator=torch.Generator().manual_seed(K))
+    idx = torch.arange(K, device="cuda").repeat(3, 1)
+    loss = distill.topk_loss(z.cuda(), idx, z.cuda())[0]
+    assert float(loss.abs().max()) <= 2.0 ** -23
+
+
+def test_student_that_equals_its_teacher_with_a_rest():
+    """2^-22 from the exponentials of the rest and as much from their sums in fp32."""
+    z = 2 * torch.randn(5, 5000, generator=torch.Generator().manual_seed(3))
+    u, idx = z.topk(64, 1)
+    loss = distill.topk_loss(z.cuda(), idx.cuda(), u.cuda(), teacher_lse=torch.logsumexp(z.double(), 1).float().cuda())[0]
+    assert float(loss.abs().max()) <= 2.0 ** -21
+
+
 def test_nan_reaches_its_row_only():
     logits, idx, u, lse = make(3, 700, 4, torch.bfloat16, seed=11)
     logits[1, 690] = float("nan")
