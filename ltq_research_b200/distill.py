@@ -156,6 +156,19 @@ def topk_grad(logits: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor, st
     return _call(logits, idx, teacher, teacher_lse, weight, temperature, GRAD, stats=stats, grad=grad, out=out)[2]
 
 
+class _TopkGrad(torch.autograd.Function):
+    """topk_grad within a backward pass.  It depends on the logits as well as on the upstream gradient, so the graph of a gradient
+    (create_graph=True) ends in a node that refuses, whatever the upstream gradient is."""
+
+    @staticmethod
+    def forward(ctx, logits, idx, teacher, teacher_lse, weight, stats, grad, temperature):
+        return topk_grad(logits, idx, teacher, stats, grad=grad, teacher_lse=teacher_lse, weight=weight, temperature=temperature)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("distill: the divergence has no second derivatives")
+
+
 class _TopkLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, idx, teacher, teacher_lse, weight, temperature):
@@ -167,8 +180,7 @@ class _TopkLoss(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         logits, idx, teacher, teacher_lse, weight, stats = ctx.saved_tensors
-        d = topk_grad(logits, idx, teacher, stats, grad=grad, teacher_lse=teacher_lse, weight=weight,
-                      temperature=ctx.temperature)
+        d = _TopkGrad.apply(logits, idx, teacher, teacher_lse, weight, stats, grad, ctx.temperature)
         return d, None, None, None, None, None
 
 
@@ -176,5 +188,5 @@ def distill_loss(logits: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor,
                  teacher_lse: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
                  temperature: float = 1.0) -> torch.Tensor:
     """topk_loss as a node of torch's autograd graph: loss [T], differentiable by the logits (the teacher and the weights
-    are constants).  The backward pass reads the logits again and runs topk_grad."""
+    are constants).  The backward pass reads the logits again and runs topk_grad; a second derivative raises RuntimeError."""
     return _TopkLoss.apply(logits, idx, teacher, teacher_lse, weight, temperature)

@@ -104,6 +104,18 @@ def lookup_grad(tokens: torch.Tensor, dout: torch.Tensor, num_rows: int, scale: 
     return out
 
 
+class _LookupGrad(torch.autograd.Function):
+    """lookup_grad within a backward pass: in the graph of a gradient (create_graph=True) a node that refuses."""
+
+    @staticmethod
+    def forward(ctx, tokens, dout, rows, scale, padding_idx, dtype):
+        return lookup_grad(tokens, dout, rows, scale, padding_idx, dtype=dtype)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("embedding: the lookup's gradient is not differentiable by dout")
+
+
 class _Lookup(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, tokens, scale, padding_idx):
@@ -113,11 +125,11 @@ class _Lookup(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
-        rows, scale, padding_idx, dtype = ctx.args
-        return lookup_grad(ctx.saved_tensors[0], dout, rows, scale, padding_idx, dtype=dtype), None, None, None
+        return _LookupGrad.apply(ctx.saved_tensors[0], dout, *ctx.args), None, None, None
 
 
 def embed(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
           padding_idx: Optional[int] = None) -> torch.Tensor:
-    """lookup as a node of torch's autograd graph: the table's gradient is lookup_grad's, in the table's type."""
+    """lookup as a node of torch's autograd graph: the table's gradient is lookup_grad's, in the table's type; a second
+    derivative (a dout that depends on what is differentiated by) raises RuntimeError."""
     return _Lookup.apply(table, tokens, scale, padding_idx)

@@ -197,6 +197,18 @@ def check_errors(device):
     check_gemm_errors(device)
 
 
+class _LinearGrad(torch.autograd.Function):
+    """linear_grad within a backward pass: in the graph of a gradient (create_graph=True) a node that refuses."""
+
+    @staticmethod
+    def forward(ctx, dy, W, dtype):
+        return linear_grad(dy, W, dtype)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("fp8: the product's gradient is not differentiable by dy")
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, W):
@@ -206,9 +218,10 @@ class _Linear(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return linear_grad(dy, ctx.W, ctx.dtype), None
+        return _LinearGrad.apply(dy, ctx.W, ctx.dtype), None
 
 
 def block_linear(x: torch.Tensor, W: BlockWeight) -> torch.Tensor:
-    """linear as a node of torch's autograd graph; the gradient by x is linear_grad's (W made with backward=True)."""
+    """linear as a node of torch's autograd graph; the gradient by x is linear_grad's (W made with backward=True); a second
+    derivative (a dy that depends on what is differentiated by) raises RuntimeError."""
     return _Linear.apply(x, W)

@@ -405,6 +405,16 @@ def test_autograd():
     assert (z.grad - want).abs().max() < 1e-6
 
 
+@pytest.mark.parametrize("upstream", ["constant", "dependent"])
+def test_second_derivatives_are_refused(upstream):
+    logits, idx, u, lse = make(4, 200, 5, torch.float32, seed=29)
+    a = logits.clone().requires_grad_()
+    loss = distill.distill_loss(a * a.detach().abs(), idx, u, teacher_lse=lse)
+    g, = torch.autograd.grad(loss.sum() if upstream == "constant" else loss.square().sum(), a, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(g.square().sum() + a.square().sum(), a)
+
+
 def test_no_rows():
     loss, d = distill.topk_loss_grad(torch.empty(0, 9, device="cuda"), torch.empty(0, 2, dtype=torch.int64, device="cuda"),
                                      torch.empty(0, 2, device="cuda"))

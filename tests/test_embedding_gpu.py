@@ -258,6 +258,14 @@ def test_grad_of_many_positions_again_and_again(n, V):
         assert torch.equal(embedding.lookup_grad(tok, dout, V), want)
 
 
+def test_second_derivatives_are_refused():
+    table = torch.randn(20, 16, device="cuda", generator=gen(10)).requires_grad_()
+    y = embedding.embed(table, torch.arange(9, device="cuda"))
+    g, = torch.autograd.grad(y.pow(3).sum(), table, create_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(g.square().sum() + table.square().sum(), table)
+
+
 def test_refusals():
     table = torch.zeros(10, 8, device="cuda")
     tok = torch.zeros(3, dtype=torch.int64, device="cuda")

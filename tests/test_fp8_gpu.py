@@ -279,6 +279,15 @@ def test_autograd():
     check(dy, W, x.grad, grad=True)
 
 
+def test_second_derivatives_are_refused():
+    g = gen(13)
+    W = fp8.BlockWeight.quantize(torch.randn(40, 96, device="cuda", generator=g), backward=True)
+    x = torch.randn(3, 96, device="cuda", generator=g).requires_grad_()
+    d, = torch.autograd.grad(fp8.block_linear(x, W).pow(3).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(d.square().sum() + x.square().sum(), x)
+
+
 def test_refusals():
     w = torch.randn(130, 200, device="cuda")
     q, s = fp8.quantize_blocks(w)
