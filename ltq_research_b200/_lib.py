@@ -182,6 +182,11 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
     return dev
 
 
+def written(t: torch.Tensor):
+    """Tells autograd that a kernel has written a tensor of the caller's: whoever saved what it held before gets torch's error."""
+    torch.autograd.graph.increment_version(t)
+
+
 def on_device(device: torch.device):
     """Context with `device` current, as a launch on its streams needs."""
     return _SAME if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)

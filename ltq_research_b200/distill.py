@@ -118,6 +118,8 @@ def _call(logits, idx, teacher, teacher_lse, weight, temperature, mode, stats=No
             ptr(dlogits), ld_d, _lib.stream_ptr(dev))
     if rc != 0:
         raise RuntimeError(f"ltq_distill_topk: error code {rc}")
+    if out is not None:
+        _lib.written(out)
     return loss, stats, dlogits
 
 

@@ -50,7 +50,8 @@ def lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
     if V < 1:
         raise ValueError("embedding: the table has no rows")
     tok = _tokens(tokens)
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((*tokens.shape, D), dtype=table.dtype, device=dev)
     elif out.dtype != table.dtype or out.shape != (*tokens.shape, D) or not out.is_contiguous():
         raise ValueError("embedding: out must be contiguous, of the table's type and shape [*tokens.shape, D]")
@@ -59,6 +60,8 @@ def lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
                                          scale, out.data_ptr(), D, _lib.stream_ptr(dev))
     if rc != 0:
         raise RuntimeError(f"ltq_embed_lookup: error code {rc}")
+    if given:
+        _lib.written(out)
     return out
 
 
@@ -84,7 +87,8 @@ def lookup_grad(tokens: torch.Tensor, dout: torch.Tensor, num_rows: int, scale: 
     if d.shape[0] > 1 and (d.stride(0) < D or (D > 1 and d.stride(1) != 1)) or (D > 1 and d.stride(1) != 1):
         d = d.contiguous()  # a gradient that autograd expanded
     ld_d = _row_stride(d, "dout")
-    if out is None:
+    given = out is not None
+    if not given:
         if accumulate:
             raise ValueError("embedding: accumulate needs the tensor to add to")
         out = torch.empty((num_rows, D), dtype=dtype, device=dev)
@@ -101,6 +105,8 @@ def lookup_grad(tokens: torch.Tensor, dout: torch.Tensor, num_rows: int, scale: 
                               _lib.stream_ptr(dev))
     if rc != 0:
         raise RuntimeError(f"ltq_embed_grad: error code {rc}")
+    if given:
+        _lib.written(out)
     return out
 
 

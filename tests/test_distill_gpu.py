@@ -405,6 +405,20 @@ def test_autograd():
     assert (z.grad - want).abs().max() < 1e-6
 
 
+@pytest.mark.parametrize("form", ["both", "gradient"])
+def test_outputs_written_in_place_tell_autograd(form):
+    logits, idx, u, lse = make(3, 300, 4, torch.float32, seed=30)
+    a = logits.clone().requires_grad_()
+    z = a.exp()  # keeps its result for the backward pass
+    stats = distill.topk_loss(z.detach(), idx, u, teacher_lse=lse)[1]
+    if form == "both":
+        distill.topk_loss_grad(z.detach(), idx, u, teacher_lse=lse, out=z.detach())
+    else:
+        distill.topk_grad(z.detach(), idx, u, stats, teacher_lse=lse, out=z.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+
+
 @pytest.mark.parametrize("upstream", ["constant", "dependent"])
 def test_second_derivatives_are_refused(upstream):
     logits, idx, u, lse = make(4, 200, 5, torch.float32, seed=29)

@@ -258,6 +258,19 @@ def test_grad_of_many_positions_again_and_again(n, V):
         assert torch.equal(embedding.lookup_grad(tok, dout, V), want)
 
 
+@pytest.mark.parametrize("form", ["lookup", "gradient", "accumulated"])
+def test_outputs_written_in_place_tell_autograd(form):
+    a = torch.randn(6, 16, device="cuda", generator=gen(11)).requires_grad_()
+    y = a.exp()  # keeps its result for the backward pass
+    table, tok = torch.randn(20, 16, device="cuda", generator=gen(12)), torch.arange(6, device="cuda")
+    if form == "lookup":
+        embedding.lookup(table, tok, out=y.detach())
+    else:
+        embedding.lookup_grad(tok, table[:6], 6, out=y.detach(), accumulate=form == "accumulated")
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_second_derivatives_are_refused():
     table = torch.randn(20, 16, device="cuda", generator=gen(10)).requires_grad_()
     y = embedding.embed(table, torch.arange(9, device="cuda"))
