@@ -110,6 +110,7 @@ class BlockWeight:
         self.q, self.s = self._lay(q), s.contiguous()  # before the transpose, which reads them
         self.qt = self._transposed(N, K) if backward else None
         self.st = s.t().contiguous() if backward else None
+        _error_flag(self.device)  # made (which synchronises) here, so that the first product may be captured into a graph
 
     @classmethod
     def quantize(cls, w: torch.Tensor, backward: bool = False) -> "BlockWeight":

@@ -279,6 +279,24 @@ def test_autograd():
     check(dy, W, x.grad, grad=True)
 
 
+@pytest.mark.parametrize("M", [3, 40])
+def test_first_product_in_a_graph(M):
+    """No call before the capture: what a first product needs once is there with the weight."""
+    from ltq_research_b200 import liqk_v2
+    torch.cuda.synchronize()
+    fp8._FLAGS.clear()
+    liqk_v2._GEMM_ERR.clear()
+    g = gen(14)
+    W = fp8.BlockWeight.quantize(torch.randn(300, 512, device="cuda", generator=g), backward=True)
+    x, dy = torch.randn(M, 512, device="cuda", generator=g), torch.randn(M, 300, device="cuda", generator=g)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, dx = fp8.linear(x, W), fp8.linear_grad(dy, W)
+    graph.replay()
+    assert torch.equal(y, fp8.linear(x, W)) and torch.equal(dx, fp8.linear_grad(dy, W))
+    fp8.check_errors(x.device)
+
+
 def test_second_derivatives_are_refused():
     g = gen(13)
     W = fp8.BlockWeight.quantize(torch.randn(40, 96, device="cuda", generator=g), backward=True)
