@@ -431,13 +431,18 @@ def _rows_ldlq(W_rot: torch.Tensor, U: torch.Tensor, U_blks_inv: torch.Tensor, d
     return _drive(_rows_ldlq_steps(W_rot, U, U_blks_inv, diag_w, spec_name, fused, gemm))
 
 
-_GEMM_ERR: Dict[str, torch.Tensor] = {}
+_GEMM_ERR: Dict[int, torch.Tensor] = {}
+
+
+def _device_index(device) -> int:
+    i = torch.device(device).index
+    return torch.cuda.current_device() if i is None else i
 
 
 def gemm_error_flag(device) -> torch.Tensor:
-    """The device int that the tensor-core GEMM sets when one of its pipeline waits runs out (one per device, shared by
+    """The device int that the tensor-core products set when one of their pipeline waits runs out (one per device, shared by
     all streams; cleared by check_gemm_errors)."""
-    key = str(torch.device(device))
+    key = _device_index(device)
     t = _GEMM_ERR.get(key)
     if t is None:
         t = torch.zeros(1, dtype=torch.int32, device=device)
@@ -447,12 +452,13 @@ def gemm_error_flag(device) -> torch.Tensor:
 
 
 def check_gemm_errors(device):
-    """Raises if a tensor-core GEMM on `device` reported a timed-out pipeline wait since the last check (a host
+    """Raises if a tensor-core product on `device` reported a timed-out pipeline wait since the last check (a host
     synchronisation: call it where the caller synchronises anyway)."""
-    t = _GEMM_ERR.get(str(torch.device(device)))
+    t = _GEMM_ERR.get(_device_index(device))
     if t is not None and int(t.item()) != 0:
         t.zero_()
-        raise RuntimeError("ltq_gemm_bf16_tn: a pipeline wait ran out; the LDLQ update of this call is not valid")
+        raise RuntimeError("a pipeline wait of a tensor-core product ran out (ltq_gemm_bf16_tn, its split forms, ltq_fp8_gemm or "
+                           "ltq_fp8_few): what the products on this device gave since the last check is not valid")
 
 
 def _scale_fit_reference(W_rot: torch.Tensor, cfg: dict):

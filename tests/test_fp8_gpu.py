@@ -297,6 +297,16 @@ def test_first_product_in_a_graph(M):
     fp8.check_errors(x.device)
 
 
+@pytest.mark.parametrize("device", ["cuda", "cuda:0"])
+def test_errors_are_found_however_the_device_is_named(device):
+    W = fp8.BlockWeight.quantize(torch.randn(64, 64, device="cuda:0"))
+    fp8.check_errors("cuda:0")
+    fp8._error_flag(W.device).fill_(1)  # as a wait that ran out does
+    with pytest.raises(RuntimeError, match="ltq_fp8_gemm"):
+        fp8.check_errors(device)
+    fp8.check_errors(device)  # reported once
+
+
 def test_second_derivatives_are_refused():
     g = gen(13)
     W = fp8.BlockWeight.quantize(torch.randn(40, 96, device="cuda", generator=g), backward=True)
