@@ -317,7 +317,8 @@ int ltq_distill_topk(const void* logits, int dtype, long long ld, const void* id
  * ltq_embed_lookup: out [n, D] = scale * table[tokens] (table [V, D], out of its dtype; tokens int64 when tok64, else
  *   int32; a token outside [0, V) reads as zeros).
  * ltq_embed_grad: out [V, D] (out_dtype) = scale * sum of the rows of dout [n, D] (dtype) whose token is the row, summed in
- *   fp32 in the order of the positions; accumulate = 1 adds to out instead (rows that no token names are not touched).
+ *   fp32, grouped by the rows' places among the sorted tokens (runs of at least 8 places, of a length that n and D give, each summed
+ *   in the order of the positions, then joined); accumulate = 1 adds to out instead (rows that no token names are not touched).
  *   Tokens outside [0, V) and `padding` (-1: none) take no gradient.  workspace: 256-byte aligned, at least
  *   ltq_embed_grad_workspace_bytes(n, D).  n <= 2^30, D <= 2^20.  Bit-identical from call to call.
  */

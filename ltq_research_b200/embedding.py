@@ -2,8 +2,8 @@
 
 * lookup       out[i] = scale * table[tokens[i]], rounded once to the table's type (one kernel, ltq_embed_lookup);
 * lookup_grad  grad[v] = scale * sum of dout[i] over the positions i with tokens[i] = v: the positions are sorted by token
-               and the runs summed in fp32 in their order, long runs split and joined (three launches, ltq_embed_grad).
-               The same bits at every call: no atomics on values.
+               and the runs summed in fp32, a run in groups that follow from its places in the sorted list (three launches,
+               ltq_embed_grad).  The same bits at every call with the same tokens: no atomics on values.
 
 A token outside [0, number of rows) reads as zeros and takes no gradient, as does the padding token in the gradient.
 There is no CPU path.

@@ -153,6 +153,42 @@ def test_grad_order_is_that_of_the_positions():
     assert (embedding.lookup_grad(tok, d, 2)[0] == 1.0).all()
 
 
+def grouped_sums(tok, d, V, chunk=8):
+    """The documented grouping, in fp32: chunks of the sorted list summed in order, a row's chunks joined in order, of nine chunks or
+    more in eight stretches of equally many."""
+    key, pos = torch.sort(tok, stable=True)
+    parts = {}
+    for at in range(len(tok)):
+        row = parts.setdefault(int(key[at]), {})
+        row[at // chunk] = row.get(at // chunk, torch.zeros(d.shape[1])) + d[pos[at]]
+
+    def total(xs):
+        s = torch.zeros(d.shape[1])
+        for x in xs:
+            s = s + x
+        return s
+    out = torch.zeros(V, d.shape[1])
+    for v, row in parts.items():
+        p = [row[c] for c in sorted(row)]
+        if len(p) > 8:
+            each = (len(p) + 7) // 8
+            p = [total(p[w * each:(w + 1) * each]) for w in range(8)]
+        out[v] = total(p)
+    return out
+
+
+@pytest.mark.parametrize("before", [0, 5, 6, 7])
+@pytest.mark.parametrize("n", [12, 64, 71, 72, 73, 200])
+def test_grad_grouping(before, n):
+    """Rows of one to many chunks that begin anywhere in a chunk, with values whose sum depends on the grouping."""
+    g = torch.Generator().manual_seed(n + before)
+    tok = torch.cat([torch.zeros(before, dtype=torch.int64), torch.ones(n, dtype=torch.int64), torch.full((3,), 2)])
+    tok = tok[torch.randperm(len(tok), generator=g)]
+    d = torch.randn(len(tok), 5, generator=g) * torch.exp2(torch.randint(-10, 25, (len(tok), 5), generator=g).float())
+    got = embedding.lookup_grad(tok.cuda(), d.cuda(), 3).cpu()
+    assert torch.equal(got, grouped_sums(tok, d, 3))
+
+
 def test_grad_padding_and_outside():
     g = gen(4)
     tok = torch.randint(-3, 55, (4, 100), device="cuda", generator=g)
