@@ -429,6 +429,27 @@ def test_second_derivatives_are_refused(upstream):
         torch.autograd.grad(g.square().sum() + a.square().sum(), a)
 
 
+@pytest.mark.parametrize("order", [0, 1])
+def test_output_beside_the_logits(order):
+    """Columns of one tensor: their rows alternate in memory and share nothing."""
+    T, V = 5, 1000
+    logits, idx, u, lse = make(T, V, 6, torch.bfloat16, seed=31)
+    buf = torch.zeros(T, 2 * V + 3, dtype=torch.bfloat16, device="cuda")
+    view, out = (buf[:, :V], buf[:, V:2 * V]) if order == 0 else (buf[:, V + 3:], buf[:, 3:V + 3])
+    view.copy_(logits)
+    got = distill.topk_loss_grad(view, idx, u, teacher_lse=lse, out=out)
+    assert torch.equal(view, logits)
+    check(logits, idx, u, lse, got=got)
+    for bad in (buf[:, 1:V + 1], buf[:, V - 1:2 * V - 1], buf[:, V + 4:]):
+        if bad.shape[1] == V and order == 0:
+            with pytest.raises(ValueError):
+                distill.topk_loss_grad(view, idx, u, teacher_lse=lse, out=bad)
+    with pytest.raises(ValueError):
+        distill.topk_loss_grad(view, idx, u, teacher_lse=lse, out=view[:1].expand(T, V))
+    with pytest.raises(ValueError):
+        distill.topk_loss_grad(view[:1], idx[:1], u[:1], out=buf[:1, 1:V + 1] if order == 0 else buf[:1, V:2 * V])
+
+
 def test_no_rows():
     loss, d = distill.topk_loss_grad(torch.empty(0, 9, device="cuda"), torch.empty(0, 2, dtype=torch.int64, device="cuda"),
                                      torch.empty(0, 2, device="cuda"))
