@@ -187,6 +187,21 @@ def written(t: torch.Tensor):
     torch.autograd.graph.increment_version(t)
 
 
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two 2-D tensors, each with rows that do not overlap, share memory."""
+    def span(t):
+        n = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+        return t.data_ptr(), t.data_ptr() + n * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    if a0 >= b1 or b0 >= a1:
+        return False
+    ld, cols_a, cols_b = a.stride(0) * a.element_size(), a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
+    if a.shape[0] <= 1 or b.shape[0] <= 1 or ld != b.stride(0) * b.element_size() or ld < cols_a or ld < cols_b:
+        return True
+    apart = (b0 - a0) % ld  # rows of one stride may lie beside each other: columns of a wider tensor
+    return not cols_a <= apart <= ld - cols_b
+
+
 def on_device(device: torch.device):
     """Context with `device` current, as a launch on its streams needs."""
     return _SAME if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)

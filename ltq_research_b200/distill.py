@@ -108,7 +108,7 @@ def _call(logits, idx, teacher, teacher_lse, weight, temperature, mode, stats=No
         else:
             dlogits = out
             same = out.data_ptr() == logits.data_ptr() and (T <= 1 or out.stride(0) == logits.stride(0))
-            if not same and _overlap(out, logits):
+            if not same and _lib.overlap(out, logits):
                 raise ValueError("distill: out may be the logits themselves, but may not overlap them otherwise")
         ld_d = _rows(dlogits, "out")
     with _lib.on_device(dev):
@@ -121,21 +121,6 @@ def _call(logits, idx, teacher, teacher_lse, weight, temperature, mode, stats=No
     if out is not None:
         _lib.written(out)
     return loss, stats, dlogits
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two tensors of one shape and type, each with rows that do not overlap, share memory."""
-    def span(t):
-        n = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
-        return t.data_ptr(), t.data_ptr() + n * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    if a0 >= b1 or b0 >= a1:
-        return False
-    ld, cols = a.stride(0) * a.element_size(), a.shape[1] * a.element_size()
-    if a.shape[0] <= 1 or a.stride(0) != b.stride(0) or ld < cols:
-        return True
-    apart = (b0 - a0) % ld  # rows of one stride may lie beside each other: columns of a wider tensor
-    return not cols <= apart <= ld - cols
 
 
 def topk_loss(logits: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor, *,

@@ -55,6 +55,8 @@ def lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
         out = torch.empty((*tokens.shape, D), dtype=table.dtype, device=dev)
     elif out.dtype != table.dtype or out.shape != (*tokens.shape, D) or not out.is_contiguous():
         raise ValueError("embedding: out must be contiguous, of the table's type and shape [*tokens.shape, D]")
+    elif _lib.overlap(out.view(-1, D), table):
+        raise ValueError("embedding: out may not overlap the table")
     with _lib.on_device(dev):
         rc = _lib.lib().ltq_embed_lookup(table.data_ptr(), code, ld, tok.data_ptr(), tok.dtype is torch.int64, tok.numel(), V, D,
                                          scale, out.data_ptr(), D, _lib.stream_ptr(dev))
@@ -95,6 +97,8 @@ def lookup_grad(tokens: torch.Tensor, dout: torch.Tensor, num_rows: int, scale: 
     elif out.shape != (num_rows, D):
         raise ValueError(f"embedding: out must be [{num_rows}, {D}]")
     ld_o = _row_stride(out, "out")
+    if given and _lib.overlap(out, d):
+        raise ValueError("embedding: out may not overlap dout")
     n = tok.numel()
     L = _lib.lib()
     ws = torch.empty(L.ltq_embed_grad_workspace_bytes(n, D), dtype=torch.uint8, device=dev)

@@ -315,6 +315,22 @@ def test_second_derivatives_are_refused():
         torch.autograd.grad(g.square().sum() + table.square().sum(), table)
 
 
+def test_outputs_that_overlap_an_input_are_refused():
+    """Rows are written while others are still read: a table or a gradient that the output overlaps would be read half written."""
+    buf = torch.randn(40, 24, device="cuda", generator=gen(13))
+    keep, tok = buf.clone(), torch.arange(10, device="cuda")
+    for f in (lambda: embedding.lookup(buf, tok, out=buf[:10]), lambda: embedding.lookup(buf[5:], tok, out=buf[2:12]),
+              lambda: embedding.lookup_grad(tok, buf[:10], 20, out=buf[5:25]),
+              lambda: embedding.lookup_grad(tok, buf[:10, :12], 10, out=buf[:10, 4:16], accumulate=True)):
+        with pytest.raises(ValueError, match="overlap"):
+            f()
+    assert torch.equal(buf, keep)
+    got = embedding.lookup_grad(tok, buf[:10, :12], 10, out=buf[:10, 12:])  # beside each other
+    check_grad(tok, keep[:10, :12], 10, got=got)
+    assert torch.equal(buf[:, :12], keep[:, :12])
+    embedding.lookup(buf[:5], torch.zeros(0, dtype=torch.int64, device="cuda"), out=buf[:0])
+
+
 def test_refusals():
     table = torch.zeros(10, 8, device="cuda")
     tok = torch.zeros(3, dtype=torch.int64, device="cuda")
