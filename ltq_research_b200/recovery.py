@@ -51,7 +51,7 @@ def score(table: torch.Tensor, tokens: torch.Tensor, body: Callable, head: fp8.B
         K = teacher.idx.shape[-1]
         loss, _ = distill.topk_loss(z, teacher.idx.reshape(-1, K), teacher.logits.reshape(-1, K),
                                     teacher_lse=None if teacher.lse is None else teacher.lse.reshape(-1),
-                                    weight=None if weight is None else weight.reshape(-1), temperature=temperature)
+                                    weight=None if weight is None else weight.reshape(-1).float(), temperature=temperature)
     return loss.view(tokens.shape)
 
 

@@ -80,6 +80,19 @@ def test_recovers():
     fp8.check_errors(t.device)
 
 
+@pytest.mark.parametrize("dtype", [torch.bool, torch.int64, torch.bfloat16])
+def test_weights_of_any_type(dtype):
+    """A mask as data loaders give it, to the step and to the score."""
+    table, body, head_w, tokens, teacher = setup(V=130, T=8)
+    head = fp8.BlockWeight.quantize(head_w, backward=True)
+    mask = (torch.arange(tokens.numel(), device="cuda") % 3 != 0).view(tokens.shape)
+    want = recovery.score(table, tokens, body, head, teacher, weight=mask.float())
+    got = recovery.score(table, tokens, body, head, teacher, weight=mask.to(dtype))
+    assert torch.equal(got, want) and not got[~mask].any()
+    loss = recovery.step(table.requires_grad_(), tokens, body, head, teacher, weight=mask.to(dtype))
+    assert abs(float(loss) - float(want.sum() / mask.sum())) < 1e-5 * float(loss) + 1e-6
+
+
 def test_table_must_train():
     table, body, head_w, tokens, teacher = setup(V=130, T=8)
     with pytest.raises(ValueError):
