@@ -113,6 +113,32 @@ def test_row_counts(T):
     check(logits, idx, u, lse)
 
 
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("T,V,ctas", [(50, 70000, 3), (38, 100003, 4), (30, 128256, 5), (25, 150001, 6), (22, 180000, 7), (19, 250000, 8)])
+def test_ctas_of_a_row(T, V, ctas, rest):
+    """Every number of CTAs that long 16-bit rows are cut into, beside the whole rows of the tests above, in place too."""
+    logits, idx, u, lse = make(T, V, 12, torch.bfloat16, seed=V, rest=rest)
+    loss, d = check(logits, idx, u, lse)
+    again = logits.clone()
+    distill.topk_loss_grad(again, idx, u, teacher_lse=lse, out=again)
+    assert torch.equal(again, d)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,off", [(400003, 0), (1 << 20, 0), ((1 << 20) - 3, 1)])
+def test_rows_longer_than_shared_memory(V, off, dtype):
+    """Slices that are held in part only (fp32 beyond about 390000 tokens), up to the longest rows; in place too."""
+    logits, idx, u, lse = make(3, V, 40, dtype, seed=V, pad=5)
+    buf = torch.zeros(3 * (V + 5) + 8, dtype=dtype, device="cuda")[off:off + 3 * (V + 5)].view(3, V + 5)[:, :V]
+    buf.copy_(logits)
+    idx[0, 0], idx[1, 0], idx[2, 1] = 0, V - 1, V // 2
+    loss, d = check(buf, idx, u, lse + 1.0)
+    d2 = distill.topk_grad(buf, idx, u, distill.topk_loss(buf, idx, u, teacher_lse=lse + 1.0)[1], teacher_lse=lse + 1.0)
+    check(buf, idx, u, lse + 1.0, got=(loss, d2))
+    distill.topk_loss_grad(buf, idx, u, teacher_lse=lse + 1.0, out=buf)
+    assert torch.equal(buf, d)
+
+
 @pytest.mark.parametrize("tau", [0.5, 2.0])
 def test_temperature_and_teacher_types(tau):
     logits, idx, u, lse = make(6, 777, 12, torch.bfloat16, seed=5, tau=tau)

@@ -214,6 +214,21 @@ def test_grad_accumulates(dtype):
     assert not embedding.lookup_grad(tok[:0], dout[:0], V).any()
 
 
+@pytest.mark.parametrize("n,V,D", [(8193, 500, 40), (20000, 30000, 264), (30000, 70, 130), (9000, 100000, 1040)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_grad_accumulates_many_positions(n, V, D, dtype):
+    """Beyond 8192 positions, with rows of one position and of many chunks, and rows that no token names."""
+    g = gen(n)
+    base = torch.randn(V, D, device="cuda", generator=g).to(dtype)
+    tok = (torch.rand(n, device="cuda", generator=g) ** 4 * V * 0.9).long()
+    dout = torch.randn(n, D, device="cuda", generator=g).to(dtype)
+    got = check_grad(tok, dout, V, scale=0.5, pad=3, base=base, dtype=dtype)
+    unnamed = torch.bincount(tok, minlength=V) == 0
+    unnamed[3] = True
+    assert bool((torch.bincount(tok, minlength=V) > 64).any()) and torch.equal(got[unnamed], base[unnamed])
+    assert torch.equal(got, embedding.lookup_grad(tok, dout, V, 0.5, 3, out=base.clone(), accumulate=True))
+
+
 @pytest.mark.parametrize("D,ld_d,ld_o,off", [(64, 72, 80, 0), (64, 65, 64, 0), (33, 40, 35, 1), (16, 16, 24, 3), (66, 68, 70, 2)])
 @pytest.mark.parametrize("dtype,out_dtype", [(torch.bfloat16, torch.float32), (torch.float32, torch.float16)])
 def test_grad_strides(D, ld_d, ld_o, off, dtype, out_dtype):

@@ -225,6 +225,57 @@ def test_long_sums(M, N, K):
     fp8.check_errors(x.device)
 
 
+# one row tile of 128 and several, rows of both widths of the streaming kernel, K cut over 1, 2, 4 and 8 CTAs, odd numbers of
+# blocks and widths; with 17 rows and more only weights of at least 18817 rows go there, and up to K = 4864
+STREAMED = [(1, 19000, 300), (3, 5000, 1100), (9, 20001, 130), (16, 38000, 1000), (1, 128256, 256), (2, 300, 9000), (16, 2100, 3333),
+            (17, 18817, 128), (17, 19072, 129), (20, 18950, 1000), (24, 25000, 2048), (31, 40009, 515), (32, 18944, 4864),
+            (32, 20000, 4000), (19, 18820, 4865), (33, 19000, 300)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", STREAMED)
+def test_streamed_weights(M, N, K, dtype):
+    g = gen(M + N + K)
+    W = fp8.BlockWeight.quantize(spread(g, N, K, torch.bfloat16) * 0.05)
+    x = torch.randn(M, K, device="cuda", generator=g).to(dtype)
+    y = fp8.linear(x, W)
+    check(x, W, y)
+    assert torch.equal(y, fp8.linear(x, W))
+    fp8.check_errors(x.device)
+
+
+@pytest.mark.parametrize("M", [1, 17, 32])
+def test_streamed_rows_of_any_stride_and_bad_values(M):
+    g = gen(15)
+    W = fp8.BlockWeight.quantize(torch.randn(19000, 400, device="cuda", generator=g))
+    x = torch.randn(M, 411, device="cuda", generator=g).bfloat16()[:, 3:403]
+    check(x, W, fp8.linear(x, W))
+    x[M // 2, 390] = float("nan")
+    y = fp8.linear(x, W)
+    bad = torch.arange(M, device="cuda") == M // 2
+    assert torch.isnan(y[bad]).all() and torch.isfinite(y[~bad]).all()
+
+
+@pytest.mark.parametrize("kind", ["random", "positive", "one large"])
+@pytest.mark.parametrize("M,N,K", [(8, 512, 128), (8, 512, 4096), (24, 20000, 128), (24, 20000, 4096), (200, 512, 1024), (200, 512, 16384)])
+def test_sums_are_those_of_fp32(M, N, K, kind):
+    """The tensor cores' sums of 32 products and what was summed before lose at most 2^-24 of the largest term for each of the 33, and
+    a block more is one rounding more: (33 + K / 128 + 4) 2^-24 of the sum of magnitudes.  (Measured: 8 at K = 128 and one product far
+    above the others, 14 at K = 16384 and all of one sign.)"""
+    g = gen(M + K)
+    w, x = torch.randn(N, K, device="cuda", generator=g), torch.randn(M, K, device="cuda", generator=g)
+    if kind == "positive":
+        w, x = w.abs(), x.abs()
+    if kind == "one large":
+        x[:, ::128] *= 300
+        w[:, ::128] *= 30
+    W = fp8.BlockWeight.quantize(w)
+    xq, xs = plain_quant(x, 1)
+    a, b = xq * expand(xs, 1, M, K), W.q[:, :K].view(torch.float8_e4m3fn).double() * expand(W.s, 128, N, K)
+    err = (fp8.linear(x, W, dtype=torch.float32).double() - a @ b.T).abs()
+    assert bool((err <= (33 + K // 128 + 4) * 2.0 ** -24 * (a.abs() @ b.abs().T)).all())
+
+
 @pytest.mark.parametrize("M,N,K", [(60, 512, 640), (300, 256, 4000), (700, 1100, 256)])
 def test_calls_one_after_another(M, N, K):
     """Calls without a pause between them, in buffers that pass from one to the next, alone and from a graph: each has the
