@@ -387,7 +387,7 @@ __device__ __forceinline__ void exact_row(const DistillParams& p, long long row)
 // works on the slots alone, while the others are in their first pass.
 // Bound: the logits read once and the gradient written once; an exponential an element and pass (16 a clock and SM) and the
 // instructions around it take 60 to 70 % of that time.  4096 x 128256 bf16 with the gradient, a quarter
-// of the rows of weight 0: 384 us, 4.8 TB/s; 2048 rows, the loss alone: 96 us, 5.5 TB/s.
+// of the rows of weight 0: 385 us, 4.8 TB/s; 2048 rows, the loss alone: 98 us, 5.4 TB/s.
 template <typename T, bool GRAD, bool REST>
 __global__ void __launch_bounds__(D_THREADS + 32, REST && !GRAD ? 5 : 0) distill_rows_kernel(const __grid_constant__ DistillParams p)
 {

@@ -10,7 +10,7 @@
 //   warps 2 .. 5  epilogue: lane = weight row; each block's sums times sw sx added to fp32 registers
 //   warps 1 ..    first quantize x
 //
-// Bound by the weight's bytes where it is large: 1 x 128256 x 2048 48 us, 5.5 TB/s; 24 rows 52 us, 5.1 TB/s: all CTAs read x
+// Bound by the weight's bytes where it is large: 1 x 128256 x 2048 48 us, 5.5 TB/s; 24 rows 51 us, 5.2 TB/s: all CTAs read x
 // from L2 at the start, and the first MMAs wait for it longer than the ring of weight blocks lasts.  A small
 // weight is bound by the chain launch, first loads, MMAs, epilogue: 1 x 8192 x 2048 12 us, where the bytes alone would take 3.
 //
@@ -331,7 +331,7 @@ struct FewPlan {
 // The quantized x of a CTA's share of K stays in its shared memory beside at least four weight blocks.  K is cut (2, 4 or 8 ways)
 // where that takes it, and further while the CTAs all run at once (two an SM of at most 16 rows) with four blocks of K or more
 // each.  False, for the other kernels, where more CTAs than that would each have to quantize their x, and for more than 32 rows:
-// at 64 (one block a buffer, 88 us for 128256 x 2048) the 256-row tiles behind a separate quantization are as fast (83 us).
+// at 64 (one block a buffer, 88 us for 128256 x 2048) the 256-row tiles behind a separate quantization are faster (70 us a call).
 bool plan_few(int M, int N, int K, int sms, FewPlan& p)
 {
     if (M < 1 || M > F_ROWS || N < 1 || K < 1 || sms < 2) return false;

@@ -19,13 +19,13 @@
 //
 // What bounds it: a block's MMAs take 512 cycles a pair, and the chain sum complete -> read (two rounds of 64 columns, for which
 // the registers beside the sums suffice) -> buffer handed back -> next MMAs about twice that, over two buffers.  8192 x 8192 x
-// 4096: 240 us, 2290 TFLOP/s (the MMAs alone, without epilogue, 160 us; a 256 x 128 tile with four buffers 290 us, for each hand-over
-// costs the issuing warp the same).
+// 4096: 267 us, 2060 TFLOP/s in a single launch (the MMAs alone, without epilogue, 160 us; a 256 x 128 tile with four buffers 290 us or
+// more, for each hand-over costs the issuing warp the same).
 //
 // Pairs walk the tiles (rows first, so that neighbours share B in L2).  The tiles that are left after the last full round are cut
 // along K into one equal share for each pair: as many slices of each tile as there are pairs for, and the rest of K of all tiles, cut
 // across tiles, for the pairs that remain.  So all tiles' slices run through the same K at the same time and a block of A or B is
-// read from memory once and by the other tiles from L2: 1003 x 2048 x 128256 249 us and 0.5 GB of reads, where shares that follow one
+// read from memory once and by the other tiles from L2: 1003 x 2048 x 128256 250 us and 0.5 GB of reads, where shares that follow one
 // another through the tiles took 266 us and 1.5 GB.  The parts go to a workspace and join_parts_kernel adds them in the order of K.  Every wait is bounded: when one runs out
 // *err is set, the role stops and the CTAs still meet at their last barrier.
 #include <algorithm>
@@ -303,7 +303,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(W_THREADS, 1)
             for (int j = 0; j < 128; j++) acc[j] = 0.f;
             // sa of W_AHEAD blocks, and of as many more on their way: L2 answers later than several blocks take while the
             // operands stream.  sb comes for 32 blocks at a time, a lane each.  The loads go past L1, whose fills would take
-            // shared-memory cycles from the MMAs' operands (8192 x 8192 x 4096: 265 us with them, 242 without).
+            // shared-memory cycles from the MMAs' operands (23 us of 8192 x 8192 x 4096).
             float sa[W_AHEAD], na[W_AHEAD], sb32 = 0.f, nb32;
             auto fetch = [&](int k) {
 #pragma unroll

@@ -41,8 +41,8 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, int* err
 }
 // The same for a whole warp, with one answer for all of its lanes: a phase may end between two lanes' last polls, and lanes that
 // went different ways would wait without limit at the next instruction of the whole warp (shfl, elect, tcgen05.ld).  A vote a poll
-// keeps the loop uniform; 8192 x 8192 x 4096 in 8 bits back to back: 311 us, 308 with lanes that poll each for themselves, 366 with
-// these joined after the loop (the epilogue spills then).
+// keeps the loop uniform; 8192 x 8192 x 4096 in 8 bits: 267 us (311 back to back), 257 (308) with lanes that poll each for themselves;
+// 366 back to back with these joined after the loop (the epilogue spills then).
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* b, uint32_t parity, int* err, uint32_t limit = GEMM_WAIT_LIMIT)
 {
     for (uint32_t i = 0; i < limit; i++)

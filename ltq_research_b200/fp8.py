@@ -1,5 +1,5 @@
-"""Products with weights held in 8-bit floating point (e4m3) under one scale per 128 x 128 block — the form of 8-bit
-checkpoints, and a comparison format beside the trellis formats (as the int8 rings are for the row tables).
+"""Products with weights held in 8-bit floating point (e4m3) under one scale per 128 x 128 block, the form of 8-bit
+checkpoints.
 
 * quantize_blocks(w) / quantize_rows(x): e4m3 values and fp32 scales max|.| / 448 (at least 2^-126), per 128 x 128 block of a
   weight, per row and 128 columns of an activation; a block that holds a NaN or an infinity becomes NaN.
